@@ -19,6 +19,8 @@ void append_attn_resources(std::string& out);
 void append_select_resources(std::string& out);
 void append_gather_resources(std::string& out);
 void append_snap_resources(std::string& out);
+void append_decode_resources(std::string& out);
+void append_insert_resources(std::string& out);
 
 // Device address of fe_prefill_static's workspace on the device of `stream` (fe_static.hip).
 hipError_t static_scratch(hipStream_t stream, float** out);

@@ -8,6 +8,7 @@ import json
 
 from .prefill import prefill, evict, select_tokens
 from .cache import gather_tokens
+from .decode import DecodeCache, decode_attention, insert_tokens, replay_path
 
 
 def kernel_resources():
@@ -23,4 +24,5 @@ def kernel_resources():
     return json.loads(buf.value.decode())
 
 
-__all__ = ["prefill", "evict", "select_tokens", "gather_tokens", "kernel_resources"]
+__all__ = ["prefill", "evict", "select_tokens", "gather_tokens", "decode_attention", "replay_path", "insert_tokens",
+           "DecodeCache", "kernel_resources"]

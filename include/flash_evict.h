@@ -211,6 +211,75 @@ int fe_snap_scores(const void* q, const void* k, float* scores, int64_t B, int64
                    void* hip_stream);
 
 /*
+ * Decoding over a bounded KV cache (no counterpart in the reference, whose decode cache only
+ * grows: quality_adapter.py:116-136). One layer's cache is k_cache/v_cache [B,Hkv,C,D] with
+ * length [B,Hkv] int32 rows in use (read as clamped to [0, C]), and, per slot, FP32 importance,
+ * int32 position and optionally the value's L1 norm, in rows of `*_stride` elements.
+ *
+ * fe_decode_attention: T new tokens (1 <= T <= 256; q [B,Hq,T,D], k/v [B,Hkv,T,D], any element
+ * strides, not in the cache yet) attend over the cache's rows and over the new rows u with
+ * tree[t,u] != 0 ([T,T] bytes, one for all batch rows or one each at tree_batch_stride; NULL:
+ * u <= t).
+ *   out[b,h,t,:] = softmax(scale * q.key) @ value  (contiguous [B,Hq,T,D]; P rounded to the input
+ *                  dtype before the product, FP32 accumulation; zeros where nothing is visible)
+ *   lse[b,h,t]   = log sum exp(scale * q.key)      (contiguous [B,Hq,T]; -inf there)
+ * With `importance` (all T tokens stay, w_t = exp(-recency_decay * (T-1-t))), for slots s < length:
+ *   importance_out[b,j,s] = importance[b,j,s] * exp(-recency_decay * T)
+ *                           + value_norm[b,j,s] * sum_{g,t} w_t p[g,t,s]
+ *   new_importance[b,j,u] = ||v[b,j,u,:]||_1 * sum_{g,t} w_t p[g,t,u]   (contiguous [B,Hkv,T])
+ * Both without their norm when value_norm is NULL. importance_out may be importance; slots from
+ * length on are left as they were. A hidden new row never reaches a query, whatever it holds.
+ * workspace: at least fe_decode_workspace_bytes(...) bytes, 16-byte aligned, not shared by calls
+ * that overlap.
+ */
+size_t fe_decode_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t C, int64_t D);
+int fe_decode_attention(const void* q, const void* k, const void* v, const void* k_cache, const void* v_cache,
+                        const int32_t* length, const uint8_t* tree, int64_t tree_batch_stride, void* out, float* lse,
+                        const float* importance, int64_t importance_stride, const float* value_norm,
+                        int64_t value_norm_stride, float* importance_out, int64_t importance_out_stride,
+                        float* new_importance, int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t C, int64_t D,
+                        const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                        const int64_t* k_cache_strides, const int64_t* v_cache_strides, int dtype, float scale,
+                        float recency_decay, void* workspace, size_t workspace_bytes, void* hip_stream);
+
+/*
+ * The importance of fe_decode_attention for the accepted path of a drafted tree alone. path [B,A]
+ * int32: nodes of the tree from the root on; a row's path ends before its first entry outside
+ * [0, T) (A_b nodes). Row i is query path[b,i] with its lse from fe_decode_attention; it sees the
+ * cache and the path's nodes up to its own. NULL: all T tokens in order (A == T).
+ * new_importance: contiguous [B,Hkv,A], zeros from A_b on. No workspace.
+ */
+int fe_replay_path(const void* q, const void* k, const void* v, const void* k_cache, const int32_t* length,
+                   const float* lse, const int32_t* path, const float* importance, int64_t importance_stride,
+                   const float* value_norm, int64_t value_norm_stride, float* importance_out,
+                   int64_t importance_out_stride, float* new_importance, int64_t B, int64_t Hq, int64_t Hkv,
+                   int64_t T, int64_t A, int64_t C, int64_t D, const int64_t* q_strides, const int64_t* k_strides,
+                   const int64_t* v_strides, const int64_t* k_cache_strides, int dtype, float scale,
+                   float recency_decay, void* hip_stream);
+
+/*
+ * Insertion of new tokens into the cache and eviction of the rows of least importance, in place.
+ * Candidates of (b,j): the length[b,j] cache rows, then the new rows (all T of k/v [B,Hkv,T,D], or
+ * the nodes of path[b] as above) as if appended to them, with positions seen[b,j], seen[b,j]+1, ...
+ * and importance new_importance [B,Hkv,A] (NULL: 0). F = min(candidates, budget) stay: the rows of
+ * the newest `recent` positions (should there be more, those at the lowest slots), then by
+ * importance (NaN above every number, -0 equal to 0), equal ones by slot. Of those, rows below slot F stay in place, and the i-th one past it goes to the
+ * i-th slot below F that was vacated. Then length = F and seen += the path's nodes; slots from F
+ * on are left as they were. value_norm may be NULL; otherwise new rows get the L1 norm of their
+ * value. T may be 0 (k and v NULL): an eviction to `budget`. 1 <= budget <= C, recent <= budget.
+ * k and v must not overlap the cache. workspace: at least fe_insert_workspace_bytes(...) bytes
+ * (may be NULL when that is 0).
+ */
+size_t fe_insert_workspace_bytes(int64_t B, int64_t Hkv, int64_t A, int64_t C, int64_t budget);
+int fe_insert_tokens(const void* k, const void* v, void* k_cache, void* v_cache, float* importance,
+                     int64_t importance_stride, int32_t* position, int64_t position_stride, float* value_norm,
+                     int64_t value_norm_stride, int32_t* length, int32_t* seen, const float* new_importance,
+                     const int32_t* path, int64_t B, int64_t Hkv, int64_t T, int64_t A, int64_t C, int64_t D,
+                     int64_t budget, int64_t recent, const int64_t* k_strides, const int64_t* v_strides,
+                     const int64_t* k_cache_strides, const int64_t* v_cache_strides, int dtype, void* workspace,
+                     size_t workspace_bytes, void* hip_stream);
+
+/*
  * Timing of the attention + importance kernels alone (the fused kernel, or the attention
  * and replay kernels of the split schedule): when enabled, fe_prefill / fe_prefill_ws
  * record a HIP event pair around them on the caller's stream. The switch and the record
