@@ -51,7 +51,7 @@ _SIGNATURES = {
     "fe_snap_scores_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i64, _i64, _i64]),
     "fe_snap_scores": (ctypes.c_int, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _I64P, _I64P, ctypes.c_int,
                                       _i64, _vp, ctypes.c_size_t, _vp]),
-    "fe_decode_workspace_bytes": (ctypes.c_size_t, [_i64] * 6),
+    "fe_decode_workspace_bytes": (ctypes.c_size_t, [_i64] * 6 + [ctypes.c_int]),
     "fe_decode_attention": (ctypes.c_int, [_vp] * 7 + [_i64, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp] + [_i64] * 6 +
                             [_I64P] * 5 + [ctypes.c_int, ctypes.c_float, ctypes.c_float, _vp, ctypes.c_size_t, _vp]),
     "fe_replay_path": (ctypes.c_int, [_vp] * 8 + [_i64, _vp, _i64, _vp, _i64, _vp] + [_i64] * 7 + [_I64P] * 4 +

@@ -144,7 +144,7 @@ def decode_attention(q, k, v, k_cache, v_cache, length, *, tree=None, scale=None
     out = torch.empty((b, hq, t, d), dtype=dtype, device=device)
     lse = torch.empty((b, hq, t), dtype=torch.float32, device=device)
     L = _lib.lib()
-    ws_bytes = L.fe_decode_workspace_bytes(b, hq, hk, t, c, d)
+    ws_bytes = L.fe_decode_workspace_bytes(b, hq, hk, t, c, d, importance is not None)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
     with _lib.on_device(device):
         rc = L.fe_decode_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),

@@ -229,10 +229,10 @@ int fe_snap_scores(const void* q, const void* k, float* scores, int64_t B, int64
  *   new_importance[b,j,u] = ||v[b,j,u,:]||_1 * sum_{g,t} w_t p[g,t,u]   (contiguous [B,Hkv,T])
  * Both without their norm when value_norm is NULL. importance_out may be importance; slots from
  * length on are left as they were. A hidden new row never reaches a query, whatever it holds.
- * workspace: at least fe_decode_workspace_bytes(...) bytes, 16-byte aligned, not shared by calls
- * that overlap.
+ * workspace: at least fe_decode_workspace_bytes(...) bytes (weights != 0: with importance),
+ * 16-byte aligned, not shared by calls that overlap.
  */
-size_t fe_decode_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t C, int64_t D);
+size_t fe_decode_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t C, int64_t D, int weights);
 int fe_decode_attention(const void* q, const void* k, const void* v, const void* k_cache, const void* v_cache,
                         const int32_t* length, const uint8_t* tree, int64_t tree_batch_stride, void* out, float* lse,
                         const float* importance, int64_t importance_stride, const float* value_norm,

@@ -148,7 +148,7 @@ ST = (ctypes.c_int64 * 4)(1, 1, 1, 1)
 def _attend_c(L, B=1, Hq=4, Hkv=2, T=3, C=8, D=16, dtype=1, scale=1., decay=0., ws=None, ws_bytes=None, imp=None, imp_st=8,
               length=P, st=ST, out=P, tree_st=0):
     if ws_bytes is None:
-        ws_bytes = L.fe_decode_workspace_bytes(B, Hq, Hkv, T, C, D) - 1      # every call here is refused
+        ws_bytes = L.fe_decode_workspace_bytes(B, Hq, Hkv, T, C, D, imp is not None) - 1      # every call here is refused
     return L.fe_decode_attention(P, P, P, P, P, length, None, tree_st, out, P, imp, imp_st, None, 0, P, 8, P, B, Hq, Hkv, T, C, D,
                                  st, st, st, st, st, dtype, scale, decay, ws, ws_bytes, None)
 
@@ -198,8 +198,12 @@ def test_c_insert_tokens_refuses():
 
 def test_workspace_sizes():
     L = _lib.lib()
-    assert L.fe_decode_workspace_bytes(1, 3, 2, 1, 8, 16) >= 0 and L.fe_decode_workspace_bytes(0, 4, 2, 1, 8, 16) == 0
-    assert L.fe_decode_workspace_bytes(1 << 40, 1 << 40, 1 << 40, 256, 1 << 40, 256) == 0
-    # at most two rounds of blocks' partials whatever the cache's length
-    assert L.fe_decode_workspace_bytes(1, 32, 8, 1, 1 << 30, 128) <= 32 << 20
+    assert L.fe_decode_workspace_bytes(1, 3, 2, 1, 8, 16, 0) >= 0 and L.fe_decode_workspace_bytes(0, 4, 2, 1, 8, 16, 0) == 0
+    assert L.fe_decode_workspace_bytes(1 << 40, 1 << 40, 1 << 40, 256, 1 << 40, 256, 1) == 0
+    # partials of as many blocks as the card holds, whatever the cache's length; with weights, few rows' logits
+    assert L.fe_decode_workspace_bytes(1, 32, 8, 1, 1 << 30, 128, 0) <= 16 << 20
+    logits = 4 * 32 * 8 * 4 * (131072 // 32 + 1)
+    size = [L.fe_decode_workspace_bytes(1, 32, 8, 1, 131072, 128, w) for w in (0, 1)]
+    assert logits <= size[1] - size[0] <= logits + 256
+    assert L.fe_decode_workspace_bytes(1, 32, 8, 32, 131072, 128, 1) == L.fe_decode_workspace_bytes(1, 32, 8, 32, 131072, 128, 0)
     assert L.fe_insert_workspace_bytes(1, 8, 0, 64, 64) == 0
