@@ -12,6 +12,8 @@
 // Counting recency back from the newest token, a prompt's importance continued chunk by chunk is the
 // importance of the whole (fe_prefill's).
 //
+//   decode_few_kernel      up to 16 query rows r = g * T + t of a group, the steps of one token: each wave takes 32 keys at
+//                          a time for all of them; the code of a call is short, as most of a small call is its reading
 //   decode_rows_kernel     up to 32 query rows r = g * T + t of a group: each wave takes 32 keys at a time for all of
 //                          them, S^T = K Q^T and O^T = V^T P^T on MFMA, with the rows' running maximum and sum
 //   decode_wide_kernel     more rows: each wave holds 32 of them, the block's waves share tiles of 64 keys in LDS
@@ -21,13 +23,16 @@
 //                          key's sum over the rows is in-lane: p = exp2(x log2e - bias), the bias holding lse and w
 //
 // Lengths are known on the device only, and differ from head to head, so a launch has as many blocks as the card
-// holds at once, and each takes an equal share of all tiles of all heads, in order (dec_share).
+// holds at once, and each takes an equal share of all tiles of all heads, in order (dec_share); the few-rows kernel's
+// blocks divide each head's tiles instead, which takes less code.
 #include <math.h>
+#include <stddef.h>
 #include <algorithm>
 #include <string>
 
 #include "fe_attn.h"
 #include "fe_internal.h"
+#include "fe_radix.h"
 #include "../../include/flash_evict.h"
 
 namespace fe {
@@ -41,37 +46,114 @@ constexpr int kDecMaxTokens = 256;   // new tokens of a call
 // Rows of a group up to which the attention leaves its logits for the importance: 8 bytes a row and key, written and
 // read, against the 2 D of reading K again.
 constexpr int kDecLogitRows = 16;
+constexpr int kDecJoinBlocks = 2048;   // blocks that share the importance of all heads
 
+// Pointers to global memory, said to be: a pointer that the compiler loses sight of (dec_hold) would be read with flat
+// instructions, which wait for LDS too.
+#define FE_GLOBAL __attribute__((address_space(1)))
+typedef const FE_GLOBAL u16* DecIn;
+typedef FE_GLOBAL float* DecF32;
+typedef const FE_GLOBAL float* DecF32In;
+typedef const FE_GLOBAL int* DecI32In;
+typedef FE_GLOBAL u32x4* DecVec;
+
+// In the order of their use, so that what a kernel needs at once lies together (dec_hold).
 struct DecArgs {
-  const u16* q;
-  const u16* k;            // new rows
-  const u16* v;
-  const u16* kc;           // cache
-  const u16* vc;
-  const int* length;       // [B * Hkv]
-  const unsigned char* tree;   // [T, T] or [B, T, T], or null: causal
-  const int* path;         // [B, A] nodes of the accepted path, or null: all T
-  u16* out;                // [B, Hq, T, D]
-  float* lse;              // [B, Hq, T]
-  const float* lse_in;     // replay
-  const float* imp;        // [B * Hkv] rows of imp_stride
-  const float* norm;
-  float* imp_out;
-  float* new_imp;          // [B * Hkv, A]
-  float* part_o;           // [slot][32 * RW][DP]: normalised partial outputs
-  float* part_ml;          // [slot][2][32 * RW]: maximum (log2 units), sum
-  int* seg;                // [segment][2]: first and last slot
-  float* logits;           // [B * Hkv][tile][R][32] in log2 units, or null
-  long long qs[4], ks[4], vs[4], kcs[4], vcs[4];
-  long long imp_stride, norm_stride, impo_stride, tree_stride;
-  int T, C, D, G, Hkv, BH, A;
-  int R, RB, RW;           // rows of a group; segments of a group, 32-row tiles of a segment
+  // replay
+  DecF32In imp;            // [B * Hkv] rows of imp_stride
+  DecF32In norm;
+  DecF32 imp_out;
+  DecF32 new_imp;          // [B * Hkv, A]
+  DecF32In lse_in;
+  DecI32In path;           // [B, A] nodes of the accepted path, or null: all T
+  long long imp_stride, norm_stride, impo_stride;
+  int A;
+  float decay_log2;
+  // all
+  DecIn q, k, v, kc;       // queries, new rows, the cache's K
+  DecI32In length;         // [B * Hkv]
+  long long qs[3], ks[3], vs[3], kcs[3];   // strides of batch, head, row
+  int T, C, D, G, Hkv, BH;
   int nb;                  // blocks that share the tiles
-  int max_tiles;           // tiles of 32 keys of a full cache and T new rows
-  int join_blocks, join_split;   // decode_join_kernel: blocks of the output; 32-lane groups that share a row
   u32 qand, qxor;          // Q's sign for a negative scale, Q's zeros for a zero one
-  float scale_log2, decay_log2;
+  float scale_log2;
+  // attention
+  DecIn vc;
+  const FE_GLOBAL unsigned char* tree;   // [T, T] or [B, T, T], or null: causal
+  DecF32 part_o;           // [slot][32 * RW][DP]: normalised partial outputs
+  DecF32 part_ml;          // [slot][2][32 * RW]: maximum (log2 units), sum
+  FE_GLOBAL int* seg;      // [segment][2]: first and last slot
+  DecF32 logits;           // [B * Hkv][tile][R][32] in log2 units, or null
+  long long vcs[3], tree_stride;
+  int R, RB, RW;           // rows of a group; segments of a group, 32-row tiles of a segment
+  int max_tiles;           // tiles of 32 keys of a full cache and T new rows
+  // element loads
+  long long qc, kcc, vcc, knc, vnc;      // channel strides of q, the cache and the new rows
+  int pad[4];
 };
+constexpr int kDecReplayArgs = 0, kDecAttnArgs = 80;   // offsets of what the kernels hold
+static_assert(offsetof(DecArgs, q) == kDecAttnArgs && offsetof(DecArgs, qc) <= kDecAttnArgs + 5 * 64 && offsetof(DecArgs, vc) <= 5 * 64 &&
+                  sizeof(DecArgs) >= kDecAttnArgs + 5 * 64, "argument windows");
+
+struct DecFewArgs {
+  DecIn q, k, v, kc, vc;
+  DecI32In length;
+  const FE_GLOBAL unsigned char* tree;
+  DecF32 part_o;           // [B * Hkv * S][16][DP]
+  DecF32 part_ml;          // [B * Hkv * S][2][16]
+  DecF32 logits;           // or null
+  long long qb, qh, qn, kb, kh, vb, vh, kcb, kch, vcb, vch, tree_stride;   // strides of batch, head, (q) row
+  u32 kn, vn, kcn, vcn;    // row strides
+  int T, C, D, R, S, max_tiles;
+  u32 qand, qxor;
+  float scale_log2;
+  int pad[9];
+};
+static_assert(offsetof(DecFewArgs, pad) <= 4 * 64 && sizeof(DecFewArgs) >= 4 * 64, "argument window");
+
+struct DecJoinArgs {
+  DecF32In part_o, part_ml, logits;
+  DecI32In seg, length;
+  FE_GLOBAL u16* out;      // [B, Hq, T, D]
+  DecF32 lse;              // [B, Hq, T]
+  DecF32In imp, norm;
+  DecF32 imp_out, new_imp;
+  DecIn v;
+  long long imp_stride, norm_stride, impo_stride, vs[3], vnc;
+  int T, C, D, G, Hkv, BH, R, RB, RS, max_tiles;   // RS: rows of a slot
+  int S;                   // splits of a head (decode_few_kernel), or 0: slots by `seg`
+  int out_blocks, split;   // blocks of the output; 32-lane groups that share a row
+  int per_head;            // blocks of a head's importance
+  float decay_log2;
+  int pad[16];
+};
+static_assert(offsetof(DecJoinArgs, pad) <= 4 * 64 && sizeof(DecJoinArgs) >= 4 * 64, "argument window");
+
+// The kernel's arguments, NV * 64 bytes of them from byte FIRST on read at once and kept in registers. Left to the
+// compiler, each is read where it is first used and again wherever that saves registers; arguments lie in host memory,
+// and a wave waited some 2000 cycles for every such read (step of one token over 1024 rows: 15.4 us of which 10 so).
+template <int FIRST, int NV, typename A>
+__device__ __forceinline__ A dec_hold(const A& arg) {
+  static_assert(sizeof(A) >= FIRST + NV * 64, "argument window");
+  A a = arg;
+  typedef u32 u32x16 __attribute__((ext_vector_type(16), aligned(4)));
+  typedef const __attribute__((address_space(4))) u32x16* args_ptr;
+  const args_ptr p = (args_ptr)((const __attribute__((address_space(4))) char*)__builtin_amdgcn_kernarg_segment_ptr() + FIRST);
+  u32x16 v[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) v[i] = p[i];
+  if constexpr (NV == 5) asm volatile("" : "+s"(v[0]), "+s"(v[1]), "+s"(v[2]), "+s"(v[3]), "+s"(v[4]));
+  if constexpr (NV == 4) asm volatile("" : "+s"(v[0]), "+s"(v[1]), "+s"(v[2]), "+s"(v[3]));
+  // from here on word by word: a spilled register of 16 words would come back whole for each word of it
+  u32 w[NV * 16];
+#pragma unroll
+  for (int i = 0; i < NV * 16; ++i) {
+    w[i] = v[i / 16][i % 16];
+    asm volatile("" : "+s"(w[i]));
+  }
+  __builtin_memcpy((char*)&a + FIRST, w, NV * 64);
+  return a;
+}
 
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kDecNegInf = -__builtin_huge_valf();
@@ -123,9 +205,15 @@ __device__ __forceinline__ u32x4 dec_vfrag(unsigned char* vt, int r0, int dt) {
 }
 
 // 16 bytes of a row: channels 8 ch .. 8 ch + 7, zeros past D.
-template <int VEC>
-__device__ __forceinline__ u32x4 dec_load8(const u16* row, long long cs, int ch, int D) {
-  return load8(row, cs, 8 * ch, D, VEC);
+__device__ __forceinline__ u32x4 dec_load8(DecIn row, long long cs, int ch, int D) {
+  u32 w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int da = 8 * ch + 2 * i, db = da + 1;
+    const u32 lo = da < D ? (u32)row[da * cs] : 0u, hi = db < D ? (u32)row[db * cs] : 0u;
+    w[i] = lo | (hi << 16);
+  }
+  return (u32x4){w[0], w[1], w[2], w[3]};
 }
 
 // Whether one of eight 16-bit values is an infinity or a NaN.
@@ -147,68 +235,66 @@ __device__ __forceinline__ bool dec_nonfinite<F16>(u32x4 x) { return dec_exponen
 template <int KT>
 __device__ __forceinline__ int dec_tiles(int n, int fresh) { return (n + KT - 1) / KT + (fresh + KT - 1) / KT; }
 
-__device__ __forceinline__ long long dec_lane64(long long x, int lane) {
-  const u32 lo = __builtin_amdgcn_readlane((u32)x, lane), hi = __builtin_amdgcn_readlane((u32)((unsigned long long)x >> 32), lane);
-  return (long long)(((unsigned long long)hi << 32) | lo);
-}
-
-// Block blockIdx.x's share [pos, hi) of the W tiles of all segments, numbered head by head and, within a head,
-// segment by segment of all its tiles; the head that holds pos and the head's first tile. Only as many blocks share
-// as there are PER tiles for each, so no block between two others is without a tile. Every wave computes it.
+// Block blockIdx.x's share [pos, hi) of the tiles of all segments, numbered head by head and, within a head, segment
+// by segment of all its tiles; the head that holds pos and the head's first tile. Only as many blocks share as there
+// are PER tiles for each, so no block between two others is without a tile. Every wave computes it. (The launch
+// keeps the number of tiles below 2^31.)
 struct DecShare {
-  long long pos, hi, base;
-  int bh;
+  int pos, hi, base, bh;
+  int len;                 // lane i: rows of head (bh & ~63) + i
 };
 template <int KT, int PER>
 __device__ __forceinline__ DecShare dec_share(const DecArgs& a, int segs, int fresh) {
   const int lane = threadIdx.x & 63;
-  long long W = 0, first = 0;
-  for (int c0 = 0; c0 < a.BH; c0 += 64) {
-    long long x = c0 + lane < a.BH ? (long long)segs * dec_tiles<KT>(dec_len(a, c0 + lane), fresh) : 0;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const long long y = __shfl_up(x, d);
-      if (lane >= d) x += y;
-    }
-    if (c0 == 0) first = x;
-    W += dec_lane64(x, 63);
-  }
+  auto tiles = [&](int len, int bh) { return bh < a.BH ? segs * dec_tiles<KT>(len, fresh) : 0; };
+  auto length = [&](int bh) { return bh < a.BH ? dec_len(a, bh) : 0; };
   DecShare s;
-  const long long nb = min((long long)a.nb, (W + PER - 1) / PER);
+  const int len0 = length(lane), scan0 = wave_inclusive_scan(tiles(len0, lane));
+  u32 W = (u32)__builtin_amdgcn_readlane(scan0, 63);
+  for (int c0 = 64; c0 < a.BH; c0 += 64) W += (u32)__builtin_amdgcn_readlane(wave_inclusive_scan(tiles(length(c0 + lane), c0 + lane)), 63);
+  const u32 nb = min((u32)a.nb, (W + PER - 1) / PER), q = W / nb, rest = W - q * nb, i = blockIdx.x;
   s.pos = s.hi = 0;
-  if ((long long)blockIdx.x < nb) {
-    s.pos = W * (long long)blockIdx.x / nb;
-    s.hi = W * ((long long)blockIdx.x + 1) / nb;
+  if (i < nb) {
+    s.pos = (int)(q * i + min(i, rest));
+    s.hi = s.pos + (int)(q + (i < rest ? 1u : 0u));
   }
   s.base = 0;
   s.bh = 0;
-  for (int c0 = 0; c0 < a.BH; c0 += 64) {
-    long long x = first;
-    if (c0) {
-      x = c0 + lane < a.BH ? (long long)segs * dec_tiles<KT>(dec_len(a, c0 + lane), fresh) : 0;
-#pragma unroll
-      for (int d = 1; d < 64; d *= 2) {
-        const long long y = __shfl_up(x, d);
-        if (lane >= d) x += y;
-      }
-    }
+  s.len = len0;
+  int x = scan0;
+  for (int c0 = 0;;) {
     const unsigned long long past = __ballot(s.base + x > s.pos);
     if (past) {
       const int at = __ffsll(past) - 1;
       s.bh = c0 + at;
-      if (at) s.base += dec_lane64(x, at - 1);
+      if (at) s.base += __builtin_amdgcn_readlane(x, at - 1);
       break;
     }
-    s.base += dec_lane64(x, 63);
+    s.base += __builtin_amdgcn_readlane(x, 63);
+    c0 += 64;
+    if (c0 >= a.BH) break;
+    s.len = length(c0 + lane);
+    x = wave_inclusive_scan(tiles(s.len, c0 + lane));
   }
   return s;
+}
+// Rows of the share's current head.
+__device__ __forceinline__ int dec_share_len(const DecShare& s) { return __builtin_amdgcn_readlane(s.len, s.bh & 63); }
+// On to the next head.
+__device__ __forceinline__ void dec_share_next(const DecArgs& a, DecShare& s) {
+  s.base = s.pos;
+  ++s.bh;
+  if ((s.bh & 63) == 0) {
+    const int bh = s.bh + (int)(threadIdx.x & 63);
+    s.len = bh < a.BH ? dec_len(a, bh) : 0;
+  }
 }
 
 // Which of a lane's 16 keys of 32 from kb (bit i: key kb + 8 (i / 4) + 4 hh + i % 4) query token tq sees, among the
 // cache's rows (fresh false) or the new ones.
 __device__ __forceinline__ u32 dec_visible(const DecArgs& a, int b, int tq, int kb, int rows, bool fresh) {
   const int k0 = kb + 4 * (int)((threadIdx.x >> 5) & 1);
-  const unsigned char* row = a.tree + b * a.tree_stride + tq * a.T;
+  const FE_GLOBAL unsigned char* row = a.tree + b * a.tree_stride + tq * a.T;
   u32 bits = 0;
 #pragma unroll 1
   for (int i = 0; i < 16; i += 4) {
@@ -223,50 +309,98 @@ __device__ __forceinline__ u32 dec_visible(const DecArgs& a, int b, int tq, int 
   return bits;
 }
 
+// The rows of a head: its cache's and its new ones'.
+struct DecRows {
+  DecIn kc, vc, k, v;
+  long long kcs, vcs, ks, vs;   // row strides
+};
+__device__ __forceinline__ DecRows dec_rows(const DecArgs& a, int b, int hkv) {
+  return {a.kc + b * a.kcs[0] + hkv * a.kcs[1], a.vc + b * a.vcs[0] + hkv * a.vcs[1], a.k + b * a.ks[0] + hkv * a.ks[1],
+          a.v + b * a.vs[0] + hkv * a.vs[1], a.kcs[2], a.vcs[2], a.ks[2], a.vs[2]};
+}
+
 // Where a tile of KT keys lies: tile t of nc of the cache, then of the new rows.
 struct DecTile {
-  const u16 *k, *v;
+  DecIn k, v;
   long long krs, vrs;
   int kb, rows;
   bool tail;
 };
 template <int KT>
-__device__ __forceinline__ DecTile dec_tile(const DecArgs& a, int b, int hkv, int n, int nc, int fresh, int t) {
+__device__ __forceinline__ DecTile dec_tile(const DecRows& r, int n, int nc, int fresh, int t) {
   DecTile x;
   x.tail = t >= nc;
   x.kb = (x.tail ? t - nc : t) * KT;
   x.rows = x.tail ? fresh : n;
-  x.krs = x.tail ? a.ks[2] : a.kcs[2];
-  x.vrs = x.tail ? a.vs[2] : a.vcs[2];
-  x.k = x.tail ? a.k + b * a.ks[0] + hkv * a.ks[1] : a.kc + b * a.kcs[0] + hkv * a.kcs[1];
-  x.v = x.tail ? a.v + b * a.vs[0] + hkv * a.vs[1] : a.vc + b * a.vcs[0] + hkv * a.vcs[1];
+  x.krs = x.tail ? r.ks : r.kcs;
+  x.vrs = x.tail ? r.vs : r.vcs;
+  x.k = x.tail ? r.k : r.kc;
+  x.v = x.tail ? r.v : r.vc;
   return x;
 }
 
-// Chunk i of NT threads' 16-byte chunks of KT rows from row kb on (zeros past `rows` and past channel D): thread tid has
-// chunk e = i * NT + tid in row order. Where a row's chunks divide the threads, a thread's channel is the same in each.
+// NT threads' 16-byte chunks of KT rows of D channels: thread tid's chunk i is e = i * NT + tid in row order. Loads
+// go out together, without a branch or a wait between them: a chunk past channel D is not loaded and keeps its zeros
+// (x starts as zeros), rows past the last are read as the last.
 template <int DP, int KT, int NT, int NL>
-__device__ __forceinline__ void dec_load_rows(const u16* p, long long rs, int kb, int rows, int D, int tid, u32x4 (&x)[NL]) {
+__device__ __forceinline__ void dec_load_rows(DecIn p, long long rs, int kb, int rows, int D, int tid, u32x4 (&x)[NL]) {
   constexpr int CPR = DP / 8;
   if constexpr (NT % CPR == 0) {
     const int key = tid / CPR, ch = 8 * (tid % CPR);
-    const u16* lp = p + key * rs + ch;
-    const bool in = ch < D;
-    if (kb + KT <= rows) {
+    if (ch < D) {
+      if (kb + KT <= rows) {
+        DecIn lp = p + (long long)(kb + key) * rs + ch;
+        const long long step = (long long)(NT / CPR) * rs;
 #pragma unroll
-      for (int i = 0; i < NL; ++i) x[i] = in ? *(const u32x4*)(lp + (long long)(kb + i * (NT / CPR)) * rs) : (u32x4){0u, 0u, 0u, 0u};
-    } else {
+        for (int i = 0; i < NL; ++i) {
+          x[i] = *(const FE_GLOBAL u32x4*)lp;
+          lp += step;
+          asm volatile("" : "+v"(lp));   // one address at a time, no table of multiples of the stride
+        }
+      } else {
 #pragma unroll
-      for (int i = 0; i < NL; ++i)
-        x[i] = in && kb + key + i * (NT / CPR) < rows ? *(const u32x4*)(lp + (long long)(kb + i * (NT / CPR)) * rs) : (u32x4){0u, 0u, 0u, 0u};
+        for (int i = 0; i < NL; ++i) x[i] = *(const FE_GLOBAL u32x4*)(p + (long long)min(kb + key + i * (NT / CPR), rows - 1) * rs + ch);
+      }
     }
   } else {
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int e = i * NT + tid, key = e / CPR, ch = 8 * (e % CPR);
-      const bool ok = kb + key < rows && ch < D && (KT * CPR % NT == 0 || key < KT);
-      x[i] = ok ? *(const u32x4*)(p + (long long)(kb + key) * rs + ch) : (u32x4){0u, 0u, 0u, 0u};
+      if (ch < D) x[i] = *(const FE_GLOBAL u32x4*)(p + (long long)min(kb + key, rows - 1) * rs + ch);
     }
+  }
+}
+// Zeros in place of the rows past the last (V: 0 * inf is not 0).
+template <int DP, int NT, int NL>
+__device__ __forceinline__ void dec_cut_rows(int kb, int rows, int tid, u32x4 (&x)[NL]) {
+#pragma unroll
+  for (int i = 0; i < NL; ++i)
+    if (kb + (i * NT + tid) / (DP / 8) >= rows) x[i] = (u32x4){0u, 0u, 0u, 0u};
+}
+
+// A lane's fragments of its query row: read, then (once the tile behind them is on its way too) with the scale's sign
+// and zeros past D and for a row that is none.
+template <int DP, int VEC>
+__device__ __forceinline__ void dec_read_q(const DecArgs& a, int b, int head, int tq, u32x4 (&qf)[DP / 16]) {
+  const int hh = (threadIdx.x >> 5) & 1;
+  const DecIn qp = a.q + b * a.qs[0] + head * a.qs[1] + tq * a.qs[2];   // a real row in any case
+#pragma unroll
+  for (int c = 0; c < DP / 16; ++c) {
+    if constexpr (VEC) {
+      qf[c] = *(const FE_GLOBAL u32x4*)(qp + (16 * c + 8 * hh < a.D ? 16 * c + 8 * hh : 0));
+    } else {
+      qf[c] = dec_load8(qp, a.qc, 2 * c + hh, a.D);
+      __builtin_amdgcn_sched_barrier(0);   // element loads: one chunk's addresses at a time
+    }
+  }
+}
+template <int DP>
+__device__ __forceinline__ void dec_set_q(const DecArgs& a, bool valid, u32x4 (&qf)[DP / 16]) {
+  const int hh = (threadIdx.x >> 5) & 1;
+#pragma unroll
+  for (int c = 0; c < DP / 16; ++c) {
+    const u32 keep = valid && 16 * c + 8 * hh < a.D ? a.qand : 0u, flip = keep ? a.qxor : 0u;
+    qf[c] = (qf[c] & keep) ^ flip;
   }
 }
 
@@ -281,10 +415,260 @@ __device__ __forceinline__ int dec_slot(const DecArgs& a, int seg, bool head, bo
   return slot;
 }
 
+template <typename E>
+__device__ __forceinline__ f32x4 dec_mfma16(u32x4 x, u32x4 y, f32x4 c);
+template <>
+__device__ __forceinline__ f32x4 dec_mfma16<BF16>(u32x4 x, u32x4 y, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), c, 0, 0, 0);
+}
+template <>
+__device__ __forceinline__ f32x4 dec_mfma16<F16>(u32x4 x, u32x4 y, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), c, 0, 0, 0);
+}
+
+// Maximum and sum over the lanes l, l ^ 16, l ^ 32, l ^ 48 (the four that hold a query's keys).
+__device__ __forceinline__ float dec_quad_max(float x) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return half_swap_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float dec_quad_sum(float x) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return half_swap_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+// Tiles of a block of the few-rows kernel: whole rounds of its four waves.
+__device__ __forceinline__ int dec_few_share(int tiles, int S) { return ((tiles + 4 * S - 1) / (4 * S)) * 4; }
+
+// Block (split, KV head, batch row). S^T = K Q^T and O^T = V^T P^T with 16 queries in the lanes' low four bits: 32 keys
+// are two accumulators of S^T, whose registers (keys 4 (lane / 16) + i of each) are P^T's operand as they are; V^T's comes
+// from transposing reads in that key order.
+// What bounds it: HBM where the cache is long (the next 32 keys' K and V are on their way to registers while a wave
+// works on these); where it is short, the reading of its own code and the one round trip to memory, so the loads of
+// a tile appear in the code once, rows past the end are read as the last, and nothing is divided that need not be.
+template <typename E, int DP>
+__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_few_kernel(const DecFewArgs args) {
+  constexpr int NC = DP / 32, NT16 = DP / 16, CPR = DP / 8, NL = DP / 16, TILE = 64 * DP, OST = DP + 4;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[4][2 * TILE];
+  __shared__ float sm[3][4][16];
+  static_assert(2 * TILE >= 16 * OST * 4 && 2 * TILE >= (32 * 16 + DP) * 4, "output, or probabilities and a value, in a wave's tiles");
+  const DecFewArgs a = dec_hold<0, 4>(args);
+  const int lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4;
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int hkv = (int)blockIdx.y, b = (int)blockIdx.z, bh = b * (int)gridDim.y + hkv;
+  int n = a.length[bh];
+  // this lane's query row (row 0 where there is none: its results go nowhere)
+  const int r = l16 < a.R ? l16 : 0;
+  const int g = a.T == 1 ? r : r / a.T, tq = r - g * a.T;
+  const DecIn qp = a.q + b * a.qb + (long long)(hkv * (a.R / a.T) + g) * a.qh + tq * a.qn;
+  u32x4 qf[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) qf[c] = *(const FE_GLOBAL u32x4*)(qp + (DP == a.D || 32 * c + 8 * lq < a.D ? 32 * c + 8 * lq : 0));
+  const DecIn kc = a.kc + b * a.kcb + hkv * a.kch, vc = a.vc + b * a.vcb + hkv * a.vch;
+  const DecIn kn = a.k + b * a.kb + hkv * a.kh, vn = a.v + b * a.vb + hkv * a.vh;
+  n = __builtin_amdgcn_readfirstlane(min(max(n, 0), a.C));
+  const int nc = (n + 31) / 32, tiles = nc + (a.T + 31) / 32, share = dec_few_share(tiles, a.S);
+  const int t0 = (int)blockIdx.x * share, t1 = min(tiles, t0 + share);
+  if (t0 >= t1) return;
+
+  unsigned char* kt = lds[wv];
+  unsigned char* vt = lds[wv] + TILE;
+  f32x4 o[NT16];
+#pragma unroll
+  for (int i = 0; i < NT16; ++i) o[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  float m = kDecNegInf, l = 0.f, lr = 0.f;   // l, lr: of the lane's keys
+  u32x4 kx[NL] = {}, vx[NL] = {};
+  int t = -1, next = t0 + wv;
+  bool set = false;
+#pragma unroll 1
+  while (true) {
+    const bool tail = t >= nc;
+    const int kb = (tail ? t - nc : t) * 32, rows = tail ? a.T : n;
+    u32 odd = 0;                           // keys of new rows with a value that is not finite (as in decode_rows_kernel)
+    if (t >= 0) {
+      if (kb + 32 > rows) dec_cut_rows<DP, 64>(kb, rows, lane, vx);
+      if (a.D != DP) {
+#pragma unroll
+        for (int i = 0; i < NL; ++i)
+          if (8 * ((i * 64 + lane) % CPR) >= a.D) kx[i] = (u32x4){0u, 0u, 0u, 0u};
+      }
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const int e = i * 64 + lane;
+        *(u32x4*)(kt + dec_k_at<DP>(e / CPR, e % CPR)) = kx[i];
+        *(u32x4*)(vt + dec_v_at<DP>(e / CPR, e % CPR)) = vx[i];
+      }
+      if (tail) {
+        u32 bad = 0;
+#pragma unroll
+        for (int i = 0; i < NL; ++i) bad |= dec_nonfinite<E>(vx[i]) ? 1u << ((i * 64 + lane) / CPR) : 0u;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) bad |= __shfl_xor(bad, d);
+        odd = __builtin_amdgcn_readfirstlane(bad);
+      }
+    }
+    if (next < t1) {
+      const bool nt = next >= nc;
+      const int nkb = (nt ? next - nc : next) * 32, last = (nt ? a.T : n) - 1;
+      const DecIn kp = nt ? kn : kc, vp = nt ? vn : vc;
+      const u32 ks = nt ? a.kn : a.kcn, vs = nt ? a.vn : a.vcn;
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const int e = i * 64 + lane, ch = 8 * (e % CPR);
+        const u32 row = (u32)min(nkb + e / CPR, last);
+        if (64 % CPR == 0 ? true : ch < a.D) {
+          const int cc = DP == a.D || ch < a.D ? ch : 0;
+          kx[i] = *(const FE_GLOBAL u32x4*)(kp + (unsigned long long)row * ks + cc);
+          vx[i] = *(const FE_GLOBAL u32x4*)(vp + (unsigned long long)row * vs + cc);
+        }
+      }
+    }
+    if (!set) {
+      set = true;
+      if (a.qand != ~0u || a.qxor != 0u || a.D != DP) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const u32 keep = 32 * c + 8 * lq < a.D ? a.qand : 0u, flip = keep ? a.qxor : 0u;
+          qf[c] = (qf[c] & keep) ^ flip;
+        }
+      }
+    }
+    if (t >= 0) {
+      if (odd) {
+        dec_wave_order();
+        for (int e = lane; e < 32 * CPR; e += 64)
+          if ((odd >> (e / CPR)) & 1u) *(u32x4*)(vt + dec_v_at<DP>(e / CPR, e % CPR)) = (u32x4){0u, 0u, 0u, 0u};
+      }
+      dec_wave_order();
+      f32x4 x[2];
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const u32x4 kf = *(const u32x4*)(kt + dec_k_at<DP>(16 * s + l16, 4 * c + lq));
+          x[s] = dec_mfma16<E>(kf, qf[c], c == 0 ? (f32x4){0.f, 0.f, 0.f, 0.f} : x[s]);
+        }
+      u32 vis = 0xffu;                      // bit 4 s + i: register i of x[s], key kb + 16 s + 4 lq + i, is visible
+      if (tail || kb + 32 > rows) {
+        const FE_GLOBAL unsigned char* row = a.tree + b * a.tree_stride + tq * a.T;
+        vis = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int key = kb + 16 * (i >> 2) + 4 * lq + (i & 3);
+          bool see = key < rows;
+          if (tail) see = see && (a.tree ? row[see ? key : 0] != 0 : key <= tq);
+          vis |= (see ? 1u : 0u) << i;
+          x[i >> 2][i & 3] = see ? x[i >> 2][i & 3] : kDecNegInf;
+        }
+      }
+      float mn = kDecNegInf;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[i >> 2][i & 3] *= a.scale_log2;
+        mn = fmaxf(mn, x[i >> 2][i & 3]);
+      }
+      if (a.logits && l16 < a.R) {
+        const DecF32 lp = a.logits + (((long long)bh * a.max_tiles + t) * a.R + l16) * 32 + 4 * lq;
+        *(FE_GLOBAL f32x4*)lp = x[0];
+        *(FE_GLOBAL f32x4*)(lp + 16) = x[1];
+      }
+      mn = fmaxf(m, dec_quad_max(mn));
+      const float ref = mn == kDecNegInf ? 0.f : mn;
+      const float alpha = fast_exp2(m - ref);
+      m = mn;
+      float ls = 0.f, lrs = 0.f;
+      u32x4 pf;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[i >> 2][i & 3] = fast_exp2(x[i >> 2][i & 3] - ref);
+        ls += x[i >> 2][i & 3];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        pf[i] = E::pack2(x[i >> 1][2 * (i & 1)], x[i >> 1][2 * (i & 1) + 1]);
+        lrs += E::to_f32((u16)pf[i]) + E::to_f32((u16)(pf[i] >> 16));
+      }
+      l = l * alpha + ls;
+      lr = lr * alpha + lrs;
+      if (__ballot(alpha != 1.f)) {
+#pragma unroll
+        for (int i = 0; i < NT16; ++i) o[i] *= alpha;
+      }
+#pragma unroll
+      for (int i = 0; i < NT16; ++i) {
+        // channels 16 i + l16: keys 4 lq .. + 3, then 16 + 4 lq .. + 3
+        const int row = 4 * lq + (l16 >> 2);
+        unsigned char* p = vt + row * (DP * 2) + ((i >> 1) ^ dec_vswz<DP>(row)) * 64 + 32 * (i & 1) + 8 * (l16 & 3);
+        const u32x2 ux = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((dec_lds_s16x4*)(dec_lds_ptr)p));
+        const u32x2 uy = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((dec_lds_s16x4*)(dec_lds_ptr)(p + 16 * DP * 2)));
+        o[i] = dec_mfma16<E>((u32x4){ux[0], ux[1], uy[0], uy[1]}, pf, o[i]);
+      }
+      if (odd) {
+        dec_wave_order();
+        float* sp = (float*)kt;             // [32 keys][16 rows] probabilities (-1: hidden)
+        float* val = sp + 32 * 16;          // a value's channels
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sp[(16 * (i >> 2) + 4 * lq + (i & 3)) * 16 + l16] = (vis >> i) & 1u ? x[i >> 2][i & 3] : -1.f;
+        for (u32 left = odd; left; left &= left - 1) {
+          const int key = __ffs((int)left) - 1;
+          for (int ch = lane; ch < DP; ch += 64) val[ch] = ch < a.D ? E::to_f32(vn[(unsigned long long)(kb + key) * a.vn + ch]) : 0.f;
+          dec_wave_order();
+          const float p = sp[key * 16 + l16];
+#pragma unroll
+          for (int i = 0; i < NT16; ++i) {
+            const f32x4 y = *(const f32x4*)(val + 16 * i + 4 * lq);
+            if (p >= 0.f || p != p) o[i] += p * y;
+          }
+          dec_wave_order();
+        }
+      }
+      dec_wave_order();                     // the next tile's stores follow this one's reads
+    }
+    if (next >= t1) break;
+    t = next;
+    next += 4;
+  }
+
+  // join the four waves (waves without a tile have a maximum of -inf and zeros)
+  l = dec_quad_sum(l);
+  lr = dec_quad_sum(lr);
+  if (lq == 0) {
+    sm[0][wv][l16] = m;
+    sm[1][wv][l16] = l;
+    sm[2][wv][l16] = lr;
+  }
+  float* mine = (float*)lds[wv];
+#pragma unroll
+  for (int i = 0; i < NT16; ++i) *(f32x4*)(mine + l16 * OST + 16 * i + 4 * lq) = o[i];
+  __syncthreads();
+  const long long slot = (long long)bh * a.S + blockIdx.x;
+#pragma unroll 1
+  for (int e = threadIdx.x; e < a.R * (DP / 4); e += 256) {
+    const int row = e / (DP / 4), ch = 4 * (e % (DP / 4));
+    const float mx = fmaxf(fmaxf(sm[0][0][row], sm[0][1][row]), fmaxf(sm[0][2][row], sm[0][3][row]));
+    const float ref = mx == kDecNegInf ? 0.f : mx;
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    float lt = 0.f, lrt = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float w = fast_exp2(sm[0][i][row] - ref);
+      s += w * *(const f32x4*)((float*)lds[i] + row * OST + ch);
+      lt += w * sm[1][i][row];
+      lrt += w * sm[2][i][row];
+    }
+    // partials are normalised by the sum of the rounded probabilities, and weighted by the exact one: so a row
+    // that one key dominates returns that key's value whatever the split
+    *(FE_GLOBAL f32x4*)(a.part_o + (slot * 16 + row) * DP + ch) = s * (lrt == 0.f ? 0.f : __builtin_amdgcn_rcpf(lrt));
+    if (ch == 0) {
+      a.part_ml[slot * 32 + row] = mx;
+      a.part_ml[slot * 32 + 16 + row] = lt;
+    }
+  }
+}
+
 // What bounds it: HBM. Few rows leave the matrix and vector units mostly idle, so every wave keeps the next 32 keys'
 // K and V on the way to registers while it works on these.
 template <typename E, int DP, int VEC>
-__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_rows_kernel(const DecArgs a) {
+__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_rows_kernel(const DecArgs args) {
   constexpr int NDC = DP / 16, NDT = DP / 32, CPR = DP / 8, TILE = 64 * DP;   // bytes of 32 rows
   constexpr int OST = 33;                // floats of a channel's 32 rows in LDS, and one against bank conflicts
   constexpr int WLDS = DP * OST * 4;     // a wave's LDS: a K and a V tile, then its output
@@ -295,53 +679,47 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_rows_kernel(cons
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   unsigned char* kt = lds[wv];
   unsigned char* vt = lds[wv] + TILE;
+  const DecArgs a = dec_hold<kDecAttnArgs, 5>(args);
 
   DecShare sh = dec_share<32, 4>(a, a.RB, a.T);
   while (sh.pos < sh.hi) {
     const int bh = sh.bh, b = bh / a.Hkv, hkv = bh - b * a.Hkv;
-    const int n = dec_len(a, bh);
+    const int n = dec_share_len(sh);
     const int nc = (n + 31) / 32, tiles = dec_tiles<32>(n, a.T);
-    const int rb = (int)((sh.pos - sh.base) / tiles), t0 = (int)((sh.pos - sh.base) - (long long)rb * tiles);
-    const int t1 = (int)min((long long)tiles, t0 + (sh.hi - sh.pos));
+    const int rb = a.RB == 1 ? 0 : (sh.pos - sh.base) / tiles, t0 = sh.pos - sh.base - rb * tiles;
+    const int t1 = min(tiles, t0 + sh.hi - sh.pos);
     sh.pos += t1 - t0;
-    if (sh.pos - sh.base == (long long)a.RB * tiles) {
-      sh.base = sh.pos;
-      ++sh.bh;
-    }
+    if (t1 == tiles && rb == a.RB - 1) dec_share_next(a, sh);
 
     const int r = rb * 32 + l32;         // this lane's query row
     const bool rv = r < a.R;
     const int g = rv ? r / a.T : 0, tq = rv ? r - g * a.T : 0;
+    const DecRows hr = dec_rows(a, b, hkv);
     u32x4 qf[NDC];
-    {
-      const u16* qp = a.q + b * a.qs[0] + (hkv * a.G + g) * a.qs[1] + tq * a.qs[2];
-#pragma unroll
-      for (int c = 0; c < NDC; ++c) {
-        qf[c] = rv ? (dec_load8<VEC>(qp, a.qs[3], 2 * c + hh, a.D) & a.qand) ^ a.qxor : (u32x4){0u, 0u, 0u, 0u};
-        if (!VEC) __builtin_amdgcn_sched_barrier(0);   // element loads: one chunk's addresses at a time
-      }
-    }
+    dec_read_q<DP, VEC>(a, b, hkv * a.G + g, tq, qf);
     f32x16 o[NDT];
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) o[dt] = (f32x16){};
     float m = kDecNegInf, l = 0.f, lr = 0.f;   // sums of the probabilities, and of these as rounded for the product
 
-    u32x4 kx[VEC ? NDC : 1], vx[VEC ? NDC : 1];
+    u32x4 kx[VEC ? NDC : 1] = {}, vx[VEC ? NDC : 1] = {};
     auto load = [&](int t) __attribute__((always_inline)) {
-      const DecTile at = dec_tile<32>(a, b, hkv, n, nc, a.T, t);
+      const DecTile at = dec_tile<32>(hr, n, nc, a.T, t);
       dec_load_rows<DP, 32, 64>(at.k, at.krs, at.kb, at.rows, a.D, lane, kx);
       dec_load_rows<DP, 32, 64>(at.v, at.vrs, at.kb, at.rows, a.D, lane, vx);
     };
     if (VEC && t0 + wv < t1) load(t0 + wv);
+    dec_set_q<DP>(a, rv, qf);
     for (int t = t0 + wv; t < t1; t += 4) {
-      const DecTile at = dec_tile<32>(a, b, hkv, n, nc, a.T, t);
+      const DecTile at = dec_tile<32>(hr, n, nc, a.T, t);
       const bool tail = at.tail;
       const int kb = at.kb, rows = at.rows;
-      const long long vcs = tail ? a.vs[3] : a.vcs[3];
+      const long long vcs = VEC ? 1 : tail ? a.vnc : a.vcc;
       // keys of the tail whose value has an infinity or a NaN: 0 * inf would reach the rows that do not see
       // them, so their values are taken out of the product and added to the rows that do
       u32 odd = 0;
       if (VEC) {
+        if (kb + 32 > rows) dec_cut_rows<DP, 64>(kb, rows, lane, vx);
 #pragma unroll
         for (int i = 0; i < NDC; ++i) {
           const int e = i * 64 + lane;
@@ -355,14 +733,14 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_rows_kernel(cons
         }
         if (t + 4 < t1) load(t + 4);
       } else {
-        const long long kcs = tail ? a.ks[3] : a.kcs[3];
+        const long long kcs = tail ? a.knc : a.kcc;
 #pragma unroll 1
         for (int i = 0; i < NDC; ++i) {
           const int e = i * 64 + lane, row = kb + e / CPR, ch = e % CPR;
-          const u32x4 x = row < rows ? dec_load8<VEC>(at.k + row * at.krs, kcs, ch, a.D) : (u32x4){0u, 0u, 0u, 0u};
+          const u32x4 x = row < rows ? dec_load8(at.k + row * at.krs, kcs, ch, a.D) : (u32x4){0u, 0u, 0u, 0u};
           *(u32x4*)(kt + dec_k_at<DP>(e / CPR, ch)) = x;
           __builtin_amdgcn_sched_barrier(0);
-          const u32x4 y = row < rows ? dec_load8<VEC>(at.v + row * at.vrs, vcs, ch, a.D) : (u32x4){0u, 0u, 0u, 0u};
+          const u32x4 y = row < rows ? dec_load8(at.v + row * at.vrs, vcs, ch, a.D) : (u32x4){0u, 0u, 0u, 0u};
           *(u32x4*)(vt + dec_v_at<DP>(e / CPR, ch)) = y;
           if (tail)
             for (unsigned long long bl = __ballot(dec_nonfinite<E>(y)); bl; bl &= bl - 1) odd |= 1u << ((i * 64 + __ffsll(bl) - 1) / CPR);
@@ -391,9 +769,9 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_rows_kernel(cons
         mn = fmaxf(mn, x[i]);
       }
       if (a.logits && rv) {
-        float* lp = a.logits + (((long long)bh * a.max_tiles + t) * a.R + r) * 32 + 4 * hh;
+        const DecF32 lp = a.logits + (((long long)bh * a.max_tiles + t) * a.R + r) * 32 + 4 * hh;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) *(f32x4*)(lp + 8 * i) = (f32x4){x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
+        for (int i = 0; i < 4; ++i) *(FE_GLOBAL f32x4*)(lp + 8 * i) = (f32x4){x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
       }
       mn = fmaxf(m, half_swap_max(mn));
       const float ref = mn == kDecNegInf ? 0.f : mn;
@@ -491,7 +869,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_rows_kernel(cons
 // What bounds it: vector work beside the products (an exponential a logit); at 256 rows a tile takes about as long as
 // its bytes from HBM.
 template <typename E, int DP, int NW>
-__global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void decode_wide_kernel(const DecArgs a) {
+__global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void decode_wide_kernel(const DecArgs args) {
   constexpr int NDC = DP / 16, NDT = DP / 32, CPR = DP / 8, TILE = 128 * DP;   // bytes of 64 rows
   constexpr int NT = NW * 64, NL = (64 * CPR + NT - 1) / NT;
   __shared__ __attribute__((aligned(1024))) unsigned char lds_k[2][TILE], lds_v[2][TILE];
@@ -500,29 +878,24 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void decode_wide_kernel(
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
 
+  const DecArgs a = dec_hold<kDecAttnArgs, 5>(args);
   DecShare sh = dec_share<64, 1>(a, a.RB, a.T);
   while (sh.pos < sh.hi) {
     const int bh = sh.bh, b = bh / a.Hkv, hkv = bh - b * a.Hkv;
-    const int n = dec_len(a, bh);
+    const int n = dec_share_len(sh);
     const int nc = (n + 63) / 64, tiles = dec_tiles<64>(n, a.T);
-    const int rb = (int)((sh.pos - sh.base) / tiles), t0 = (int)((sh.pos - sh.base) - (long long)rb * tiles);
-    const int t1 = (int)min((long long)tiles, t0 + (sh.hi - sh.pos));
+    const int rb = a.RB == 1 ? 0 : (sh.pos - sh.base) / tiles, t0 = sh.pos - sh.base - rb * tiles;
+    const int t1 = min(tiles, t0 + sh.hi - sh.pos);
     sh.pos += t1 - t0;
-    if (sh.pos - sh.base == (long long)a.RB * tiles) {
-      sh.base = sh.pos;
-      ++sh.bh;
-    }
+    if (t1 == tiles && rb == a.RB - 1) dec_share_next(a, sh);
 
     const int r = (rb * a.RW + wv) * 32 + l32;
     const bool live = wv < a.RW && (rb * a.RW + wv) * 32 < a.R;   // the wave has rows
     const bool rv = live && r < a.R;
     const int g = rv ? r / a.T : 0, tq = rv ? r - g * a.T : 0;
+    const DecRows hr = dec_rows(a, b, hkv);
     u32x4 qf[NDC];
-    {
-      const u16* qp = a.q + b * a.qs[0] + (hkv * a.G + g) * a.qs[1] + tq * a.qs[2];
-#pragma unroll
-      for (int c = 0; c < NDC; ++c) qf[c] = rv ? (dec_load8<1>(qp, 1, 2 * c + hh, a.D) & a.qand) ^ a.qxor : (u32x4){0u, 0u, 0u, 0u};
-    }
+    dec_read_q<DP, 1>(a, b, hkv * a.G + g, tq, qf);
     f32x16 o[NDT];
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) o[dt] = (f32x16){};
@@ -530,13 +903,15 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void decode_wide_kernel(
     u32 ones2;
     asm volatile("s_mov_b32 %0, %1" : "=s"(ones2) : "i"(E::kOnes2));
 
-    u32x4 kx[NL], vx[NL];
+    u32x4 kx[NL] = {}, vx[NL] = {};
     auto load = [&](int t) __attribute__((always_inline)) {
-      const DecTile at = dec_tile<64>(a, b, hkv, n, nc, a.T, t);
+      const DecTile at = dec_tile<64>(hr, n, nc, a.T, t);
       dec_load_rows<DP, 64, NT>(at.k, at.krs, at.kb, at.rows, a.D, tid, kx);
       dec_load_rows<DP, 64, NT>(at.v, at.vrs, at.kb, at.rows, a.D, tid, vx);
     };
     auto store = [&](int t, int buf) __attribute__((always_inline)) {
+      const DecTile at = dec_tile<64>(hr, n, nc, a.T, t);
+      if (at.kb + 64 > at.rows) dec_cut_rows<DP, NT>(at.kb, at.rows, tid, vx);
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
         const int e = i * NT + tid, key = e / CPR, ch = e % CPR;
@@ -556,6 +931,7 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void decode_wide_kernel(
       }
     };
     load(t0);
+    dec_set_q<DP>(a, rv, qf);
     store(t0, t0 & 1);
     __syncthreads();
     for (int t = t0; t < t1; ++t) {
@@ -629,7 +1005,7 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void decode_wide_kernel(
           exponentials();
         }
         if (odd) {
-          const u16* vp = a.v + b * a.vs[0] + hkv * a.vs[1];
+          const DecIn vp = hr.v;
 #pragma unroll 1
           for (unsigned long long left = odd; left; left &= left - 1) {
             const int key = __ffsll(left) - 1;
@@ -644,7 +1020,7 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void decode_wide_kernel(
             const float nan = half_swap_max(mine != mine ? 1.f : 0.f);
             const float pr = nan > 0.f ? __builtin_nanf("") : pk;
             const bool sees = pk >= 0.f || nan > 0.f;
-            const u16* row = vp + (long long)(kb + key) * a.vs[2];
+            const DecIn row = vp + (long long)(kb + key) * hr.vs;
             for (int ch = lane; ch < DP; ch += 64) s_row[wv][ch] = ch < a.D ? E::to_f32(row[ch]) : 0.f;
             dec_wave_order();
 #pragma unroll
@@ -682,12 +1058,12 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void decode_wide_kernel(
     if (rv) {
       const float inv = lr == 0.f ? 0.f : 1.f / lr;
       const int row = wv * 32 + l32;
-      float* po = a.part_o + ((long long)slot * a.RW * 32 + row) * DP;
+      const DecF32 po = a.part_o + ((long long)slot * a.RW * 32 + row) * DP;
 #pragma unroll
       for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          *(f32x4*)(po + 32 * dt + 8 * i + 4 * hh) =
+          *(FE_GLOBAL f32x4*)(po + 32 * dt + 8 * i + 4 * hh) =
               (f32x4){o[dt][4 * i] * inv, o[dt][4 * i + 1] * inv, o[dt][4 * i + 2] * inv, o[dt][4 * i + 3] * inv};
       if (hh == 0) {
         a.part_ml[(long long)slot * 64 * a.RW + row] = m;
@@ -697,52 +1073,93 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void decode_wide_kernel(
   }
 }
 
-// Blocks below join_blocks: out = sum_s w_s O_s / sum w_s with w_s = l_s 2^(m_s - m), eight 32-lane groups a block,
-// join_split of them (1 or 8) on each row. Later blocks, where there are logits: eight tiles of 32 keys of a head,
-// importance_out and new_importance.
+// A segment's first slot and its number of slots.
+__device__ __forceinline__ void dec_slots(const DecJoinArgs& a, int bh, int sg, int& first, int& count) {
+  if (a.S) {
+    const int n = min(max(a.length[bh], 0), a.C), tiles = dec_tiles<32>(n, a.T), share = dec_few_share(tiles, a.S);
+    first = bh * a.S;
+    count = (tiles + share - 1) / share;
+  } else {
+    first = a.seg[2 * sg];
+    count = a.seg[2 * sg + 1] - first + 1;
+  }
+}
+
+// Blocks below out_blocks: out = sum_s w_s O_s / sum w_s with w_s = l_s 2^(m_s - m), eight 32-lane groups a block,
+// `split` of them (1 or 8) on each row. Later blocks, where there are logits: importance_out and new_importance, tiles
+// of 32 keys of a head, per_head blocks on each.
+// What bounds it: waits. Its few loads depend on each other (slots, maxima, values), so what can be is read before.
 template <typename E, int DP>
-__global__ __launch_bounds__(256) void decode_join_kernel(const DecArgs a) {
+__global__ __launch_bounds__(256) void decode_join_kernel(const DecJoinArgs args) {
   constexpr int NV = (DP + 127) / 128;      // float4 of a lane
+  constexpr int PF = 4;                     // splits, or rows of logits, in flight
   __shared__ float sm[8][32], sl[8][32];
   __shared__ float bias[32];
   __shared__ f32x4 so[8][32 * NV];
+  const DecJoinArgs a = dec_hold<0, 4>(args);
   const int l32 = threadIdx.x & 31, grp = threadIdx.x >> 5;
-  const int RS = a.RW * 32;                 // rows of a segment
-  if ((int)blockIdx.x < a.join_blocks) {
-    const int per = 8 / a.join_split, sub = grp % a.join_split;
-    const long long gr = (long long)blockIdx.x * per + grp / a.join_split;   // row of all heads' rows
-    const bool rv = gr < (long long)a.BH * a.R;
-    const int bh = rv ? (int)(gr / a.R) : 0, r = rv ? (int)(gr - (long long)bh * a.R) : 0;
-    const int sg = bh * a.RB + r / RS, row = r % RS;
-    const int first = a.seg[2 * sg], count = rv ? a.seg[2 * sg + 1] - first + 1 : 0;
-    const float* ml = a.part_ml + (long long)first * 2 * RS + row;
-    float m = kDecNegInf;
-    for (int s = l32; s < count; s += 32) m = fmaxf(m, ml[(long long)s * 2 * RS]);
+  const int RS = a.RS;
+  if ((int)blockIdx.x < a.out_blocks) {
+    const int split = a.split, per = 8 / split, sub = grp % split;
+    const int gr = (int)blockIdx.x * per + grp / split;   // row of all heads' rows
+    const bool rv = gr < a.BH * a.R;
+    const int bh = rv ? gr / a.R : 0, r = rv ? gr - bh * a.R : 0;
+    const int sgr = a.RB == 1 ? 0 : r / RS, row = r - sgr * RS;
+    int first, count;
+    dec_slots(a, bh, bh * a.RB + sgr, first, count);
+    if (!rv) count = 0;
+    const DecF32In ml = a.part_ml + (long long)first * 2 * RS + row;
+    const DecF32In po = a.part_o + ((long long)first * RS + row) * DP + 4 * l32;
+    auto values = [&](int s, f32x4 (&x)[NV]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int d = 16; d; d /= 2) m = fmaxf(m, __shfl_xor(m, d));
-    const float ref = m == kDecNegInf ? 0.f : m;
-    float l = 0.f;
-    for (int s = l32; s < count; s += 32) l += ml[(long long)s * 2 * RS + RS] * fast_exp2(ml[(long long)s * 2 * RS] - ref);
+      for (int v = 0; v < NV; ++v)
+        x[v] = 128 * v + 4 * l32 < DP ? *(const FE_GLOBAL f32x4*)(po + (long long)s * RS * DP + 128 * v) : (f32x4){0.f, 0.f, 0.f, 0.f};
+    };
+    f32x4 x[PF][NV];
+#pragma unroll
+    for (int i = 0; i < PF; ++i)
+      if (sub + i * split < count) values(sub + i * split, x[i]);
+    float m = kDecNegInf, l = 0.f;
+    for (int s = l32; s < count; s += 32) {
+      const float ms = ml[(long long)s * 2 * RS], ls = ml[(long long)s * 2 * RS + RS];
+      const float mn = fmaxf(m, ms), ref = mn == kDecNegInf ? 0.f : mn;
+      l = l * fast_exp2(m - ref) + ls * fast_exp2(ms - ref);
+      m = mn;
+    }
+    float mx = m;
+#pragma unroll
+    for (int d = 16; d; d /= 2) mx = fmaxf(mx, __shfl_xor(mx, d));
+    const float ref = mx == kDecNegInf ? 0.f : mx;
+    l *= fast_exp2(m - ref);
+    m = mx;
 #pragma unroll
     for (int d = 16; d; d /= 2) l += __shfl_xor(l, d);
     f32x4 acc[NV];
 #pragma unroll
     for (int v = 0; v < NV; ++v) acc[v] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    const float* po = a.part_o + ((long long)first * RS + row) * DP + 4 * l32;
-#pragma unroll 4
-    for (int s = sub; s < count; s += a.join_split) {
-      // a split that this row sees nothing of has a weight of 0 and values of 0
-      const float w = ml[(long long)s * 2 * RS + RS] * fast_exp2(ml[(long long)s * 2 * RS] - ref);
+    for (int s0 = sub; s0 < count; s0 += PF * split) {
+      if (s0 != sub) {
 #pragma unroll
-      for (int v = 0; v < NV; ++v)
-        if (128 * v + 4 * l32 < DP) acc[v] += w * *(const f32x4*)(po + (long long)s * RS * DP + 128 * v);
+        for (int i = 0; i < PF; ++i)
+          if (s0 + i * split < count) values(s0 + i * split, x[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < PF; ++i) {
+        const int s = s0 + i * split;
+        if (s < count) {
+          // a split that this row sees nothing of has a weight of 0 and values of 0
+          const float w = ml[(long long)s * 2 * RS + RS] * fast_exp2(ml[(long long)s * 2 * RS] - ref);
+#pragma unroll
+          for (int v = 0; v < NV; ++v) acc[v] += w * x[i][v];
+        }
+      }
     }
-    if (a.join_split > 1) {
+    if (split > 1) {
 #pragma unroll
       for (int v = 0; v < NV; ++v) so[grp][v * 32 + l32] = acc[v];
       __syncthreads();
       if (sub) return;
-      for (int i = 1; i < a.join_split; ++i)
+      for (int i = 1; i < split; ++i)
 #pragma unroll
         for (int v = 0; v < NV; ++v) acc[v] += so[grp + i][v * 32 + l32];
     }
@@ -754,9 +1171,9 @@ __global__ __launch_bounds__(256) void decode_join_kernel(const DecArgs a) {
     for (int v = 0; v < NV; ++v) {
       const int d = 128 * v + 4 * l32;
       const u32 w0 = E::pack2(acc[v][0] * inv, acc[v][1] * inv), w1 = E::pack2(acc[v][2] * inv, acc[v][3] * inv);
-      u16* op = a.out + at * a.D + d;
+      FE_GLOBAL u16* op = a.out + at * a.D + d;
       if (a.D % 4 == 0) {
-        if (d < a.D) *(u32x2*)op = (u32x2){w0, w1};
+        if (d < a.D) *(FE_GLOBAL u32x2*)op = (u32x2){w0, w1};
       } else {
         const u16 h[4] = {(u16)w0, (u16)(w0 >> 16), (u16)w1, (u16)(w1 >> 16)};
 #pragma unroll
@@ -769,55 +1186,80 @@ __global__ __launch_bounds__(256) void decode_join_kernel(const DecArgs a) {
   }
 
   // importance: a head's R <= kDecLogitRows rows are one segment
-  const int blk = (int)blockIdx.x - a.join_blocks, bh = blk % a.BH, t = blk / a.BH * 8 + grp;
+  const int blk = (int)blockIdx.x - a.out_blocks, bh = blk / a.per_head, part = blk - bh * a.per_head;
   const int b = bh / a.Hkv, hkv = bh - b * a.Hkv;
-  const int n = dec_len(a, bh), nc = (n + 31) / 32, tiles = dec_tiles<32>(n, a.T);
-  if (blk / a.BH * 8 >= tiles) return;
-  {
-    const int first = a.seg[2 * bh], count = a.seg[2 * bh + 1] - first + 1;
-    const float* ml = a.part_ml + (long long)first * 64 + l32;
-    const bool rv = l32 < a.R;
-    float m = kDecNegInf;
-    for (int s = grp; s < count; s += 8) m = rv ? fmaxf(m, ml[s * 64]) : m;
-    sm[grp][l32] = m;
-    __syncthreads();
+  int first, count;
+  dec_slots(a, bh, bh, first, count);
+  const int n = min(max(a.length[bh], 0), a.C), nc = (n + 31) / 32, tiles = dec_tiles<32>(n, a.T);
+  int t = part * 8 + grp;
+  float x[PF], old = 0.f, w = 1.f;          // a tile's first rows of logits; its keys' importance and norms
+  auto fetch = [&]() __attribute__((always_inline)) {
+    if (t >= tiles) return;
+    const DecF32In lp = a.logits + ((long long)bh * a.max_tiles + t) * a.R * 32 + l32;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = fmaxf(m, sm[i][l32]);
-    const float ref = m == kDecNegInf ? 0.f : m;
-    float l = 0.f;
-    for (int s = grp; s < count; s += 8) l += rv ? ml[s * 64 + 32] * fast_exp2(ml[s * 64] - ref) : 0.f;
+    for (int i = 0; i < PF; ++i) x[i] = lp[min(i, a.R - 1) * 32];
+    const int key = t * 32 + l32;
+    if (key < n) {
+      old = a.imp[bh * a.imp_stride + key];
+      if (a.norm) w = a.norm[bh * a.norm_stride + key];
+    }
+  };
+  fetch();
+  {
+    const DecF32In ml = a.part_ml + (long long)first * 2 * RS + l32;
+    const bool rv = l32 < a.R;
+    float m = kDecNegInf, l = 0.f;
+    for (int s = grp; s < count; s += 8) {
+      const float ms = rv ? ml[s * 2 * RS] : kDecNegInf, ls = rv ? ml[s * 2 * RS + RS] : 0.f;
+      const float mn = fmaxf(m, ms), ref = mn == kDecNegInf ? 0.f : mn;
+      l = l * fast_exp2(m - ref) + ls * fast_exp2(ms - ref);
+      m = mn;
+    }
+    sm[grp][l32] = m;
     sl[grp][l32] = l;
     __syncthreads();
     if (grp == 0) {
+#pragma unroll
+      for (int i = 1; i < 8; ++i) m = fmaxf(m, sm[i][l32]);
+      const float ref = m == kDecNegInf ? 0.f : m;
       l = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) l += sl[i][l32];
-      // log2 of l and of w = 2^(-decay (T - 1 - t)); rows that see nothing give no weight
-      bias[l32] = l == 0.f ? -kDecNegInf : ref + fast_log2(l) + a.decay_log2 * (float)(a.T - 1 - l32 % a.T);
+      for (int i = 0; i < 8; ++i) l += sl[i][l32] * fast_exp2(sm[i][l32] - ref);
+      // log2 of l and of w = 2^(-decay (T - 1 - t)); rows that see nothing, or are none, give no weight
+      bias[l32] = l == 0.f || !rv ? -kDecNegInf : ref + fast_log2(l) + a.decay_log2 * (float)(a.T - 1 - l32 % a.T);
     }
     __syncthreads();
   }
-  if (t >= tiles) return;
-  const float* lp = a.logits + ((long long)bh * a.max_tiles + t) * a.R * 32 + l32;
-  float sum = 0.f;
-#pragma unroll 4
-  for (int r = 0; r < a.R; ++r) sum += fast_exp2(lp[r * 32] - bias[r]);
-  if (t < nc) {
-    const int key = t * 32 + l32;
-    if (key < n) {
-      const float old = a.imp[bh * a.imp_stride + key] * fast_exp2(-a.decay_log2 * (float)a.T);
-      a.imp_out[bh * a.impo_stride + key] = old + (a.norm ? a.norm[bh * a.norm_stride + key] : 1.f) * sum;
+  const float keep = fast_exp2(-a.decay_log2 * (float)a.T);
+  while (t < tiles) {
+    float sum = 0.f;
+    const float o = old, nw = w;
+#pragma unroll
+    for (int i = 0; i < PF; ++i) sum += fast_exp2(x[i] - bias[i]);
+    const DecF32In lp = a.logits + ((long long)bh * a.max_tiles + t) * a.R * 32 + l32;
+    for (int r0 = PF; r0 < a.R; r0 += PF) {
+#pragma unroll
+      for (int i = 0; i < PF; ++i) x[i] = lp[min(r0 + i, a.R - 1) * 32];
+#pragma unroll
+      for (int i = 0; i < PF; ++i) sum += fast_exp2(x[i] - bias[r0 + i]);
     }
-  } else {
-    const int u = (t - nc) * 32 + l32;
-    if (u < a.T) {
-      float w = 1.f;
-      if (a.norm) {
-        const u16* vp = a.v + b * a.vs[0] + hkv * a.vs[1] + u * a.vs[2];
-        w = 0.f;
-        for (int d = 0; d < a.D; ++d) w += fabsf(E::to_f32(vp[d * a.vs[3]]));
+    const int now = t;
+    t += 8 * a.per_head;
+    fetch();
+    if (now < nc) {
+      const int key = now * 32 + l32;
+      if (key < n) a.imp_out[bh * a.impo_stride + key] = o * keep + (a.norm ? nw : 1.f) * sum;
+    } else {
+      const int u = (now - nc) * 32 + l32;
+      if (u < a.T) {
+        float nu = 1.f;
+        if (a.norm) {
+          const DecIn vp = a.v + b * a.vs[0] + hkv * a.vs[1] + u * a.vs[2];
+          nu = 0.f;
+          for (int d = 0; d < a.D; ++d) nu += fabsf(E::to_f32(vp[d * a.vnc]));
+        }
+        a.new_imp[(long long)bh * a.T + u] = nu * sum;
       }
-      a.new_imp[(long long)bh * a.T + u] = w * sum;
     }
   }
 }
@@ -845,7 +1287,7 @@ constexpr int dec_replay_rows() { return DP > 128 ? 32 : 64; }
 // way, against the rows' Q in LDS. More rows than that has room for take K again (from L2 mostly), adding to what
 // the rows before left.
 template <typename E, int DP, int VEC>
-__global__ __launch_bounds__(256, 2) void decode_replay_kernel(const DecArgs a) {
+__global__ __launch_bounds__(256, 2) void decode_replay_kernel(const DecArgs args) {
   constexpr int NDC = DP / 16, CPR = DP / 8, TILE = 64 * DP, CH = dec_replay_rows<DP>();
   __shared__ __attribute__((aligned(1024))) unsigned char lds[4][TILE];
   __shared__ __attribute__((aligned(1024))) unsigned char lds_q[CH * DP * 2];
@@ -854,24 +1296,23 @@ __global__ __launch_bounds__(256, 2) void decode_replay_kernel(const DecArgs a) 
   const int lane = threadIdx.x & 63, l32 = lane & 31, hh = lane >> 5;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
+  const DecArgs a = dec_hold<kDecReplayArgs, 5>(args);
   DecShare sh = dec_share<32, 4>(a, 1, a.A);
   while (sh.pos < sh.hi) {
     const int bh = sh.bh, b = bh / a.Hkv, hkv = bh - b * a.Hkv;
-    const int n = dec_len(a, bh);
+    const int n = dec_share_len(sh);
     const int nc = (n + 31) / 32, tiles = dec_tiles<32>(n, a.A);
-    const int t0 = (int)(sh.pos - sh.base), t1 = (int)min((long long)tiles, t0 + (sh.hi - sh.pos));
+    const int t0 = sh.pos - sh.base, t1 = min(tiles, t0 + sh.hi - sh.pos);
     sh.pos += t1 - t0;
-    if (t1 == tiles) {
-      sh.base = sh.pos;
-      ++sh.bh;
-    }
+    if (t1 == tiles) dec_share_next(a, sh);
     const int na = dec_path_len(a, b), rows = a.G * na;
-    const int* path = a.path ? a.path + (long long)b * a.A : nullptr;
+    const DecI32In path = a.path ? a.path + (long long)b * a.A : (DecI32In) nullptr;
     const float keep = fast_exp2(-a.decay_log2 * (float)na);
 
-    u32x4 kx[VEC ? NDC : 1];
+    u32x4 kx[VEC ? NDC : 1] = {};
+    const DecRows hr = dec_rows(a, b, hkv);
     auto load = [&](int t) __attribute__((always_inline)) {
-      if constexpr (VEC) dec_load_rows<DP, 32, 64>(a.kc + b * a.kcs[0] + hkv * a.kcs[1], a.kcs[2], t * 32, n, a.D, lane, kx);
+      if constexpr (VEC) dec_load_rows<DP, 32, 64>(hr.kc, hr.kcs, t * 32, n, a.D, lane, kx);
     };
     for (int r0 = 0; r0 == 0 || r0 < rows; r0 += CH) {
       if (VEC && t0 + wv < min(t1, nc)) load(t0 + wv);
@@ -896,7 +1337,12 @@ __global__ __launch_bounds__(256, 2) void decode_replay_kernel(const DecArgs a) 
         u32x4 x = {0u, 0u, 0u, 0u};
         if (r < rows) {
           const int g = r / na, node = path ? path[r - g * na] : r - g * na;
-          x = (dec_load8<VEC>(a.q + b * a.qs[0] + (hkv * a.G + g) * a.qs[1] + node * a.qs[2], a.qs[3], ch, a.D) & a.qand) ^ a.qxor;
+          const DecIn qp = a.q + b * a.qs[0] + (hkv * a.G + g) * a.qs[1] + node * a.qs[2];
+          if (VEC) {
+            if (8 * ch < a.D) x = (*(const FE_GLOBAL u32x4*)(qp + 8 * ch) & a.qand) ^ a.qxor;
+          } else {
+            x = (dec_load8(qp, a.qc, ch, a.D) & a.qand) ^ a.qxor;
+          }
         }
         *(u32x4*)(lds_q + dec_k_at<DP>(e / CPR, ch)) = x;
       }
@@ -914,13 +1360,17 @@ __global__ __launch_bounds__(256, 2) void decode_replay_kernel(const DecArgs a) 
           }
           if (t + 4 < min(t1, nc)) load(t + 4);
         } else {
-          const u16* kp = tail ? a.k + b * a.ks[0] + hkv * a.ks[1] : a.kc + b * a.kcs[0] + hkv * a.kcs[1];
-          const long long krs = tail ? a.ks[2] : a.kcs[2], kcs = tail ? a.ks[3] : a.kcs[3];
+          const DecIn kp = tail ? hr.k : hr.kc;
+          const long long krs = tail ? hr.ks : hr.kcs, kcs = VEC ? 1 : tail ? a.knc : a.kcc;
 #pragma unroll 1
           for (int i = 0; i < NDC; ++i) {
             const int e = i * 64 + lane, key = kb + e / CPR, ch = e % CPR;
             const int row = tail && path && key < krows ? path[key] : key;   // new rows in the path's order
-            const u32x4 x = key < krows ? dec_load8<VEC>(kp + row * krs, kcs, ch, a.D) : (u32x4){0u, 0u, 0u, 0u};
+            u32x4 x = {0u, 0u, 0u, 0u};
+            if (key < krows) {
+              if (!VEC) x = dec_load8(kp + row * krs, kcs, ch, a.D);
+              else if (8 * ch < a.D) x = *(const FE_GLOBAL u32x4*)(kp + row * krs + 8 * ch);
+            }
             *(u32x4*)(lds[wv] + dec_k_at<DP>(e / CPR, ch)) = x;
           }
         }
@@ -950,7 +1400,7 @@ __global__ __launch_bounds__(256, 2) void decode_replay_kernel(const DecArgs a) 
         if (!tail) {
           if (key < n) {
             const float w = a.norm ? a.norm[bh * a.norm_stride + key] : 1.f;
-            float* to = a.imp_out + bh * a.impo_stride + key;
+            const DecF32 to = a.imp_out + bh * a.impo_stride + key;
             *to = (r0 ? *to : a.imp[bh * a.imp_stride + key] * keep) + w * sum;
           }
         } else if (key < a.A) {
@@ -958,12 +1408,13 @@ __global__ __launch_bounds__(256, 2) void decode_replay_kernel(const DecArgs a) 
           if (key < na) {
             w = 1.f;
             if (a.norm) {
-              const u16* vp = a.v + b * a.vs[0] + hkv * a.vs[1] + (path ? path[key] : key) * a.vs[2];
+              const DecIn vp = hr.v + (path ? path[key] : key) * hr.vs;
+              const long long vnc = VEC ? 1 : a.vnc;
               w = 0.f;
-              for (int d = 0; d < a.D; ++d) w += fabsf(E::to_f32(vp[d * a.vs[3]]));
+              for (int d = 0; d < a.D; ++d) w += fabsf(E::to_f32(vp[d * vnc]));
             }
           }
-          float* to = a.new_imp + (long long)bh * a.A + key;
+          const DecF32 to = a.new_imp + (long long)bh * a.A + key;
           *to = (r0 ? *to : 0.f) + (key < na ? w * sum : 0.f);
         }
       }
@@ -973,7 +1424,7 @@ __global__ __launch_bounds__(256, 2) void decode_replay_kernel(const DecArgs a) 
 
 #define FE_DEC_DIMS(X) X(64) X(96) X(128) X(192) X(256)
 #define FE_DEC_ROW(DP, E, T)                                                                                            \
-  {DP, T, {(const void*)decode_rows_kernel<E, DP, 0>, (const void*)decode_rows_kernel<E, DP, 1>},                       \
+  {DP, T, (const void*)decode_few_kernel<E, DP>, {(const void*)decode_rows_kernel<E, DP, 0>, (const void*)decode_rows_kernel<E, DP, 1>},                       \
    {(const void*)decode_wide_kernel<E, DP, 4>, (const void*)decode_wide_kernel<E, DP, (DP > 128 ? 4 : 8)>},              \
    (const void*)decode_join_kernel<E, DP>,                                                                              \
    {(const void*)decode_replay_kernel<E, DP, 0>, (const void*)decode_replay_kernel<E, DP, 1>}},
@@ -982,6 +1433,7 @@ __global__ __launch_bounds__(256, 2) void decode_replay_kernel(const DecArgs a) 
 // waves, and of eight where their registers allow it.
 struct DecKernels {
   int dp, dtype;
+  const void* few;
   const void* rows[2];
   const void* wide[2];
   const void* join;
@@ -997,9 +1449,9 @@ const DecKernels& dec_kernels(int64_t D, int dtype) {
 
 void append_decode_resources(std::string& out) {
   for (const auto& e : kDecKernels) {
-    const void* fns[7] = {e.rows[1], e.wide[0], e.wide[1], e.join, e.replay[1], e.rows[0], e.replay[0]};
-    const char* names[7] = {"decode_rows", "decode_wide4", "decode_wide8", "decode_join", "decode_replay", "decode_rows_elements", "decode_replay_elements"};
-    for (int i = 0; i < 7; ++i) {
+    const void* fns[8] = {e.rows[1], e.wide[0], e.wide[1], e.join, e.replay[1], e.rows[0], e.replay[0], e.few};
+    const char* names[8] = {"decode_rows", "decode_wide4", "decode_wide8", "decode_join", "decode_replay", "decode_rows_elements", "decode_replay_elements", "decode_few"};
+    for (int i = 0; i < 8; ++i) {
       if (i == 2 && e.dp > 128) continue;
       hipFuncAttributes attr;
       if (hipFuncGetAttributes(&attr, fns[i]) != hipSuccess) continue;
@@ -1037,15 +1489,16 @@ int dec_check(const char* who, int64_t B, int64_t Hq, int64_t Hkv, int64_t T, in
     set_error(w + ": scale must be finite, recency_decay finite and nonnegative");
     return FE_ERR_INVALID;
   }
+  const int64_t most = std::max<int64_t>((Hq / Hkv * T + 31) / 32, 1);   // segments of a head
   if (C > (1LL << 30) || Hq / Hkv > 32767 || B > (1LL << 30) || Hkv > (1LL << 30) || B * Hkv > (1LL << 24) ||
-      B * Hkv * ((C + T + 127) / 128) > 0x7fffffffLL || B * Hkv * (((Hq / Hkv) * T + 31) / 32) > 0x7fffffLL) {
+      B * Hkv * most > 0x7fffffLL || (double)(B * Hkv * most) * (double)((C + 31) / 32 + (T + 31) / 32) > 2147483647.) {
     set_error(w + ": sizes exceed the supported range");
     return FE_ERR_UNSUPPORTED;
   }
   return FE_OK;
 }
 
-int dec_strides(const char* who, const int64_t* const* in, long long (*out[])[4], int count) {
+int dec_strides(const char* who, const int64_t* const* in, long long (*out)[4], int count) {
   for (int i = 0; i < count; ++i) {
     if (!in[i]) {
       set_error(std::string(who) + ": null stride array");
@@ -1056,7 +1509,7 @@ int dec_strides(const char* who, const int64_t* const* in, long long (*out[])[4]
         set_error(std::string(who) + ": negative strides are not supported");
         return FE_ERR_INVALID;
       }
-      (*out[i])[j] = in[i][j];
+      out[i][j] = in[i][j];
     }
   }
   return FE_OK;
@@ -1064,14 +1517,17 @@ int dec_strides(const char* who, const int64_t* const* in, long long (*out[])[4]
 
 // How an attention launch is laid out; the same for the workspace's size and the call, whatever the layout of rows.
 struct DecPlan {
-  bool wide;
+  bool few, wide;
+  int S;                       // splits of a head (few)
+  int RS;                      // rows of a slot
   int waves, RB, RW, nb;       // waves of a wide block; segments of a head, 32-row tiles of one, blocks
   long long slots;
   size_t o, ml, seg, logits, bytes;   // offsets
 };
-DecPlan dec_plan(int64_t BH, int64_t R, int64_t C, int64_t T, int64_t DP, bool vec, bool weights) {
+DecPlan dec_plan(int64_t BH, int64_t R, int64_t C, int64_t T, int64_t DP, bool vec, bool near, bool weights) {
   DecPlan p = {};
   const int64_t RT = (R + 31) / 32;
+  p.few = vec && near && R <= 16;
   p.wide = vec && RT > 1;
   if (p.wide) {
     p.waves = DP > 128 || RT <= 4 ? 4 : 8;
@@ -1086,20 +1542,28 @@ DecPlan dec_plan(int64_t BH, int64_t R, int64_t C, int64_t T, int64_t DP, bool v
   const int64_t resident = p.wide ? (p.waves == 8 || DP > 128 ? 256 : 512) : (DP > 128 ? 256 : 512);
   p.nb = (int)std::max<int64_t>(1, std::min(resident, p.wide ? tiles : (tiles + 3) / 4));
   p.slots = p.nb + BH * p.RB;
+  p.RS = 32 * p.RW;
+  if (p.few) {
+    p.S = (int)std::max<int64_t>(1, std::min(resident / BH, (tiles / BH + 3) / 4));
+    p.nb = (int)(p.S * BH);
+    p.slots = p.nb;
+    p.RS = 16;
+  }
   auto area = [&](size_t elems) {
     const size_t at = p.bytes;
     p.bytes += (elems * 4 + 255) / 256 * 256;
     return at;
   };
-  p.o = area((size_t)p.slots * p.RW * 32 * DP);
-  p.ml = area((size_t)p.slots * p.RW * 64);
+  p.o = area((size_t)p.slots * p.RS * DP);
+  p.ml = area((size_t)p.slots * p.RS * 2);
   p.seg = area((size_t)BH * p.RB * 2);
   p.logits = p.bytes;
   if (weights && R <= kDecLogitRows) area((size_t)BH * ((C + 31) / 32 + (T + 31) / 32) * R * 32);
   return p;
 }
 
-int dec_launch(const char* who, const void* fn, dim3 grid, dim3 block, DecArgs& a, hipStream_t stream) {
+template <typename A>
+int dec_launch(const char* who, const void* fn, dim3 grid, dim3 block, A& a, hipStream_t stream) {
   void* args[] = {&a};
   hipError_t err = hipLaunchKernel(fn, grid, block, args, 0, stream);
   if (err != hipSuccess) {
@@ -1109,7 +1573,7 @@ int dec_launch(const char* who, const void* fn, dim3 grid, dim3 block, DecArgs& 
   return FE_OK;
 }
 
-int dec_replay(const char* who, const DecKernels& kn, int vec, DecArgs& a, hipStream_t stream) {
+int dec_replay(const char* who, const DecKernels& kn, bool vec, DecArgs& a, hipStream_t stream) {
   // as many blocks as the card holds at once, of at least a tile a wave
   const long long tiles = (long long)a.BH * ((a.C + 31) / 32 + (a.A + 31) / 32);
   a.nb = (int)std::max<long long>(1, std::min<long long>(kn.dp > 128 ? 512 : 768, (tiles + 3) / 4));
@@ -1127,13 +1591,38 @@ extern "C" size_t fe_decode_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, 
       B * Hkv * ((Hq / Hkv * T + 31) / 32) > 0x7fffffLL)
     return 0;
   const int64_t dp = dec_kernels(D, 0).dp;
-  return std::max(dec_plan(B * Hkv, Hq / Hkv * T, C, T, dp, false, weights != 0).bytes,
-                  dec_plan(B * Hkv, Hq / Hkv * T, C, T, dp, true, weights != 0).bytes);
+  size_t bytes = 0;
+  for (int i = 0; i < 3; ++i) bytes = std::max(bytes, dec_plan(B * Hkv, Hq / Hkv * T, C, T, dp, i > 0, i > 1, weights != 0).bytes);
+  return bytes;
 }
 
-// The signs and zeros of Q that let a launch use a positive scale: a negative one runs as |scale| on -Q, a zero one
-// as 1 on zeros (masked logits, -inf, times a zero scale would be NaN).
-static void dec_scale(DecArgs& a, float scale, float decay) {
+template <typename P, typename Q>
+static void dec_set(P& to, Q* from) { to = (P)(uintptr_t)from; }
+
+// What every launch needs. A negative scale runs as |scale| on -Q, a zero one as 1 on zeros (a masked logit, -inf,
+// times a zero scale would be NaN).
+static void dec_common(DecArgs& a, const void* q, const void* k, const void* v, const void* k_cache, const int32_t* length,
+                       const long long (*st)[4], int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t C, int64_t D, float scale,
+                       float decay) {
+  dec_set(a.q, q);
+  dec_set(a.k, k);
+  dec_set(a.v, v);
+  dec_set(a.kc, k_cache);
+  dec_set(a.length, length);
+  std::copy(st[0], st[0] + 3, a.qs);
+  std::copy(st[1], st[1] + 3, a.ks);
+  std::copy(st[2], st[2] + 3, a.vs);
+  std::copy(st[3], st[3] + 3, a.kcs);
+  a.qc = st[0][3];
+  a.knc = st[1][3];
+  a.vnc = st[2][3];
+  a.kcc = st[3][3];
+  a.T = a.A = (int)T;
+  a.C = (int)C;
+  a.D = (int)D;
+  a.G = (int)(Hq / Hkv);
+  a.Hkv = (int)Hkv;
+  a.BH = (int)(B * Hkv);
   a.qand = scale == 0.f ? 0u : ~0u;
   a.qxor = scale < 0.f ? 0x80008000u : 0u;
   a.scale_log2 = scale == 0.f ? 1.f : (float)(fabs((double)scale) * 1.4426950408889634);
@@ -1159,9 +1648,8 @@ extern "C" int fe_decode_attention(const void* q, const void* k, const void* v, 
     set_error(std::string(who) + ": invalid row stride");
     return FE_ERR_INVALID;
   }
-  DecArgs a = {};
   const int64_t* in[5] = {q_strides, k_strides, v_strides, k_cache_strides, v_cache_strides};
-  long long(*st[5])[4] = {&a.qs, &a.ks, &a.vs, &a.kcs, &a.vcs};
+  long long st[5][4];
   if (int rc = dec_strides(who, in, st, 5)) return rc;
   const DecKernels& kn = dec_kernels(D, dtype);
   const size_t need = fe_decode_workspace_bytes(B, Hq, Hkv, T, C, D, importance != nullptr);
@@ -1169,59 +1657,111 @@ extern "C" int fe_decode_attention(const void* q, const void* k, const void* v, 
     set_error(std::string(who) + ": workspace too small; need " + std::to_string(need) + " bytes");
     return FE_ERR_WORKSPACE;
   }
-  a.q = (const u16*)q;
-  a.k = (const u16*)k;
-  a.v = (const u16*)v;
-  a.kc = (const u16*)k_cache;
-  a.vc = (const u16*)v_cache;
-  a.length = length;
-  a.tree = tree;
+  const bool vec = vec_ok(q, st[0], B, Hq, T, D) && vec_ok(k, st[1], B, Hkv, T, D) && vec_ok(v, st[2], B, Hkv, T, D) &&
+                   vec_ok(k_cache, st[3], B, Hkv, C, D) && vec_ok(v_cache, st[4], B, Hkv, C, D);
+  DecArgs a = {};
+  dec_common(a, q, k, v, k_cache, length, st, B, Hq, Hkv, T, C, D, scale, recency_decay);
+  dec_set(a.vc, v_cache);
+  std::copy(st[4], st[4] + 3, a.vcs);
+  a.vcc = st[4][3];
+  dec_set(a.tree, tree);
   a.tree_stride = tree_batch_stride;
-  a.out = (u16*)out;
-  a.lse = lse;
-  a.lse_in = lse;
-  a.T = (int)T;
-  a.A = (int)T;
-  a.C = (int)C;
-  a.D = (int)D;
-  a.G = (int)(Hq / Hkv);
-  a.Hkv = (int)Hkv;
-  a.BH = (int)(B * Hkv);
   a.R = a.G * a.T;
-  dec_scale(a, scale, recency_decay);
-  const int vec = vec_ok(q, a.qs, B, Hq, T, D) && vec_ok(k, a.ks, B, Hkv, T, D) && vec_ok(v, a.vs, B, Hkv, T, D) &&
-                  vec_ok(k_cache, a.kcs, B, Hkv, C, D) && vec_ok(v_cache, a.vcs, B, Hkv, C, D);
-  const DecPlan p = dec_plan(a.BH, a.R, C, T, kn.dp, vec, importance != nullptr);
+  // the few-rows kernel takes 32-bit row strides, and heads and batch rows as grid axes
+  const bool near = std::max({st[1][2], st[2][2], st[3][2], st[4][2]}) <= 0x7fffffffLL && Hkv <= 65535 && B <= 65535;
+  const DecPlan p = dec_plan(a.BH, a.R, C, T, kn.dp, vec, near, importance != nullptr);
   const bool logits = importance && a.R <= kDecLogitRows;
+  char* ws = (char*)workspace;
   a.RB = p.RB;
   a.RW = p.RW;
   a.nb = p.nb;
   a.max_tiles = (int)((C + 31) / 32 + (T + 31) / 32);
-  a.part_o = (float*)((char*)workspace + p.o);
-  a.part_ml = (float*)((char*)workspace + p.ml);
-  a.seg = (int*)((char*)workspace + p.seg);
-  a.logits = logits ? (float*)((char*)workspace + p.logits) : nullptr;
-  a.imp = importance;
-  a.imp_stride = importance_stride;
-  a.norm = value_norm;
-  a.norm_stride = value_norm_stride;
-  a.imp_out = importance_out;
-  a.impo_stride = importance_out_stride;
-  a.new_imp = new_importance;
+  dec_set(a.part_o, ws + p.o);
+  dec_set(a.part_ml, ws + p.ml);
+  dec_set(a.seg, ws + p.seg);
+  if (logits) dec_set(a.logits, ws + p.logits);
   hipStream_t stream = (hipStream_t)hip_stream;
-  if (p.wide) {
+  if (p.few) {
+    DecFewArgs f = {};
+    f.q = a.q;
+    f.k = a.k;
+    f.v = a.v;
+    f.kc = a.kc;
+    f.vc = a.vc;
+    f.length = a.length;
+    f.tree = a.tree;
+    f.part_o = a.part_o;
+    f.part_ml = a.part_ml;
+    f.logits = a.logits;
+    f.qb = st[0][0], f.qh = st[0][1], f.qn = st[0][2];
+    f.kb = st[1][0], f.kh = st[1][1], f.kn = (u32)st[1][2];
+    f.vb = st[2][0], f.vh = st[2][1], f.vn = (u32)st[2][2];
+    f.kcb = st[3][0], f.kch = st[3][1], f.kcn = (u32)st[3][2];
+    f.vcb = st[4][0], f.vch = st[4][1], f.vcn = (u32)st[4][2];
+    f.tree_stride = tree_batch_stride;
+    f.T = a.T;
+    f.C = a.C;
+    f.D = a.D;
+    f.R = a.R;
+    f.S = p.S;
+    f.max_tiles = a.max_tiles;
+    f.qand = a.qand;
+    f.qxor = a.qxor;
+    f.scale_log2 = a.scale_log2;
+    if (int rc = dec_launch(who, kn.few, dim3((unsigned)p.S, (unsigned)Hkv, (unsigned)B), dim3(256), f, stream)) return rc;
+  } else if (p.wide) {
     if (int rc = dec_launch(who, kn.wide[p.waves == 8], dim3((unsigned)p.nb), dim3(64 * p.waves), a, stream)) return rc;
   } else {
     if (int rc = dec_launch(who, kn.rows[vec], dim3((unsigned)p.nb), dim3(256), a, stream)) return rc;
   }
+  DecJoinArgs o = {};
+  dec_set(o.part_o, ws + p.o);
+  dec_set(o.part_ml, ws + p.ml);
+  dec_set(o.seg, ws + p.seg);
+  o.logits = a.logits;
+  o.length = a.length;
+  dec_set(o.out, out);
+  dec_set(o.lse, lse);
+  o.v = a.v;
+  std::copy(st[2], st[2] + 3, o.vs);
+  o.vnc = st[2][3];
+  o.T = a.T;
+  o.C = a.C;
+  o.D = a.D;
+  o.G = a.G;
+  o.Hkv = a.Hkv;
+  o.BH = a.BH;
+  o.R = a.R;
+  o.RB = a.RB;
+  o.RS = p.RS;
+  o.S = p.S;
+  o.max_tiles = a.max_tiles;
+  o.decay_log2 = a.decay_log2;
   // eight groups on a row where it has many splits, else a group a row
   const long long rows = (long long)a.BH * a.R;
-  a.join_split = p.nb >= 8 * a.BH * a.RB ? 8 : 1;
-  a.join_blocks = (int)((rows * a.join_split + 7) / 8);
-  const long long blocks = a.join_blocks + (logits ? (long long)a.BH * ((a.max_tiles + 7) / 8) : 0);
-  if (int rc = dec_launch(who, kn.join, dim3((unsigned)blocks), dim3(256), a, stream)) return rc;
-  if (logits) return FE_OK;
-  if (!importance) return FE_OK;
+  o.split = p.nb >= 8 * a.BH * a.RB ? 8 : 1;
+  o.out_blocks = (int)((rows * o.split + 7) / 8);
+  long long blocks = o.out_blocks;
+  if (importance) {
+    dec_set(a.imp, importance);
+    a.imp_stride = o.imp_stride = importance_stride;
+    dec_set(a.norm, value_norm);
+    a.norm_stride = o.norm_stride = value_norm_stride;
+    dec_set(a.imp_out, importance_out);
+    a.impo_stride = o.impo_stride = importance_out_stride;
+    dec_set(a.new_imp, new_importance);
+    o.imp = a.imp;
+    o.norm = a.norm;
+    o.imp_out = a.imp_out;
+    o.new_imp = a.new_imp;
+  }
+  if (logits) {
+    o.per_head = (int)std::min<long long>((a.max_tiles + 7) / 8, std::max<long long>(1, kDecJoinBlocks / a.BH));
+    blocks += (long long)a.BH * o.per_head;
+  }
+  if (int rc = dec_launch(who, kn.join, dim3((unsigned)blocks), dim3(256), o, stream)) return rc;
+  if (!importance || logits) return FE_OK;
+  dec_set(a.lse_in, lse);
   return dec_replay(who, kn, vec, a, stream);
 }
 
@@ -1247,33 +1787,23 @@ extern "C" int fe_replay_path(const void* q, const void* k, const void* v, const
     set_error(std::string(who) + ": invalid row stride");
     return FE_ERR_INVALID;
   }
-  DecArgs a = {};
   const int64_t* in[4] = {q_strides, k_strides, v_strides, k_cache_strides};
-  long long(*st[4])[4] = {&a.qs, &a.ks, &a.vs, &a.kcs};
+  long long st[4][4];
   if (int rc = dec_strides(who, in, st, 4)) return rc;
   const DecKernels& kn = dec_kernels(D, dtype);
-  a.q = (const u16*)q;
-  a.k = (const u16*)k;
-  a.v = (const u16*)v;
-  a.kc = (const u16*)k_cache;
-  a.length = length;
-  a.lse_in = lse;
-  a.path = path;
-  a.T = (int)T;
+  const bool vec = vec_ok(q, st[0], B, Hq, T, D) && vec_ok(k, st[1], B, Hkv, T, D) && vec_ok(v, st[2], B, Hkv, T, D) &&
+                   vec_ok(k_cache, st[3], B, Hkv, C, D);
+  DecArgs a = {};
+  dec_common(a, q, k, v, k_cache, length, st, B, Hq, Hkv, T, C, D, scale, recency_decay);
   a.A = (int)A;
-  a.C = (int)C;
-  a.D = (int)D;
-  a.G = (int)(Hq / Hkv);
-  a.Hkv = (int)Hkv;
-  a.BH = (int)(B * Hkv);
-  dec_scale(a, scale, recency_decay);
-  const int vec = vec_ok(q, a.qs, B, Hq, T, D) && vec_ok(k, a.ks, B, Hkv, T, D) && vec_ok(k_cache, a.kcs, B, Hkv, C, D);
-  a.imp = importance;
+  dec_set(a.lse_in, lse);
+  dec_set(a.path, path);
+  dec_set(a.imp, importance);
   a.imp_stride = importance_stride;
-  a.norm = value_norm;
+  dec_set(a.norm, value_norm);
   a.norm_stride = value_norm_stride;
-  a.imp_out = importance_out;
+  dec_set(a.imp_out, importance_out);
   a.impo_stride = importance_out_stride;
-  a.new_imp = new_importance;
+  dec_set(a.new_imp, new_importance);
   return dec_replay(who, kn, vec, a, (hipStream_t)hip_stream);
 }
