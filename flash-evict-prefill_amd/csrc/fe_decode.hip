@@ -46,7 +46,7 @@ constexpr int kDecMaxTokens = 256;   // new tokens of a call
 // Rows of a group up to which the attention leaves its logits for the importance: 8 bytes a row and key, written and
 // read, against the 2 D of reading K again.
 constexpr int kDecLogitRows = 16;
-constexpr int kDecJoinBlocks = 2048;   // blocks that share the importance of all heads
+constexpr int kDecJoinBlocks = 1024;   // blocks that share the importance of all heads
 
 // Pointers to global memory, said to be: a pointer that the compiler loses sight of (dec_hold) would be read with flat
 // instructions, which wait for LDS too.
@@ -111,6 +111,22 @@ struct DecFewArgs {
 };
 static_assert(offsetof(DecFewArgs, pad) <= 4 * 64 && sizeof(DecFewArgs) >= 4 * 64, "argument window");
 
+struct DecFewJoinArgs {
+  DecF32In part_o, part_ml, logits;
+  DecI32In length;
+  FE_GLOBAL u16* out;      // [B, Hq, T, D]
+  DecF32 lse;              // [B, Hq, T]
+  DecF32In imp, norm;
+  DecF32 imp_out, new_imp;
+  DecIn v;
+  long long imp_stride, norm_stride, impo_stride, vb, vh;
+  u32 vn;
+  int T, C, D, R, S, max_tiles;
+  float decay_log2;
+  int pad[8];
+};
+static_assert(offsetof(DecFewJoinArgs, pad) <= 3 * 64 && sizeof(DecFewJoinArgs) >= 3 * 64, "argument window");
+
 struct DecJoinArgs {
   DecF32In part_o, part_ml, logits;
   DecI32In seg, length;
@@ -121,7 +137,6 @@ struct DecJoinArgs {
   DecIn v;
   long long imp_stride, norm_stride, impo_stride, vs[3], vnc;
   int T, C, D, G, Hkv, BH, R, RB, RS, max_tiles;   // RS: rows of a slot
-  int S;                   // splits of a head (decode_few_kernel), or 0: slots by `seg`
   int out_blocks, split;   // blocks of the output; 32-lane groups that share a row
   int per_head;            // blocks of a head's importance
   float decay_log2;
@@ -143,6 +158,7 @@ __device__ __forceinline__ A dec_hold(const A& arg) {
 #pragma unroll
   for (int i = 0; i < NV; ++i) v[i] = p[i];
   if constexpr (NV == 5) asm volatile("" : "+s"(v[0]), "+s"(v[1]), "+s"(v[2]), "+s"(v[3]), "+s"(v[4]));
+  if constexpr (NV == 3) asm volatile("" : "+s"(v[0]), "+s"(v[1]), "+s"(v[2]));
   if constexpr (NV == 4) asm volatile("" : "+s"(v[0]), "+s"(v[1]), "+s"(v[2]), "+s"(v[3]));
   // from here on word by word: a spilled register of 16 words would come back whole for each word of it
   u32 w[NV * 16];
@@ -665,6 +681,152 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_few_kernel(const
   }
 }
 
+// Joins the splits of decode_few_kernel. Blocks below R of a head: an output row, DP / 4 threads on each slot's values,
+// each merging its slots as it reads them (maximum, sum, values), and the groups of threads through LDS. The others:
+// the head's importance, a tile of 32 keys to 32 lanes.
+// What bounds it: two round trips to memory and the reading of its code; on long caches the logits' and weights' bytes.
+template <typename E, int DP>
+__global__ __launch_bounds__(256) void decode_few_join_kernel(const DecFewJoinArgs args) {
+  constexpr int LPR = DP / 4, NG = 256 / LPR, PF = 4;   // threads on a slot, groups of them; loads in flight
+  __shared__ float sm[16][16], sl[16][16], bias[16];
+  __shared__ f32x4 so[NG * LPR];
+  const DecFewJoinArgs a = dec_hold<0, 3>(args);
+  const int tid = threadIdx.x, hkv = (int)blockIdx.y, b = (int)blockIdx.z, bh = b * (int)gridDim.y + hkv;
+  const int n = __builtin_amdgcn_readfirstlane(min(max(a.length[bh], 0), a.C));
+  const int nc = (n + 31) / 32, tiles = nc + (a.T + 31) / 32, share = dec_few_share(tiles, a.S), count = (tiles + share - 1) / share;
+  const long long first = (long long)bh * a.S;
+  if ((int)blockIdx.x < a.R) {
+    const int row = (int)blockIdx.x, grp = tid / LPR, c4 = tid - grp * LPR;
+    const DecF32In ml = a.part_ml + first * 32 + row;
+    const DecF32In po = a.part_o + (first * 16 + row) * DP + 4 * c4;
+    float m = kDecNegInf, l = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int s0 = grp; s0 < count && grp < NG; s0 += PF * NG) {
+      float ms[PF], ls[PF];
+      f32x4 x[PF];
+#pragma unroll
+      for (int i = 0; i < PF; ++i) {
+        const int s = min(s0 + i * NG, count - 1);
+        ms[i] = ml[s * 32];
+        ls[i] = ml[s * 32 + 16];
+        x[i] = *(const FE_GLOBAL f32x4*)(po + (long long)s * 16 * DP);
+      }
+#pragma unroll
+      for (int i = 0; i < PF; ++i)
+        if (i && s0 + i * NG >= count) ms[i] = kDecNegInf, ls[i] = 0.f, x[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      float mn = m;
+#pragma unroll
+      for (int i = 0; i < PF; ++i) mn = fmaxf(mn, ms[i]);
+      const float ref = mn == kDecNegInf ? 0.f : mn, keep = fast_exp2(m - ref);
+      l *= keep;
+      acc *= keep;
+#pragma unroll
+      for (int i = 0; i < PF; ++i) {
+        // a split that this row sees nothing of has a weight of 0 and values of 0
+        const float w = ls[i] * fast_exp2(ms[i] - ref);
+        l += w;
+        acc += w * x[i];
+      }
+      m = mn;
+    }
+    if (grp < NG) {
+      so[tid] = acc;
+      if (c4 == 0) sm[0][grp] = m, sl[0][grp] = l;
+    }
+    __syncthreads();
+    if (grp) return;
+    float mx = m;
+#pragma unroll
+    for (int i = 1; i < NG; ++i) mx = fmaxf(mx, sm[0][i]);
+    const float ref = mx == kDecNegInf ? 0.f : mx, keep = fast_exp2(m - ref);
+    l *= keep;
+    acc *= keep;
+#pragma unroll
+    for (int i = 1; i < NG; ++i) {
+      const float w = fast_exp2(sm[0][i] - ref);
+      l += w * sl[0][i];
+      acc += w * so[i * LPR + c4];
+    }
+    acc *= l == 0.f ? 0.f : 1.f / l;
+    const long long at = (long long)bh * a.R + row;       // [B, Hkv, G, T]
+    if (4 * c4 < a.D) *(FE_GLOBAL u32x2*)(a.out + at * a.D + 4 * c4) = (u32x2){E::pack2(acc[0], acc[1]), E::pack2(acc[2], acc[3])};
+    if (c4 == 0) a.lse[at] = l == 0.f ? kDecNegInf : (ref + fast_log2(l)) * kLn2;
+    return;
+  }
+
+  const int part = (int)blockIdx.x - a.R, step = 8 * ((int)gridDim.x - a.R), l32 = tid & 31;
+  int t = part * 8 + (tid >> 5);
+  if (part * 8 >= tiles) return;
+  float x[PF], old = 0.f, w = 1.f;          // a tile's first rows of logits; its keys' importance and norms
+  {
+    const int row = tid & 15, grp = tid >> 4;
+    const DecF32In ml = a.part_ml + first * 32 + row;
+    float m = kDecNegInf, l = 0.f;
+    if (row < a.R) {
+#pragma unroll 1
+      for (int s = grp; s < count; s += 16) {
+        const float ms = ml[s * 32], ls = ml[s * 32 + 16];
+        const float mn = fmaxf(m, ms), ref = mn == kDecNegInf ? 0.f : mn;
+        l = l * fast_exp2(m - ref) + ls * fast_exp2(ms - ref);
+        m = mn;
+      }
+    }
+    sm[grp][row] = m;
+    sl[grp][row] = l;
+    __syncthreads();
+    if (tid < 16) {
+#pragma unroll 4
+      for (int i = 1; i < 16; ++i) m = fmaxf(m, sm[i][row]);
+      const float ref = m == kDecNegInf ? 0.f : m;
+      l = 0.f;
+#pragma unroll 4
+      for (int i = 0; i < 16; ++i) l += sl[i][row] * fast_exp2(sm[i][row] - ref);
+      // log2 of l and of w = 2^(-decay (T - 1 - t)); rows that see nothing, or are none, give no weight
+      bias[row] = l == 0.f || row >= a.R ? -kDecNegInf : ref + fast_log2(l) + a.decay_log2 * (float)(a.T - 1 - row % a.T);
+    }
+    __syncthreads();
+  }
+  const float keep = fast_exp2(-a.decay_log2 * (float)a.T);
+#pragma unroll 1
+  for (; t < tiles; t += step) {
+    const DecF32In lp = a.logits + ((long long)bh * a.max_tiles + t) * a.R * 32 + l32;
+    const int key = t * 32 + l32;
+#pragma unroll
+    for (int i = 0; i < PF; ++i) x[i] = lp[min(i, a.R - 1) * 32];
+    if (key < n) {
+      old = a.imp[bh * a.imp_stride + key];
+      if (a.norm) w = a.norm[bh * a.norm_stride + key];
+    }
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < PF; ++i) sum += fast_exp2(x[i] - bias[i]);
+#pragma unroll 1
+    for (int r0 = PF; r0 < a.R; r0 += PF) {
+#pragma unroll
+      for (int i = 0; i < PF; ++i) x[i] = lp[min(r0 + i, a.R - 1) * 32];
+#pragma unroll
+      for (int i = 0; i < PF; ++i) sum += fast_exp2(x[i] - bias[r0 + i]);
+    }
+    if (t < nc) {
+      if (key < n) a.imp_out[bh * a.impo_stride + key] = old * keep + w * sum;
+    } else if (key - nc * 32 < a.T) {
+      const int u = key - nc * 32;
+      float nu = 1.f;
+      if (a.norm) {
+        const FE_GLOBAL u32x4* vp = (const FE_GLOBAL u32x4*)(a.v + b * a.vb + hkv * a.vh + (unsigned long long)u * a.vn);
+        nu = 0.f;
+        for (int d = 0; d < a.D / 8; ++d) {
+          const u32x4 y = vp[d];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) nu += fabsf(E::to_f32((u16)y[i])) + fabsf(E::to_f32((u16)(y[i] >> 16)));
+        }
+      }
+      a.new_imp[(long long)bh * a.T + u] = nu * sum;
+    }
+  }
+}
+
 // What bounds it: HBM. Few rows leave the matrix and vector units mostly idle, so every wave keeps the next 32 keys'
 // K and V on the way to registers while it works on these.
 template <typename E, int DP, int VEC>
@@ -1074,15 +1236,9 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void decode_wide_kernel(
 }
 
 // A segment's first slot and its number of slots.
-__device__ __forceinline__ void dec_slots(const DecJoinArgs& a, int bh, int sg, int& first, int& count) {
-  if (a.S) {
-    const int n = min(max(a.length[bh], 0), a.C), tiles = dec_tiles<32>(n, a.T), share = dec_few_share(tiles, a.S);
-    first = bh * a.S;
-    count = (tiles + share - 1) / share;
-  } else {
-    first = a.seg[2 * sg];
-    count = a.seg[2 * sg + 1] - first + 1;
-  }
+__device__ __forceinline__ void dec_slots(const DecJoinArgs& a, int sg, int& first, int& count) {
+  first = a.seg[2 * sg];
+  count = a.seg[2 * sg + 1] - first + 1;
 }
 
 // Blocks below out_blocks: out = sum_s w_s O_s / sum w_s with w_s = l_s 2^(m_s - m), eight 32-lane groups a block,
@@ -1106,7 +1262,7 @@ __global__ __launch_bounds__(256) void decode_join_kernel(const DecJoinArgs args
     const int bh = rv ? gr / a.R : 0, r = rv ? gr - bh * a.R : 0;
     const int sgr = a.RB == 1 ? 0 : r / RS, row = r - sgr * RS;
     int first, count;
-    dec_slots(a, bh, bh * a.RB + sgr, first, count);
+    dec_slots(a, bh * a.RB + sgr, first, count);
     if (!rv) count = 0;
     const DecF32In ml = a.part_ml + (long long)first * 2 * RS + row;
     const DecF32In po = a.part_o + ((long long)first * RS + row) * DP + 4 * l32;
@@ -1189,7 +1345,7 @@ __global__ __launch_bounds__(256) void decode_join_kernel(const DecJoinArgs args
   const int blk = (int)blockIdx.x - a.out_blocks, bh = blk / a.per_head, part = blk - bh * a.per_head;
   const int b = bh / a.Hkv, hkv = bh - b * a.Hkv;
   int first, count;
-  dec_slots(a, bh, bh, first, count);
+  dec_slots(a, bh, first, count);
   const int n = min(max(a.length[bh], 0), a.C), nc = (n + 31) / 32, tiles = dec_tiles<32>(n, a.T);
   int t = part * 8 + grp;
   float x[PF], old = 0.f, w = 1.f;          // a tile's first rows of logits; its keys' importance and norms
@@ -1424,7 +1580,7 @@ __global__ __launch_bounds__(256, 2) void decode_replay_kernel(const DecArgs arg
 
 #define FE_DEC_DIMS(X) X(64) X(96) X(128) X(192) X(256)
 #define FE_DEC_ROW(DP, E, T)                                                                                            \
-  {DP, T, (const void*)decode_few_kernel<E, DP>, {(const void*)decode_rows_kernel<E, DP, 0>, (const void*)decode_rows_kernel<E, DP, 1>},                       \
+  {DP, T, {(const void*)decode_few_kernel<E, DP>, (const void*)decode_few_join_kernel<E, DP>}, {(const void*)decode_rows_kernel<E, DP, 0>, (const void*)decode_rows_kernel<E, DP, 1>},                       \
    {(const void*)decode_wide_kernel<E, DP, 4>, (const void*)decode_wide_kernel<E, DP, (DP > 128 ? 4 : 8)>},              \
    (const void*)decode_join_kernel<E, DP>,                                                                              \
    {(const void*)decode_replay_kernel<E, DP, 0>, (const void*)decode_replay_kernel<E, DP, 1>}},
@@ -1433,7 +1589,7 @@ __global__ __launch_bounds__(256, 2) void decode_replay_kernel(const DecArgs arg
 // waves, and of eight where their registers allow it.
 struct DecKernels {
   int dp, dtype;
-  const void* few;
+  const void* few[2];          // and its join
   const void* rows[2];
   const void* wide[2];
   const void* join;
@@ -1449,9 +1605,9 @@ const DecKernels& dec_kernels(int64_t D, int dtype) {
 
 void append_decode_resources(std::string& out) {
   for (const auto& e : kDecKernels) {
-    const void* fns[8] = {e.rows[1], e.wide[0], e.wide[1], e.join, e.replay[1], e.rows[0], e.replay[0], e.few};
-    const char* names[8] = {"decode_rows", "decode_wide4", "decode_wide8", "decode_join", "decode_replay", "decode_rows_elements", "decode_replay_elements", "decode_few"};
-    for (int i = 0; i < 8; ++i) {
+    const void* fns[9] = {e.rows[1], e.wide[0], e.wide[1], e.join, e.replay[1], e.rows[0], e.replay[0], e.few[0], e.few[1]};
+    const char* names[9] = {"decode_rows", "decode_wide4", "decode_wide8", "decode_join", "decode_replay", "decode_rows_elements", "decode_replay_elements", "decode_few", "decode_few_join"};
+    for (int i = 0; i < 9; ++i) {
       if (i == 2 && e.dp > 128) continue;
       hipFuncAttributes attr;
       if (hipFuncGetAttributes(&attr, fns[i]) != hipSuccess) continue;
@@ -1708,8 +1864,36 @@ extern "C" int fe_decode_attention(const void* q, const void* k, const void* v, 
     f.qand = a.qand;
     f.qxor = a.qxor;
     f.scale_log2 = a.scale_log2;
-    if (int rc = dec_launch(who, kn.few, dim3((unsigned)p.S, (unsigned)Hkv, (unsigned)B), dim3(256), f, stream)) return rc;
-  } else if (p.wide) {
+    if (int rc = dec_launch(who, kn.few[0], dim3((unsigned)p.S, (unsigned)Hkv, (unsigned)B), dim3(256), f, stream)) return rc;
+    DecFewJoinArgs o = {};
+    o.part_o = (DecF32In)a.part_o;
+    o.part_ml = (DecF32In)a.part_ml;
+    o.logits = (DecF32In)a.logits;
+    o.length = a.length;
+    dec_set(o.out, out);
+    dec_set(o.lse, lse);
+    dec_set(o.imp, importance);
+    dec_set(o.norm, value_norm);
+    dec_set(o.imp_out, importance_out);
+    dec_set(o.new_imp, new_importance);
+    o.v = a.v;
+    o.imp_stride = importance_stride;
+    o.norm_stride = value_norm_stride;
+    o.impo_stride = importance_out_stride;
+    o.vb = f.vb;
+    o.vh = f.vh;
+    o.vn = f.vn;
+    o.T = a.T;
+    o.C = a.C;
+    o.D = a.D;
+    o.R = a.R;
+    o.S = p.S;
+    o.max_tiles = a.max_tiles;
+    o.decay_log2 = a.decay_log2;
+    const int64_t per = logits ? std::min<int64_t>((a.max_tiles + 7) / 8, std::max<int64_t>(1, kDecJoinBlocks / a.BH)) : 0;
+    return dec_launch(who, kn.few[1], dim3((unsigned)(a.R + per), (unsigned)Hkv, (unsigned)B), dim3(256), o, stream);
+  }
+  if (p.wide) {
     if (int rc = dec_launch(who, kn.wide[p.waves == 8], dim3((unsigned)p.nb), dim3(64 * p.waves), a, stream)) return rc;
   } else {
     if (int rc = dec_launch(who, kn.rows[vec], dim3((unsigned)p.nb), dim3(256), a, stream)) return rc;
@@ -1734,7 +1918,6 @@ extern "C" int fe_decode_attention(const void* q, const void* k, const void* v, 
   o.R = a.R;
   o.RB = a.RB;
   o.RS = p.RS;
-  o.S = p.S;
   o.max_tiles = a.max_tiles;
   o.decay_log2 = a.decay_log2;
   // eight groups on a row where it has many splits, else a group a row
