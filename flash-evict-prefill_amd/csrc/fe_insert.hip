@@ -9,11 +9,16 @@
 // wherever they lie, and no row is both read and written: sources are new rows or slots at or past F, targets are
 // vacated slots below F.
 //
-// One 1024-thread workgroup per (b, j): a radix select of the threshold over order keys, one ordered pass that lists
-// the vacated slots and the rows that move, then a row per wave (half a wave on K, half on V).
+//   insert_few_kernel    up to 256 new rows and 256 evicted ones, on caches of up to 32512 slots: one 1024-thread block a
+//                        head. Order keys are staged in LDS; up to eight victims are drawn one by one as the least key (of
+//                        equal ones the highest slot), more are found by a radix select and an ordered pass
+//   insert_list_kernel   otherwise: the same by a radix select over the head's rows in memory; leaves the list of moves
+//   insert_move_kernel   carries it out, the whole card on it
 #include <math.h>
+#include <stddef.h>
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "fe_attn.h"
 #include "fe_internal.h"
@@ -22,195 +27,431 @@
 
 namespace fe {
 
+#define FE_GLOBAL __attribute__((address_space(1)))
+typedef const FE_GLOBAL u16* InsIn;
+typedef FE_GLOBAL u16* InsOut;
+
+constexpr int kInsFew = 256;         // new rows, and evicted ones, of insert_few_kernel
+constexpr int kInsKeys = 32768;      // its candidates (128 KiB of LDS)
+constexpr int kInsDraw = 8;          // victims drawn one by one
+
 struct InsArgs {
-  const u16* k;
-  const u16* v;
-  u16* kc;
-  u16* vc;
-  float* imp;              // [B * Hkv] rows of imp_stride
-  int* pos;
-  float* norm;             // or null
-  int* length;
-  int* seen;
-  const float* new_imp;    // [B * Hkv, A], or null: 0
-  const int* path;         // [B, A], or null: all T
-  int* lists;              // [B * Hkv][2][E]: vacated slots, moving candidates
-  long long ks[4], vs[4], kcs[4], vcs[4];
+  InsIn k, v;
+  InsOut kc, vc;
+  FE_GLOBAL float* imp;    // [B * Hkv] rows of imp_stride
+  FE_GLOBAL int* pos;
+  FE_GLOBAL float* norm;   // or null
+  FE_GLOBAL int* length;
+  FE_GLOBAL int* seen;
+  const FE_GLOBAL float* new_imp;    // [B * Hkv, A], or null: 0
+  const FE_GLOBAL int* path;         // [B, A], or null: all T
+  FE_GLOBAL int* lists;    // [B * Hkv][4 + 2 P]: pairs from the front, rows that stay from the back, n, seen; slots; sources
+  long long kb, kh, kn, vb, vh, vn, kcb, kch, kcn, vcb, vch, vcn;   // strides of batch, head, row
   long long imp_stride, pos_stride, norm_stride;
-  int T, A, C, D, Hkv, budget, recent, E;
-  int bf16, kvec, vvec, kcvec, vcvec;
+  int T, A, C, D, Hkv, budget, recent, P, bf16;
+  int pad;
+  long long kd, vd, kcd, vcd;   // channel strides
 };
+static_assert(offsetof(InsArgs, kd) == 4 * 64, "argument window");
 
-// Order key of a candidate: protected ones above NaN, NaN above every number.
-__device__ __forceinline__ u32 ins_key(float w, bool held) { return held ? 0xffffffffu : min(order_key(w), 0xfffffffeu); }
-
-// Copies row `src` of one operand to slot `dst` by 32 lanes (l32); returns the lane's sum of absolute values.
-template <bool BF>
-__device__ __forceinline__ float ins_row(const u16* from, long long fcs, int fvec, u16* to, long long tcs, int tvec, int D,
-                                         int l32) {
-  float sum = 0.f;
-  for (int d = 8 * l32; d < D; d += 256) {
-    const u32x4 x = load8(from, fcs, d, D, fvec);
-    if (tvec) {
-      *(u32x4*)(to + d) = x;
-    } else {
+// The arguments, read at once and kept in registers: read where they are used, each costs a trip to host memory.
+__device__ __forceinline__ InsArgs ins_hold(const InsArgs& arg) {
+  InsArgs a = arg;
+  typedef u32 u32x16 __attribute__((ext_vector_type(16), aligned(4)));
+  typedef const __attribute__((address_space(4))) u32x16* args_ptr;
+  const args_ptr p = (args_ptr)__builtin_amdgcn_kernarg_segment_ptr();
+  u32x16 v[4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (d + e < D) to[(long long)(d + e) * tcs] = (u16)(x[e >> 1] >> (16 * (e & 1)));
-    }
+  for (int i = 0; i < 4; ++i) v[i] = p[i];
+  asm volatile("" : "+s"(v[0]), "+s"(v[1]), "+s"(v[2]), "+s"(v[3]));
+  u32 w[64];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const u16 h = (u16)(x[e >> 1] >> (16 * (e & 1)));
-      sum += fabsf(BF ? BF16::to_f32(h) : F16::to_f32(h));
-    }
+  for (int i = 0; i < 64; ++i) {
+    w[i] = v[i / 16][i % 16];
+    asm volatile("" : "+s"(w[i]));
   }
-  return sum;
+  __builtin_memcpy(&a, w, 4 * 64);
+  return a;
 }
 
-__global__ __launch_bounds__(1024) void insert_kernel(const InsArgs a) {
+// Order keys: a drawn victim above everything, then protected candidates, NaN, numbers.
+constexpr u32 kKeyDrawn = 0xffffffffu, kKeyHeld = 0xfffffffeu, kKeyNan = 0xfffffffdu;
+__device__ __forceinline__ u32 ins_key(float w, bool held) { return held ? kKeyHeld : min(order_key(w), kKeyNan); }
+
+// A head: its candidates and what they become.
+struct InsHead {
+  InsIn kn, vn;
+  InsOut kc, vc;
+  FE_GLOBAL float* imp;
+  FE_GLOBAL int* pos;
+  FE_GLOBAL float* norm;
+  const FE_GLOBAL float* fresh;
+  const FE_GLOBAL int* path;
+  int n, seen;
+};
+__device__ __forceinline__ InsHead ins_head(const InsArgs& a, int b, int hkv, int n, int seen) {
+  const long long bh = (long long)b * a.Hkv + hkv;
+  InsHead h;
+  h.kn = a.k + b * a.kb + hkv * a.kh;
+  h.vn = a.v + b * a.vb + hkv * a.vh;
+  h.kc = a.kc + b * a.kcb + hkv * a.kch;
+  h.vc = a.vc + b * a.vcb + hkv * a.vch;
+  h.imp = a.imp + bh * a.imp_stride;
+  h.pos = a.pos + bh * a.pos_stride;
+  h.norm = a.norm ? a.norm + bh * a.norm_stride : a.norm;
+  h.fresh = a.new_imp ? a.new_imp + bh * a.A : a.new_imp;
+  h.path = a.path ? a.path + (long long)b * a.A : a.path;
+  h.n = n;
+  h.seen = seen;
+  return h;
+}
+
+// Carries out `count` moves (pair(j): source candidate and target slot) by NT threads: a 16-byte chunk of K or V a thread,
+// then eight lanes on each row's numbers (a new row's value norm is a sum over its chunks, in a fixed order).
+template <int NT, bool VEC, typename Pair>
+__device__ __forceinline__ void ins_move(const InsArgs& a, const InsHead& h, int count, int tid, Pair pair) {
+  const int CH = (a.D + 7) / 8, per = 2 * CH;
+#pragma unroll 1
+  for (int u = tid; u < count * per; u += NT) {
+    const int j = u / per, e = u - j * per;
+    const bool isv = e >= CH;
+    const int ch = 8 * (isv ? e - CH : e);
+    int src, dst;
+    pair(j, src, dst);
+    const bool fresh = src >= h.n;
+    const int row = fresh ? (h.path ? h.path[src - h.n] : src - h.n) : src;
+    const InsIn from = fresh ? (isv ? h.vn + row * a.vn : h.kn + row * a.kn) : (isv ? (InsIn)h.vc + row * a.vcn : (InsIn)h.kc + row * a.kcn);
+    const InsOut to = isv ? h.vc + dst * a.vcn : h.kc + dst * a.kcn;
+    if (VEC) {
+      *(FE_GLOBAL u32x4*)(to + ch) = *(const FE_GLOBAL u32x4*)(from + ch);
+    } else {
+      const long long fs = fresh ? (isv ? a.vd : a.kd) : (isv ? a.vcd : a.kcd), ts = isv ? a.vcd : a.kcd;
+      for (int d = ch; d < min(ch + 8, a.D); ++d) to[d * ts] = from[d * fs];
+    }
+  }
+#pragma unroll 1
+  for (int j = tid >> 3; j < count; j += NT / 8) {
+    int src, dst;
+    pair(j, src, dst);
+    const bool fresh = src >= h.n;
+    const int at = src - h.n;
+    float s = 0.f;
+    if (fresh && h.norm) {
+      const InsIn from = h.vn + (long long)(h.path ? h.path[at] : at) * a.vn;
+      for (int ch = 8 * (tid & 7); ch < a.D; ch += 64) {
+        u16 x[8];
+        if (VEC) {
+          const u32x4 y = *(const FE_GLOBAL u32x4*)(from + ch);
+          __builtin_memcpy(x, &y, 16);
+        } else {
+          for (int d = 0; d < 8; ++d) x[d] = ch + d < a.D ? from[(ch + d) * a.vd] : (u16)0;
+        }
+#pragma unroll
+        for (int d = 0; d < 8; ++d) s += fabsf(a.bf16 ? BF16::to_f32(x[d]) : F16::to_f32(x[d]));
+      }
+    }
+#pragma unroll
+    for (int d = 1; d < 8; d *= 2) s += __shfl_xor(s, d);
+    if ((tid & 7) == 0) {
+      if (h.norm) h.norm[dst] = fresh ? s : h.norm[src];
+      h.imp[dst] = fresh ? (h.fresh ? h.fresh[at] : 0.f) : h.imp[src];
+      h.pos[dst] = fresh ? h.seen + at : h.pos[src];
+    }
+  }
+}
+
+// Leading nodes of a path that name one of the T tokens, by the whole block. s: one int of LDS.
+__device__ __forceinline__ int ins_path_len(const InsArgs& a, const FE_GLOBAL int* path, int* s) {
+  if (threadIdx.x == 0) *s = a.A;
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.A; i += 1024)
+    if (path[i] < 0 || path[i] >= a.T) atomicMin(s, i);
+  __syncthreads();
+  return __builtin_amdgcn_readfirstlane(*s);
+}
+
+// In candidate order, with PER consecutive candidates a thread: hole(i, rank) for each evicted one below F, mover(i, rank)
+// for each kept one at or past F, stay(i, rank) for each kept new one below F. Returns the numbers of movers and of
+// those that stay. key > thr is kept, and the first `need` of the eq candidates with key == thr.
+template <int PER, typename Get, typename Hole, typename Mover, typename Stay>
+__device__ __forceinline__ void ins_order(Get get, int n, int M, int F, u32 thr, int need, int eq, int* tmp, Hole hole, Mover mover,
+                                          Stay stay, int& moves, int& stays) {
+  int eq_before = 0, holes = 0;
+  moves = stays = 0;
+#pragma unroll 1
+  for (int base = 0; base < M; base += 1024 * PER) {
+    const int i0 = base + (int)threadIdx.x * PER;
+    u32 key[PER];
+    int neq = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      key[i] = i0 + i < M ? get(i0 + i) : 0u;
+      neq += i0 + i < M && key[i] == thr ? 1 : 0;
+    }
+    int rank = 0, total;
+    if (need < eq) {
+      rank = eq_before + block_exclusive_scan(neq, tmp, total);
+      eq_before += total;
+    }
+    u32 kept = 0;
+    int nh = 0, nm = 0, ns = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const bool in = i0 + i < M;
+      bool k = in && key[i] > thr;
+      if (in && key[i] == thr) {
+        k = need == eq || rank < need;
+        ++rank;
+      }
+      kept |= k ? 1u << i : 0u;
+      nh += in && !k && i0 + i < F ? 1 : 0;
+      nm += k && i0 + i >= F ? 1 : 0;
+      ns += k && i0 + i >= n && i0 + i < F ? 1 : 0;
+    }
+    // counts of a round are at most 1024 * PER: 13 bits and more each in two scans
+    int at = block_exclusive_scan(nh | (nm << 16), tmp, total);
+    int h = holes + (at & 0xffff), m = moves + (at >> 16);
+    holes += total & 0xffff;
+    moves += total >> 16;
+    int s = stays + block_exclusive_scan(ns, tmp, total);
+    stays += total;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int c = i0 + i;
+      const bool k = (kept >> i) & 1u;
+      if (c < M && !k && c < F) hole(c, h++);
+      if (k && c >= F) mover(c, m++);
+      if (k && c >= n && c < F) stay(c, s++);
+    }
+  }
+}
+
+template <bool VEC>
+__global__ __launch_bounds__(1024) void insert_few_kernel(const InsArgs args) {
+  __shared__ u32 skey[kInsKeys];
+  __shared__ int s_src[2 * kInsFew], s_dst[2 * kInsFew];   // moves, then the rows that stay
   __shared__ u32 hist[2 * 2048];
   __shared__ __attribute__((aligned(16))) int tmp[2 * kSelWaves];
   __shared__ SelShared sh;
-  __shared__ int s_len;
-  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hh = lane >> 5, wv = tid >> 6;
-  const int bh = (int)blockIdx.x, b = bh / a.Hkv, hkv = bh - b * a.Hkv;
-  const int n = min(max(a.length[bh], 0), a.C);
-  const int seen = a.seen[bh];
-  const int* path = a.path ? a.path + (long long)b * a.A : nullptr;
-  if (path) {
-    // leading nodes that name one of the T tokens
-    if (tid == 0) s_len = a.A;
-    __syncthreads();
-    for (int i = tid; i < a.A; i += 1024)
-      if (path[i] < 0 || path[i] >= a.T) atomicMin(&s_len, i);
-    __syncthreads();
-  }
-  const int na = path ? s_len : a.A;
-  const int M = n + na, F = min(M, a.budget);
+  __shared__ u32 red_k[2][16];
+  __shared__ int red_i[2][16], s_len;
+  const InsArgs a = ins_hold(args);
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int hkv = (int)blockIdx.x, b = (int)blockIdx.y, bh = b * a.Hkv + hkv;
+  const int len = a.length[bh], seen = __builtin_amdgcn_readfirstlane(a.seen[bh]);
+  const int n = __builtin_amdgcn_readfirstlane(min(max(len, 0), a.C));
+  const InsHead h = ins_head(a, b, hkv, n, seen);
+  const int na = h.path ? ins_path_len(a, h.path, &s_len) : a.A;
+  const int M = n + na, F = min(M, a.budget), e = M - F;
   const long long held = (long long)seen + na - a.recent;   // first protected position
-  float* imp = a.imp + bh * a.imp_stride;
-  int* pos = a.pos + bh * a.pos_stride;
-  const float* fresh = a.new_imp ? a.new_imp + (long long)bh * a.A : nullptr;
-  int* holes = a.lists + (long long)bh * 2 * a.E;
-  int* movers = holes + a.E;
 
-  auto get = [&](int i) -> u32 {
-    if (i < n) return ins_key(imp[i], pos[i] >= held);
-    return ins_key(fresh ? fresh[i - n] : 0.f, (long long)seen + (i - n) >= held);
-  };
-  int moves = 0;
-  u32 thr = 0;
-  int need = 0, eq = 0;
-  if (M > F) {
-    radix_select(get, M, F, 0u, 0xffffffffu, hist, tmp, &sh, thr, need, eq);
-    int eq_before = 0, hole_before = 0, move_before = 0;
-    for (int base = 0; base < M; base += 1024) {
-      const int i = base + tid;
-      const u32 key = i < M ? get(i) : 0u;
-      bool kept = i < M && key > thr;
-      if (need < eq) {
-        int total;
-        const int rank = eq_before + block_exclusive_scan(i < M && key == thr ? 1 : 0, tmp, total);
-        eq_before += total;
-        kept = kept || (i < M && key == thr && rank < need);
-      } else {
-        kept = kept || (i < M && key == thr);
-      }
-      const int hole = i < F && !kept, mover = i >= F && kept;
-      int total;
-      const int at = block_exclusive_scan(hole | (mover << 16), tmp, total);
-      if (hole) holes[hole_before + (at & 0xffff)] = i;
-      if (mover) movers[move_before + (at >> 16)] = i;
-      hole_before += total & 0xffff;
-      move_before += total >> 16;
-    }
-    moves = move_before;
-  }
-  __syncthreads();
-
-  // the new rows that stay where they were appended, then the rows that move
-  const u16* kn = a.k + b * a.ks[0] + hkv * a.ks[1];
-  const u16* vn = a.v + b * a.vs[0] + hkv * a.vs[1];
-  u16* kc = a.kc + b * a.kcs[0] + hkv * a.kcs[1];
-  u16* vc = a.vc + b * a.vcs[0] + hkv * a.vcs[1];
-  const int appended = max(F - n, 0);
-  for (int j = wv; j < appended + moves; j += kSelWaves) {
-    int src, dst;
-    if (j < appended) {
-      src = dst = n + j;
-    } else {
-      src = movers[j - appended];
-      dst = holes[j - appended];
-    }
-    if (j < appended && M > F) {
-      // a new row below F that was not kept: its slot is among the vacated ones
-      const u32 key = get(src);
-      bool kept = key > thr;
-      if (key == thr) {
-        kept = need == eq;
-        if (!kept) {
-          kept = true;
-          for (int i = 0; i < moves; ++i) kept = kept && holes[i] != src;
+  int moves = 0, stays = F > n ? F - n : 0;
+  if (e > 0) {
+    u32 bk = kKeyDrawn;                     // the thread's least key, of equal ones the highest slot
+    int bi = -1;
+    constexpr int U = 4;
+#pragma unroll 1
+    for (int base = tid; base < M; base += 1024 * U) {
+      float w[U];
+      int p[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = base + 1024 * u;
+        const bool old = i < n;
+        const int at = old ? i : 0;
+        w[u] = h.imp[at];
+        p[u] = h.pos[at];
+        if (!old) {
+          w[u] = i < M && h.fresh ? h.fresh[i - n] : 0.f;
+          p[u] = seen + (i - n);
         }
       }
-      if (!kept) continue;
-    }
-    const bool is_new = src >= n;
-    const int row = is_new ? (path ? path[src - n] : src - n) : src;
-    float s;
-    if (hh == 0) {
-      const u16* from = is_new ? kn + (long long)row * a.ks[2] : kc + (long long)row * a.kcs[2];
-      s = ins_row<true>(from, is_new ? a.ks[3] : a.kcs[3], is_new ? a.kvec : a.kcvec, kc + (long long)dst * a.kcs[2], a.kcs[3],
-                        a.kcvec, a.D, l32);
-    } else {
-      const u16* from = is_new ? vn + (long long)row * a.vs[2] : vc + (long long)row * a.vcs[2];
-      u16* to = vc + (long long)dst * a.vcs[2];
-      const long long fcs = is_new ? a.vs[3] : a.vcs[3];
-      const int fv = is_new ? a.vvec : a.vcvec;
-      s = a.bf16 ? ins_row<true>(from, fcs, fv, to, a.vcs[3], a.vcvec, a.D, l32)
-                 : ins_row<false>(from, fcs, fv, to, a.vcs[3], a.vcvec, a.D, l32);
-    }
 #pragma unroll
-    for (int d = 1; d < 32; d *= 2) s += __shfl_xor(s, d);
-    if (lane == 32) {
-      if (a.norm) {
-        float* norm = a.norm + bh * a.norm_stride;
-        norm[dst] = is_new ? s : norm[src];
+      for (int u = 0; u < U; ++u) {
+        const int i = base + 1024 * u;
+        if (i < M) {
+          const u32 key = ins_key(w[u], (i < n ? (long long)p[u] : (long long)seen + (i - n)) >= held);
+          skey[i] = key;
+          if (key <= bk) bk = key, bi = i;
+        }
       }
-      imp[dst] = is_new ? (fresh ? fresh[src - n] : 0.f) : imp[src];
-      pos[dst] = is_new ? seen + (src - n) : pos[src];
     }
+    if (e <= kInsDraw) {
+      int vict[kInsDraw];
+#pragma unroll
+      for (int r = 0; r < kInsDraw; ++r) vict[r] = 0x7fffffff;
+#pragma unroll 1
+      for (int r = 0; r < e; ++r) {
+        const u32 wk = (u32)__builtin_amdgcn_readlane((int)wave_inclusive_min(bk), 63);
+        const int wi = __builtin_amdgcn_readlane((int)wave_inclusive_max(bk == wk ? (u32)(bi + 1) : 0u), 63) - 1;
+        if (lane == 0) red_k[r & 1][wv] = wk, red_i[r & 1][wv] = wi;
+        lds_barrier();
+        const u32 k16 = red_k[r & 1][lane & 15];
+        const int i16 = red_i[r & 1][lane & 15];
+        const u32 K = (u32)__builtin_amdgcn_readlane((int)wave_inclusive_min(k16), 63);
+        const int I = __builtin_amdgcn_readlane((int)wave_inclusive_max(k16 == K ? (u32)(i16 + 1) : 0u), 63) - 1;
+#pragma unroll
+        for (int q = 0; q < kInsDraw; ++q) vict[q] = q == r ? I : vict[q];
+        if (r + 1 < e && (I & 1023) == tid) {
+          skey[I] = kKeyDrawn;
+          bk = kKeyDrawn;
+          bi = -1;
+          for (int i = tid; i < M; i += 1024)
+            if (skey[i] <= bk && skey[i] != kKeyDrawn) bk = skey[i], bi = i;
+        }
+      }
+      // a victim below F leaves a hole, in order; a candidate at or past F that is no victim moves, in order; new rows
+      // below F that are no victims stay
+      if (tid < e) {
+        int mine = 0, hole = 0, before = 0, same = 0;
+#pragma unroll
+        for (int q = 0; q < kInsDraw; ++q) mine = q == tid ? vict[q] : mine;
+#pragma unroll
+        for (int q = 0; q < kInsDraw; ++q) {
+          hole += vict[q] < mine ? 1 : 0;                       // holes before this one (victims below it are below F)
+          before += vict[q] >= F && vict[q] < F + tid ? 1 : 0;  // victims at or past F before candidate F + tid
+          same += vict[q] == F + tid ? 1 : 0;
+        }
+        if (mine < F) s_dst[hole] = mine;
+        if (!same) s_src[tid - before] = F + tid;
+      }
+      int past = 0, fresh = 0;
+#pragma unroll
+      for (int q = 0; q < kInsDraw; ++q) {
+        past += vict[q] >= F && vict[q] < M ? 1 : 0;
+        fresh += vict[q] >= n && vict[q] < F ? 1 : 0;
+      }
+      moves = e - past;
+      for (int i = tid; i < F - n; i += 1024) {
+        int before = 0, same = 0;
+#pragma unroll
+        for (int q = 0; q < kInsDraw; ++q) {
+          before += vict[q] >= n && vict[q] < n + i ? 1 : 0;
+          same += vict[q] == n + i ? 1 : 0;
+        }
+        if (!same) s_src[kInsFew + i - before] = s_dst[kInsFew + i - before] = n + i;
+      }
+      stays -= fresh;
+    } else {
+      __syncthreads();
+      u32 thr;
+      int need, eq;
+      auto get = [&](int i) -> u32 { return skey[i]; };
+      radix_select(get, M, F, 0u, 0xffffffffu, hist, tmp, &sh, thr, need, eq);
+      ins_order<4>(get, n, M, F, thr, need, eq, tmp, [&](int i, int r) { s_dst[r] = i; }, [&](int i, int r) { s_src[r] = i; },
+                   [&](int i, int r) { s_src[kInsFew + r] = s_dst[kInsFew + r] = i; }, moves, stays);
+    }
+  } else {
+    for (int i = tid; i < stays; i += 1024) s_src[kInsFew + i] = s_dst[kInsFew + i] = n + i;
   }
+  __syncthreads();
+  ins_move<1024, VEC>(a, h, moves + stays, tid, [&](int j, int& src, int& dst) {
+    const int at = j < moves ? j : kInsFew + j - moves;
+    src = s_src[at];
+    dst = s_dst[at];
+  });
   if (tid == 0) {
     a.length[bh] = F;
     a.seen[bh] = seen + na;
   }
 }
 
+__global__ __launch_bounds__(1024) void insert_list_kernel(const InsArgs args) {
+  __shared__ u32 hist[2 * 2048];
+  __shared__ __attribute__((aligned(16))) int tmp[2 * kSelWaves];
+  __shared__ SelShared sh;
+  __shared__ int s_len;
+  const InsArgs a = ins_hold(args);
+  const int hkv = (int)blockIdx.x, b = (int)blockIdx.y, bh = b * a.Hkv + hkv;
+  const int n = __builtin_amdgcn_readfirstlane(min(max(a.length[bh], 0), a.C)), seen = __builtin_amdgcn_readfirstlane(a.seen[bh]);
+  const InsHead h = ins_head(a, b, hkv, n, seen);
+  const int na = h.path ? ins_path_len(a, h.path, &s_len) : a.A;
+  const int M = n + na, F = min(M, a.budget);
+  const long long held = (long long)seen + na - a.recent;
+  FE_GLOBAL int* list = a.lists + (long long)bh * (4 + 2 * (long long)a.P);
+  FE_GLOBAL int* dst = list + 4;
+  FE_GLOBAL int* src = dst + a.P;
+  int moves = 0, stays = F > n ? F - n : 0;
+  if (M > F) {
+    auto get = [&](int i) -> u32 {
+      if (i < n) return ins_key(h.imp[i], h.pos[i] >= held);
+      return ins_key(h.fresh ? h.fresh[i - n] : 0.f, (long long)seen + (i - n) >= held);
+    };
+    u32 thr;
+    int need, eq;
+    radix_select(get, M, F, 0u, 0xffffffffu, hist, tmp, &sh, thr, need, eq);
+    ins_order<8>(get, n, M, F, thr, need, eq, tmp, [&](int i, int r) { dst[r] = i; }, [&](int i, int r) { src[r] = i; },
+                 [&](int i, int r) { src[a.P - 1 - r] = dst[a.P - 1 - r] = i; }, moves, stays);
+  } else {
+    for (int i = threadIdx.x; i < stays; i += 1024) src[a.P - 1 - i] = dst[a.P - 1 - i] = n + i;
+  }
+  __syncthreads();                          // every wave has read the length
+  if (threadIdx.x == 0) {
+    list[0] = moves;
+    list[1] = stays;
+    list[2] = n;
+    list[3] = seen;
+    a.length[bh] = F;
+    a.seen[bh] = seen + na;
+  }
+}
+
+template <bool VEC>
+__global__ __launch_bounds__(256) void insert_move_kernel(const InsArgs args) {
+  const InsArgs a = ins_hold(args);
+  const int hkv = (int)blockIdx.y, b = (int)blockIdx.z, bh = b * a.Hkv + hkv;
+  const FE_GLOBAL int* list = a.lists + (long long)bh * (4 + 2 * (long long)a.P);
+  const int moves = list[0], all = moves + list[1];
+  const InsHead h = ins_head(a, b, hkv, list[2], list[3]);
+  const FE_GLOBAL int* dsts = list + 4;
+  const FE_GLOBAL int* srcs = dsts + a.P;
+  // 32 rows a block at a time
+#pragma unroll 1
+  for (int r0 = 32 * (int)blockIdx.x; r0 < all; r0 += 32 * (int)gridDim.x)
+    ins_move<256, VEC>(a, h, min(32, all - r0), threadIdx.x, [&](int j, int& src, int& dst) {
+      const int at = r0 + j < moves ? r0 + j : a.P - 1 - (r0 + j - moves);
+      src = srcs[at];
+      dst = dsts[at];
+    });
+}
+
+struct InsKernel {
+  const void* fn;
+  const char* name;
+};
+const InsKernel kInsKernels[] = {{(const void*)insert_few_kernel<false>, "insert_few_elements"}, {(const void*)insert_few_kernel<true>, "insert_few"},
+                                 {(const void*)insert_move_kernel<false>, "insert_move_elements"}, {(const void*)insert_move_kernel<true>, "insert_move"},
+                                 {(const void*)insert_list_kernel, "insert_list"}};
+
 void append_insert_resources(std::string& out) {
-  hipFuncAttributes attr;
-  if (hipFuncGetAttributes(&attr, (const void*)insert_kernel) != hipSuccess) return;
-  char buf[512];
-  snprintf(buf, sizeof(buf),
-           "{\"kernel\":\"insert_kernel\",\"registers_per_thread\":%d,\"lds_static_bytes\":%zu,"
-           "\"lds_dynamic_bytes\":0,\"scratch_bytes_per_thread\":%zu,\"max_threads_per_block\":%d},",
-           attr.numRegs, (size_t)attr.sharedSizeBytes, (size_t)attr.localSizeBytes, attr.maxThreadsPerBlock);
-  out += buf;
+  for (const auto& e : kInsKernels) {
+    hipFuncAttributes attr;
+    if (hipFuncGetAttributes(&attr, e.fn) != hipSuccess) continue;
+    char buf[512];
+    snprintf(buf, sizeof(buf),
+             "{\"kernel\":\"%s\",\"registers_per_thread\":%d,\"lds_static_bytes\":%zu,"
+             "\"lds_dynamic_bytes\":0,\"scratch_bytes_per_thread\":%zu,\"max_threads_per_block\":%d},",
+             e.name, attr.numRegs, (size_t)attr.sharedSizeBytes, (size_t)attr.localSizeBytes, attr.maxThreadsPerBlock);
+    out += buf;
+  }
 }
 
 namespace {
-// Rows that an insertion can move: they come from past the budget and go below it.
-int64_t ins_list(int64_t C, int64_t A, int64_t budget) { return std::max<int64_t>(0, std::min(C + A - budget, budget)); }
+// Whether the few-rows kernel holds all that any lengths can ask for.
+bool ins_few(int64_t C, int64_t A, int64_t budget) { return A <= kInsFew && C + A - budget <= kInsFew && C + A <= kInsKeys; }
+// Rows that an insertion can write: new ones, and those from past the budget; all below it.
+int64_t ins_list(int64_t C, int64_t A, int64_t budget) { return std::min(A + C - budget, budget); }
 }  // namespace
 }  // namespace fe
 
 using namespace fe;
 
 extern "C" size_t fe_insert_workspace_bytes(int64_t B, int64_t Hkv, int64_t A, int64_t C, int64_t budget) {
-  if (B < 1 || Hkv < 1 || A < 0 || C < 1 || budget < 1 || budget > C || B > (1LL << 24) || Hkv > (1LL << 24) || A > (1LL << 29) ||
+  if (B < 1 || Hkv < 1 || A < 0 || C < 1 || budget < 1 || budget > C || B > 65535 || Hkv > 65535 || A > (1LL << 29) ||
       C > (1LL << 30) || B * Hkv > (1LL << 24))
     return 0;
-  return (size_t)(B * Hkv * 2 * ins_list(C, A, budget)) * sizeof(int);
+  if (ins_few(C, A, budget)) return 0;
+  return (size_t)(B * Hkv) * (size_t)(4 + 2 * ins_list(C, A, budget)) * sizeof(int);
 }
 
 extern "C" int fe_insert_tokens(const void* k, const void* v, void* k_cache, void* v_cache, float* importance,
@@ -231,7 +472,7 @@ extern "C" int fe_insert_tokens(const void* k, const void* v, void* k_cache, voi
     set_error(std::string(who) + ": dtype must be fp16 or bf16");
     return FE_ERR_INVALID;
   }
-  if (C > (1LL << 30) || T > (1LL << 29) || B > (1LL << 24) || Hkv > (1LL << 24) || B * Hkv > (1LL << 24)) {
+  if (C > (1LL << 30) || T > (1LL << 29) || B > 65535 || Hkv > 65535 || B * Hkv > (1LL << 24)) {
     set_error(std::string(who) + ": sizes exceed the supported range");
     return FE_ERR_UNSUPPORTED;
   }
@@ -243,41 +484,44 @@ extern "C" int fe_insert_tokens(const void* k, const void* v, void* k_cache, voi
     set_error(std::string(who) + ": invalid row stride");
     return FE_ERR_INVALID;
   }
-  const int64_t* in[4] = {k_strides, v_strides, k_cache_strides, v_cache_strides};
-  InsArgs a = {};
-  long long(*st[4])[4] = {&a.ks, &a.vs, &a.kcs, &a.vcs};
+  const int64_t* st[4] = {k_strides, v_strides, k_cache_strides, v_cache_strides};
   for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      if (!in[i] || in[i][j] < 0) {
+    for (int j = 0; j < 4; ++j)
+      if (!st[i] || st[i][j] < 0) {
         set_error(std::string(who) + ": null or negative strides");
         return FE_ERR_INVALID;
       }
-      (*st[i])[j] = in[i][j];
-    }
   const size_t need = fe_insert_workspace_bytes(B, Hkv, A, C, budget);
   if (need && (!workspace || workspace_bytes < need)) {
     set_error(std::string(who) + ": workspace too small; need " + std::to_string(need) + " bytes");
     return FE_ERR_WORKSPACE;
   }
-  auto vec = [&](const void* p, const long long(&s)[4], int64_t N) {
+  auto vec = [&](const void* p, const int64_t* s, int64_t N) {
     return D % 8 == 0 && s[3] == 1 && (uintptr_t)p % 16 == 0 && (B <= 1 || s[0] % 8 == 0) && (Hkv <= 1 || s[1] % 8 == 0) &&
            (N <= 1 || s[2] % 8 == 0);
   };
-  a.k = (const u16*)k;
-  a.v = (const u16*)v;
-  a.kc = (u16*)k_cache;
-  a.vc = (u16*)v_cache;
-  a.imp = importance;
+  const bool v16 = vec(k, st[0], T) && vec(v, st[1], T) && vec(k_cache, st[2], C) && vec(v_cache, st[3], C);
+  InsArgs a = {};
+  auto set = [](auto& to, auto* from) { to = (std::remove_reference_t<decltype(to)>)(uintptr_t)from; };
+  set(a.k, k);
+  set(a.v, v);
+  set(a.kc, k_cache);
+  set(a.vc, v_cache);
+  set(a.imp, importance);
+  set(a.pos, position);
+  set(a.norm, value_norm);
+  set(a.length, length);
+  set(a.seen, seen);
+  set(a.new_imp, new_importance);
+  set(a.path, path);
+  set(a.lists, workspace);
+  a.kb = st[0][0], a.kh = st[0][1], a.kn = st[0][2], a.kd = st[0][3];
+  a.vb = st[1][0], a.vh = st[1][1], a.vn = st[1][2], a.vd = st[1][3];
+  a.kcb = st[2][0], a.kch = st[2][1], a.kcn = st[2][2], a.kcd = st[2][3];
+  a.vcb = st[3][0], a.vch = st[3][1], a.vcn = st[3][2], a.vcd = st[3][3];
   a.imp_stride = importance_stride;
-  a.pos = position;
   a.pos_stride = position_stride;
-  a.norm = value_norm;
   a.norm_stride = value_norm_stride;
-  a.length = length;
-  a.seen = seen;
-  a.new_imp = new_importance;
-  a.path = path;
-  a.lists = (int*)workspace;
   a.T = (int)T;
   a.A = (int)A;
   a.C = (int)C;
@@ -285,17 +529,20 @@ extern "C" int fe_insert_tokens(const void* k, const void* v, void* k_cache, voi
   a.Hkv = (int)Hkv;
   a.budget = (int)budget;
   a.recent = (int)recent;
-  a.E = (int)ins_list(C, A, budget);
+  a.P = (int)ins_list(C, A, budget);
   a.bf16 = dtype == FE_DTYPE_BF16;
-  a.kvec = vec(k, a.ks, T);
-  a.vvec = vec(v, a.vs, T);
-  a.kcvec = vec(k_cache, a.kcs, C);
-  a.vcvec = vec(v_cache, a.vcs, C);
-  hipLaunchKernelGGL(insert_kernel, dim3((unsigned)(B * Hkv)), dim3(1024), 0, (hipStream_t)hip_stream, a);
-  hipError_t err = hipGetLastError();
-  if (err != hipSuccess) {
-    set_error(std::string(who) + ": launch: " + hipGetErrorString(err));
-    return FE_ERR_HIP;
-  }
-  return FE_OK;
+  hipStream_t stream = (hipStream_t)hip_stream;
+  auto launch = [&](const void* fn, dim3 grid, dim3 block) {
+    void* args[] = {&a};
+    const hipError_t err = hipLaunchKernel(fn, grid, block, args, 0, stream);
+    if (err != hipSuccess) set_error(std::string(who) + ": launch: " + hipGetErrorString(err));
+    return err == hipSuccess ? FE_OK : FE_ERR_HIP;
+  };
+  const dim3 heads((unsigned)Hkv, (unsigned)B);
+  if (ins_few(C, A, budget)) return launch(kInsKernels[v16].fn, heads, dim3(1024));
+  if (int rc = launch(kInsKernels[4].fn, heads, dim3(1024))) return rc;
+  if (!a.P) return FE_OK;
+  // 32 rows a block, up to some 4096 blocks
+  const int64_t blocks = std::min<int64_t>((a.P + 31) / 32, std::max<int64_t>(1, 4096 / (B * Hkv)));
+  return launch(kInsKernels[2 + v16].fn, dim3((unsigned)blocks, (unsigned)Hkv, (unsigned)B), dim3(256));
 }

@@ -182,8 +182,8 @@ def test_c_replay_path_refuses():
 def test_c_insert_tokens_refuses():
     L = _lib.lib()
 
-    def call(B=1, Hkv=2, T=3, A=3, C=8, D=16, budget=8, recent=0, dtype=1, path=None, k=P, imp=P, imp_st=8, ws=None, ws_bytes=0, st=ST):
-        return L.fe_insert_tokens(k, k, P, P, imp, imp_st, P, 8, None, 0, P, P, None, path, B, Hkv, T, A, C, D, budget, recent,
+    def call(B=1, Hkv=2, T=3, A=3, C=8, D=16, budget=8, recent=0, dtype=1, path=None, k=P, imp=P, imp_st=8, ws=None, ws_bytes=0, st=ST, pos_st=8):
+        return L.fe_insert_tokens(k, k, P, P, imp, imp_st, P, pos_st, None, 0, P, P, None, path, B, Hkv, T, A, C, D, budget, recent,
                                   st, st, ST, ST, dtype, ws, ws_bytes, None)
 
     for bad in (dict(B=0), dict(Hkv=0), dict(T=-1), dict(A=2), dict(A=4, path=P), dict(C=0), dict(D=257), dict(budget=0), dict(budget=9),
@@ -191,9 +191,15 @@ def test_c_insert_tokens_refuses():
         assert call(**bad) == INVALID, bad
         assert L.fe_last_error().decode().startswith("fe_insert_tokens")
     assert call(C=(1 << 30) + 1, imp_st=1 << 31) == UNSUPPORTED
-    need = L.fe_insert_workspace_bytes(1, 2, 3, 8, 8)
-    assert need >= 4 * 2 * 2 * 3
-    assert call() == WORKSPACE and call(ws=P, ws_bytes=need - 1) == WORKSPACE
+    assert call(B=1 << 16) == UNSUPPORTED
+    # few rows need no workspace; a prompt's worth does
+    assert L.fe_insert_workspace_bytes(1, 2, 3, 8, 8) == 0
+    big = dict(T=300, A=300, C=1000, imp_st=1000, budget=900)
+    need = L.fe_insert_workspace_bytes(1, 2, 300, 1000, 900)
+    assert need >= 4 * 2 * 2 * 400
+    # position_stride is 8 in every call: below 1000 slots
+    assert call(**big) == INVALID
+    assert call(pos_st=1000, **big) == WORKSPACE and call(pos_st=1000, ws=P, ws_bytes=need - 1, **big) == WORKSPACE
 
 
 def test_workspace_sizes():
