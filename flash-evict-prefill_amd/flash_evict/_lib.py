@@ -101,13 +101,20 @@ def check(rc, what):
 
 _I64x3 = ctypes.c_int64 * 3
 _I64x4 = ctypes.c_int64 * 4
+_stride_arrays = {}
 
 
 def strides(t):
-    """Element strides of a tensor as a ctypes int64[len] array."""
+    """Element strides of a tensor as a ctypes int64[len] array, one for each set of strides (the
+    library only reads them)."""
     st = t.stride()
-    n = len(st)
-    return (_I64x4 if n == 4 else _I64x3 if n == 3 else ctypes.c_int64 * n)(*st)
+    got = _stride_arrays.get(st)
+    if got is None:
+        if len(_stride_arrays) >= 4096:
+            _stride_arrays.clear()
+        n = len(st)
+        got = _stride_arrays[st] = (_I64x4 if n == 4 else _I64x3 if n == 3 else ctypes.c_int64 * n)(*st)
+    return got
 
 
 _SAME_DEVICE = contextlib.nullcontext()

@@ -18,6 +18,7 @@ so a step can be captured in a graph. Inference only, fp16 and bf16, head dims u
 kernels read 16 bytes at a time where the channel stride is 1, the head dim a multiple of 8 and
 rows lie on 16-byte boundaries, and element by element otherwise.
 """
+import functools
 import math
 
 import torch
@@ -31,13 +32,14 @@ MAX_TOKENS = 256    # new tokens of one call (a longer chunk is passed in parts)
 
 
 def _check_new(q, k, v, k_cache, scale, recency_decay):
-    """Shape, type and device rules shared by decode_attention and replay_path; (scale, decay)."""
-    if q.ndim != 4 or k.ndim != 4 or v.ndim != 4 or k_cache.ndim != 4:
+    """Shape, type and device rules shared by decode_attention and replay_path; the sizes, device,
+    dtype, scale and decay."""
+    qs, ks, cs = q.shape, k.shape, k_cache.shape
+    if len(qs) != 4 or len(ks) != 4 or v.ndim != 4 or len(cs) != 4:
         raise ValueError("q must have shape [batch, heads, tokens, channels], k, v and the cache [batch, kv_heads, rows, channels]")
-    b, hq, t, d = q.shape
-    hk = k.shape[1]
-    if min(b, hq, t, d, hk, k_cache.shape[2]) < 1 or k.shape != (b, hk, t, d) or v.shape != k.shape \
-            or k_cache.shape[:2] != (b, hk) or k_cache.shape[3] != d:
+    b, hq, t, d = qs
+    hk, c = ks[1], cs[2]
+    if b < 1 or hq < 1 or t < 1 or d < 1 or hk < 1 or c < 1 or ks != (b, hk, t, d) or v.shape != ks or cs != (b, hk, c, d):
         raise ValueError("Expected nonempty q, k, v of equal batch, tokens and channels and a cache of their batch, KV heads and channels")
     if hq % hk or d > 256:
         raise ValueError("Query heads must be divisible by KV heads; head dimension must be <= 256")
@@ -46,18 +48,28 @@ def _check_new(q, k, v, k_cache, scale, recency_decay):
     device, dtype = q.device, q.dtype
     if not q.is_cuda or dtype not in _DTYPES:
         raise ValueError("CUDA fp16 or bf16 inputs required")
-    for x in (k, v, k_cache):
-        if x.device != device or x.dtype != dtype:
-            raise ValueError("q, k, v and the cache must have the same device and dtype")
+    if k.device != device or v.device != device or k_cache.device != device or k.dtype != dtype or v.dtype != dtype \
+            or k_cache.dtype != dtype:
+        raise ValueError("q, k, v and the cache must have the same device and dtype")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or k_cache.requires_grad):
         raise ValueError("Inference only: no backward implementation")
     scale = d ** -0.5 if scale is None else float(scale)
     if not math.isfinite(scale):
         raise ValueError("scale must be finite")
     recency_decay = float(recency_decay)
-    if not math.isfinite(recency_decay) or recency_decay < 0:
+    if not (0. <= recency_decay < math.inf):
         raise ValueError("recency_decay must be finite and nonnegative")
-    return scale, recency_decay
+    return b, hq, hk, t, c, d, device, dtype, scale, recency_decay
+
+
+@functools.lru_cache(maxsize=4096)
+def _decode_workspace(*sizes):
+    return _lib.lib().fe_decode_workspace_bytes(*sizes)
+
+
+@functools.lru_cache(maxsize=4096)
+def _insert_workspace(*sizes):
+    return _lib.lib().fe_insert_workspace_bytes(*sizes)
 
 
 def _check_heads(x, name, b, hk, device):
@@ -115,10 +127,7 @@ def decode_attention(q, k, v, k_cache, v_cache, length, *, tree=None, scale=None
     their values' L1 norms. Without value_norm (FP32 [B, Hkv, C]) neither is weighted by a norm.
     For a drafted tree leave `importance` out, and call replay_path once the path is known.
     """
-    scale, recency_decay = _check_new(q, k, v, k_cache, scale, recency_decay)
-    b, hq, t, d = q.shape
-    hk, c = k_cache.shape[1:3]
-    device, dtype = q.device, q.dtype
+    b, hq, hk, t, c, d, device, dtype, scale, recency_decay = _check_new(q, k, v, k_cache, scale, recency_decay)
     if v_cache.shape != k_cache.shape or v_cache.device != device or v_cache.dtype != dtype:
         raise ValueError("k_cache and v_cache must have the same shape, device and dtype")
     _check_heads(length, "length", b, hk, device)
@@ -144,7 +153,7 @@ def decode_attention(q, k, v, k_cache, v_cache, length, *, tree=None, scale=None
     out = torch.empty((b, hq, t, d), dtype=dtype, device=device)
     lse = torch.empty((b, hq, t), dtype=torch.float32, device=device)
     L = _lib.lib()
-    ws_bytes = L.fe_decode_workspace_bytes(b, hq, hk, t, c, d, importance is not None)
+    ws_bytes = _decode_workspace(b, hq, hk, t, c, d, importance is not None)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
     with _lib.on_device(device):
         rc = L.fe_decode_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
@@ -168,10 +177,7 @@ def replay_path(q, k, v, k_cache, length, lse, path, importance, *, scale=None, 
     and importance_out are as in decode_attention; new_importance is 0 past a path's end. None as
     the path stands for all T tokens in order.
     """
-    scale, recency_decay = _check_new(q, k, v, k_cache, scale, recency_decay)
-    b, hq, t, d = q.shape
-    hk, c = k_cache.shape[1:3]
-    device, dtype = q.device, q.dtype
+    b, hq, hk, t, c, d, device, dtype, scale, recency_decay = _check_new(q, k, v, k_cache, scale, recency_decay)
     _check_heads(length, "length", b, hk, device)
     if lse.shape != (b, hq, t) or lse.dtype != torch.float32 or lse.device != device:
         raise ValueError("lse must be the float32 [batch, heads, tokens] of decode_attention")
@@ -217,9 +223,10 @@ def insert_tokens(k, v, k_cache, v_cache, importance, position, length, seen, bu
     length on are left as they were. new_importance is FP32 [B, Hkv, T or A], None for zeros.
     k = v = None inserts nothing: an eviction down to `budget`. 1 <= budget <= C, recent <= budget.
     """
-    if k_cache.ndim != 4 or v_cache.shape != k_cache.shape or min(k_cache.shape) < 1 or k_cache.shape[3] > 256:
+    cs = k_cache.shape
+    if len(cs) != 4 or v_cache.shape != cs or min(cs) < 1 or cs[3] > 256:
         raise ValueError("The cache must be two nonempty [batch, kv_heads, slots, channels] tensors of at most 256 channels")
-    b, hk, c, d = k_cache.shape
+    b, hk, c, d = cs
     device, dtype = k_cache.device, k_cache.dtype
     if not k_cache.is_cuda or dtype not in _DTYPES or v_cache.device != device or v_cache.dtype != dtype:
         raise ValueError("CUDA fp16 or bf16 caches of one device and dtype required")
@@ -227,18 +234,22 @@ def insert_tokens(k, v, k_cache, v_cache, importance, position, length, seen, bu
         raise ValueError("k and v come together, path and new_importance with them")
     t = 0
     if k is not None:
-        if k.ndim != 4 or v.shape != k.shape or k.shape[:2] != (b, hk) or k.shape[3] != d:
+        ks = k.shape
+        if len(ks) != 4 or v.shape != ks or ks != (b, hk, ks[2], d):
             raise ValueError("k and v must be [batch, kv_heads, tokens, channels] tensors like the cache")
         if k.device != device or v.device != device or k.dtype != dtype or v.dtype != dtype:
             raise ValueError("k, v and the cache must have the same device and dtype")
-        t = k.shape[2]
+        t = ks[2]
+        # in place, and in no order: the new rows may not lie in the cache's memory
         mine = (k_cache.untyped_storage().data_ptr(), v_cache.untyped_storage().data_ptr())
         if t and (k.untyped_storage().data_ptr() in mine or v.untyped_storage().data_ptr() in mine):
             raise ValueError("k and v may not share the cache's memory")
     for x, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        if any(st == 0 and n > 1 for st, n in zip(x.stride(), x.shape)):
+        st = x.stride()
+        if 0 in st and any(y == 0 and z > 1 for y, z in zip(st, x.shape)):
             raise ValueError("%s is written: it may not be expanded" % name)
-    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (k, v, k_cache, v_cache, importance)):
+    if torch.is_grad_enabled() and (k_cache.requires_grad or v_cache.requires_grad or importance.requires_grad
+                                    or (k is not None and (k.requires_grad or v.requires_grad))):
         raise ValueError("Inference only: no backward implementation")
     if not _is_int(budget) or not 1 <= budget <= c:
         raise ValueError("budget must be an integer in [1, cache slots]")
@@ -262,7 +273,7 @@ def insert_tokens(k, v, k_cache, v_cache, importance, position, length, seen, bu
     if t == 0:
         k = v = k_cache                     # strides of a size-0 axis are not read
     L = _lib.lib()
-    ws_bytes = L.fe_insert_workspace_bytes(b, hk, a, c, budget)
+    ws_bytes = _insert_workspace(b, hk, a, c, budget)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device) if ws_bytes else None
     with _lib.on_device(device):
         rc = L.fe_insert_tokens(k.data_ptr() if t else None, v.data_ptr() if t else None, k_cache.data_ptr(), v_cache.data_ptr(),
