@@ -21,6 +21,7 @@
 //                          (few rows), the importance, whose probabilities need the joined lse
 //   decode_replay_kernel   the importance otherwise: S = Q K^T for the rows that stay, lanes holding keys, so that a
 //                          key's sum over the rows is in-lane: p = exp2(x log2e - bias), the bias holding lse and w
+//                          (decode_replay_elements_kernel for rows that do not allow 16-byte loads)
 //
 // Lengths are known on the device only, and differ from head to head, so a launch has as many blocks as the card
 // holds at once, and each takes an equal share of all tiles of all heads, in order (dec_share); the few-rows kernel's
@@ -110,6 +111,21 @@ struct DecFewArgs {
   int pad[9];
 };
 static_assert(offsetof(DecFewArgs, pad) <= 4 * 64 && sizeof(DecFewArgs) >= 4 * 64, "argument window");
+
+struct DecReplayArgs {
+  DecIn q, k, v, kc;
+  DecI32In length, path;   // path: or null, all T
+  DecF32In lse, imp, norm;
+  DecF32 imp_out, new_imp;
+  long long qb, qh, qn, kb, kh, vb, vh, kcb, kch;   // strides of batch, head, (q) row
+  long long imp_stride, norm_stride, impo_stride;
+  u32 kn, vn, kcn;         // row strides
+  int T, C, D, G, A, S;
+  u32 qand, qxor;
+  float scale_log2, decay_log2;
+  int pad[6];
+};
+static_assert(offsetof(DecReplayArgs, pad) <= 4 * 64 && sizeof(DecReplayArgs) >= 4 * 64, "argument window");
 
 struct DecFewJoinArgs {
   DecF32In part_o, part_ml, logits;
@@ -1435,15 +1451,196 @@ __device__ __forceinline__ int dec_path_len(const DecArgs& a, int b) {
   return __builtin_amdgcn_readfirstlane(len);
 }
 
+// Block (split, KV head, batch row), as decode_few_kernel. Rows r = g * A_b + i of the path, 64 at a time, with their Q in
+// registers as four tiles of 16; a wave takes 32 keys at a time, straight into the products' operands (a lane's 16
+// bytes of a key lie beside its neighbours' of the same key, 64 bytes in all), the next 32 on the way. More than 64
+// rows take K again, adding to what the rows before left.
+// What bounds it: reading K; on short caches the trips to memory one after the other (path, then its rows).
+template <typename E, int DP>
+__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_replay_kernel(const DecReplayArgs args) {
+  constexpr int NC = DP / 32, RT = 4, CH = 16 * RT;
+  __shared__ __attribute__((aligned(16))) float bias[CH];
+  __shared__ int place[CH], node[CH];      // a row's index on the path, and its token
+  const DecReplayArgs a = dec_hold<0, 4>(args);
+  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, lq = lane >> 4;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int hkv = (int)blockIdx.y, b = (int)blockIdx.z, bh = b * (int)gridDim.y + hkv;
+  const DecI32In path = a.path ? a.path + (long long)b * a.A : a.path;
+  int n = a.length[bh], na = a.A;
+  if (path) {
+    na = 0;
+    for (int i0 = 0; i0 < a.A; i0 += 64) {
+      const int x = path[min(i0 + lane, a.A - 1)];
+      const unsigned long long ok = __ballot(i0 + lane < a.A && x >= 0 && x < a.T);
+      const int run = ok == ~0ull ? 64 : __ffsll(~ok) - 1;
+      na += run;
+      if (run < 64) break;
+    }
+  }
+  n = __builtin_amdgcn_readfirstlane(min(max(n, 0), a.C));
+  const int nc = (n + 31) / 32, tiles = nc + (a.A + 31) / 32, share = dec_few_share(tiles, a.S);
+  const int t0 = (int)blockIdx.x * share, t1 = min(tiles, t0 + share);
+  if (t0 >= t1) return;
+  const int rend = a.G * na;
+  const DecIn kc = a.kc + b * a.kcb + hkv * a.kch, kn = a.k + b * a.kb + hkv * a.kh;
+  const float keep = fast_exp2(-a.decay_log2 * (float)na);
+
+#pragma unroll 1
+  for (int r0 = 0; r0 == 0 || r0 < rend; r0 += CH) {
+    __syncthreads();                        // the rows before are done with
+    if (tid < CH) {
+      const int r = r0 + tid;
+      float bs = -kDecNegInf;
+      int at = 0, nd = 0;
+      if (r < rend) {
+        const int g = r / na;
+        at = r - g * na;
+        nd = path ? path[at] : at;
+        const float z = a.lse[((long long)bh * a.G + g) * a.T + nd];
+        // nothing visible (lse = -inf): the row gives no weight
+        if (z != kDecNegInf) bs = z * (1.f / kLn2) + a.decay_log2 * (float)(na - 1 - at);
+        nd |= g << 16;
+      }
+      bias[tid] = bs;
+      place[tid] = at;
+      node[tid] = nd;
+    }
+    __syncthreads();
+    u32x4 qf[RT][NC];
+    f32x4 bs[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      if (16 * rt < rend - r0) {
+        const int nd = node[16 * rt + l16];   // a real row in any case
+        const DecIn qp = a.q + b * a.qb + (long long)(hkv * a.G + (nd >> 16)) * a.qh + (nd & 0xffff) * a.qn;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) qf[rt][c] = *(const FE_GLOBAL u32x4*)(qp + (DP == a.D || 32 * c + 8 * lq < a.D ? 32 * c + 8 * lq : 0));
+        bs[rt] = *(const f32x4*)(bias + 16 * rt + 4 * lq);
+      }
+    }
+    u32x4 kx[2][NC];
+    float ox = 0.f, wx = 1.f, old = 0.f, w = 1.f;   // importance and norm of key kb + lane (lanes below 32)
+    int t = -1, next = t0 + wv;
+    bool set = false;
+#pragma unroll 1
+    while (true) {
+      u32x4 kf[2][NC];
+      if (t >= 0) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int c = 0; c < NC; ++c) kf[s][c] = kx[s][c];
+        if (a.D != DP) {
+          int D = a.D;
+          asm volatile("" : "+s"(D));
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+              if (32 * c + 8 * lq >= D) kf[s][c] = (u32x4){0u, 0u, 0u, 0u};
+        }
+        old = ox;
+        w = wx;
+      }
+      if (next < t1) {
+        const bool nt = next >= nc;
+        const int kb = (nt ? next - nc : next) * 32;
+        int D = a.D;
+        asm volatile("" : "+s"(D));
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          u32 row = (u32)min(kb + 16 * s + l16, nt ? max(na, 1) - 1 : n - 1);
+          if (nt && path) row = (u32)min(max(path[row], 0), a.T - 1);   // new rows in the path's order
+          const DecIn kp = (nt ? kn : kc) + (unsigned long long)row * (nt ? a.kn : a.kcn);
+#pragma unroll
+          for (int c = 0; c < NC; ++c) kx[s][c] = *(const FE_GLOBAL u32x4*)(kp + (32 * c + 8 * lq < D ? 32 * c + 8 * lq : 0));
+        }
+        if (!nt && lane < 32) {
+          const int key = min(kb + lane, n - 1);
+          ox = r0 ? a.imp_out[bh * a.impo_stride + key] : a.imp[bh * a.imp_stride + key];
+          if (a.norm) wx = a.norm[bh * a.norm_stride + key];
+        }
+      }
+      if (!set) {
+        set = true;
+        if (a.qand != ~0u || a.qxor != 0u || a.D != DP) {
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+              const u32 kept = 32 * c + 8 * lq < a.D ? a.qand : 0u, flip = kept ? a.qxor : 0u;
+              qf[rt][c] = (qf[rt][c] & kept) ^ flip;
+            }
+        }
+      }
+      if (t >= 0) {
+        const bool tail = t >= nc;
+        const int kb = (tail ? t - nc : t) * 32;
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          if (16 * rt < rend - r0) {
+            // lanes hold keys kb + 16 s + l16; register i holds row 16 rt + 4 lq + i
+            f32x4 x[2];
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+              for (int c = 0; c < NC; ++c) x[s] = dec_mfma16<E>(qf[rt][c], kf[s][c], c == 0 ? (f32x4){0.f, 0.f, 0.f, 0.f} : x[s]);
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) x[s][i] = fast_exp2(x[s][i] * a.scale_log2 - bs[rt][i]);
+            if (tail || 16 * (rt + 1) > rend - r0) {
+              int left = rend - r0;
+              asm volatile("" : "+s"(left));   // compared here, not kept as masks across the loop
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int rr = 16 * rt + 4 * lq + i, at = place[rr];
+#pragma unroll
+                for (int s = 0; s < 2; ++s)     // no row, whatever the key; row `at` of the path sees new row u <= at
+                  if (rr >= left || (tail && at < kb + 16 * s + l16)) x[s][i] = 0.f;
+              }
+            }
+#pragma unroll
+            for (int s = 0; s < 2; ++s) sum[s] += (x[s][0] + x[s][1]) + (x[s][2] + x[s][3]);
+          }
+        }
+        const float s0 = dec_quad_sum(sum[0]), s1 = dec_quad_sum(sum[1]);
+        const float total = lq == 0 ? s0 : s1;
+        const int key = kb + lane;
+        if (!tail) {
+          if (lane < 32 && key < n) a.imp_out[bh * a.impo_stride + key] = old * (r0 ? 1.f : keep) + w * total;
+        } else if (lane < 32 && key < a.A) {
+          float nu = 1.f;
+          if (a.norm && key < na) {
+            const FE_GLOBAL u32x4* vp =
+                (const FE_GLOBAL u32x4*)(a.v + b * a.vb + hkv * a.vh + (unsigned long long)(u32)(path ? path[key] : key) * a.vn);
+            nu = 0.f;
+            for (int d = 0; d < a.D / 8; ++d) {
+              const u32x4 y = vp[d];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) nu += fabsf(E::to_f32((u16)y[i])) + fabsf(E::to_f32((u16)(y[i] >> 16)));
+            }
+          }
+          const DecF32 to = a.new_imp + (long long)bh * a.A + key;
+          *to = (r0 ? *to : 0.f) + (key < na ? nu * total : 0.f);
+        }
+      }
+      if (next >= t1) break;
+      t = next;
+      next += 4;
+    }
+  }
+}
+
 // Rows whose Q is in LDS at a time.
 template <int DP>
 constexpr int dec_replay_rows() { return DP > 128 ? 32 : 64; }
 
-// What bounds it: reading K. A wave takes 32 keys at a time through its own LDS into registers, the next 32 on the
-// way, against the rows' Q in LDS. More rows than that has room for take K again (from L2 mostly), adding to what
-// the rows before left.
-template <typename E, int DP, int VEC>
-__global__ __launch_bounds__(256, 2) void decode_replay_kernel(const DecArgs args) {
+// Any layout, element by element: a wave takes 32 keys at a time through its own LDS into registers, against the rows'
+// Q in LDS. More rows than that has room for take K again, adding to what the rows before left.
+template <typename E, int DP>
+__global__ __launch_bounds__(256, 2) void decode_replay_elements_kernel(const DecArgs args) {
   constexpr int NDC = DP / 16, CPR = DP / 8, TILE = 64 * DP, CH = dec_replay_rows<DP>();
   __shared__ __attribute__((aligned(1024))) unsigned char lds[4][TILE];
   __shared__ __attribute__((aligned(1024))) unsigned char lds_q[CH * DP * 2];
@@ -1465,13 +1662,8 @@ __global__ __launch_bounds__(256, 2) void decode_replay_kernel(const DecArgs arg
     const DecI32In path = a.path ? a.path + (long long)b * a.A : (DecI32In) nullptr;
     const float keep = fast_exp2(-a.decay_log2 * (float)na);
 
-    u32x4 kx[VEC ? NDC : 1] = {};
     const DecRows hr = dec_rows(a, b, hkv);
-    auto load = [&](int t) __attribute__((always_inline)) {
-      if constexpr (VEC) dec_load_rows<DP, 32, 64>(hr.kc, hr.kcs, t * 32, n, a.D, lane, kx);
-    };
     for (int r0 = 0; r0 == 0 || r0 < rows; r0 += CH) {
-      if (VEC && t0 + wv < min(t1, nc)) load(t0 + wv);
       __syncthreads();                      // the rows before are done with
       for (int i = threadIdx.x; i < CH; i += 256) {
         const int r = r0 + i;
@@ -1494,11 +1686,7 @@ __global__ __launch_bounds__(256, 2) void decode_replay_kernel(const DecArgs arg
         if (r < rows) {
           const int g = r / na, node = path ? path[r - g * na] : r - g * na;
           const DecIn qp = a.q + b * a.qs[0] + (hkv * a.G + g) * a.qs[1] + node * a.qs[2];
-          if (VEC) {
-            if (8 * ch < a.D) x = (*(const FE_GLOBAL u32x4*)(qp + 8 * ch) & a.qand) ^ a.qxor;
-          } else {
-            x = (dec_load8(qp, a.qc, ch, a.D) & a.qand) ^ a.qxor;
-          }
+          x = (dec_load8(qp, a.qc, ch, a.D) & a.qand) ^ a.qxor;
         }
         *(u32x4*)(lds_q + dec_k_at<DP>(e / CPR, ch)) = x;
       }
@@ -1508,25 +1696,15 @@ __global__ __launch_bounds__(256, 2) void decode_replay_kernel(const DecArgs arg
       for (int t = t0 + wv; t < t1; t += 4) {
         const bool tail = t >= nc;
         const int kb = tail ? (t - nc) * 32 : t * 32, krows = tail ? na : n;
-        if (VEC && !tail) {
-#pragma unroll
-          for (int i = 0; i < NDC; ++i) {
-            const int e = i * 64 + lane;
-            *(u32x4*)(lds[wv] + dec_k_at<DP>(e / CPR, e % CPR)) = kx[i];
-          }
-          if (t + 4 < min(t1, nc)) load(t + 4);
-        } else {
+        {
           const DecIn kp = tail ? hr.k : hr.kc;
-          const long long krs = tail ? hr.ks : hr.kcs, kcs = VEC ? 1 : tail ? a.knc : a.kcc;
+          const long long krs = tail ? hr.ks : hr.kcs, kcs = tail ? a.knc : a.kcc;
 #pragma unroll 1
           for (int i = 0; i < NDC; ++i) {
             const int e = i * 64 + lane, key = kb + e / CPR, ch = e % CPR;
             const int row = tail && path && key < krows ? path[key] : key;   // new rows in the path's order
             u32x4 x = {0u, 0u, 0u, 0u};
-            if (key < krows) {
-              if (!VEC) x = dec_load8(kp + row * krs, kcs, ch, a.D);
-              else if (8 * ch < a.D) x = *(const FE_GLOBAL u32x4*)(kp + row * krs + 8 * ch);
-            }
+            if (key < krows) x = dec_load8(kp + row * krs, kcs, ch, a.D);
             *(u32x4*)(lds[wv] + dec_k_at<DP>(e / CPR, ch)) = x;
           }
         }
@@ -1565,9 +1743,8 @@ __global__ __launch_bounds__(256, 2) void decode_replay_kernel(const DecArgs arg
             w = 1.f;
             if (a.norm) {
               const DecIn vp = hr.v + (path ? path[key] : key) * hr.vs;
-              const long long vnc = VEC ? 1 : a.vnc;
               w = 0.f;
-              for (int d = 0; d < a.D; ++d) w += fabsf(E::to_f32(vp[d * vnc]));
+              for (int d = 0; d < a.D; ++d) w += fabsf(E::to_f32(vp[d * a.vnc]));
             }
           }
           const DecF32 to = a.new_imp + (long long)bh * a.A + key;
@@ -1583,7 +1760,7 @@ __global__ __launch_bounds__(256, 2) void decode_replay_kernel(const DecArgs arg
   {DP, T, {(const void*)decode_few_kernel<E, DP>, (const void*)decode_few_join_kernel<E, DP>}, {(const void*)decode_rows_kernel<E, DP, 0>, (const void*)decode_rows_kernel<E, DP, 1>},                       \
    {(const void*)decode_wide_kernel<E, DP, 4>, (const void*)decode_wide_kernel<E, DP, (DP > 128 ? 4 : 8)>},              \
    (const void*)decode_join_kernel<E, DP>,                                                                              \
-   {(const void*)decode_replay_kernel<E, DP, 0>, (const void*)decode_replay_kernel<E, DP, 1>}},
+   {(const void*)decode_replay_elements_kernel<E, DP>, (const void*)decode_replay_kernel<E, DP>}},
 #define FE_DEC_ROWS(DP) FE_DEC_ROW(DP, F16, FE_DTYPE_F16) FE_DEC_ROW(DP, BF16, FE_DTYPE_BF16)
 // Kernels by tile dim. rows and replay: the second takes operands whose rows all allow 16-byte loads. wide: of four
 // waves, and of eight where their registers allow it.
@@ -1729,11 +1906,44 @@ int dec_launch(const char* who, const void* fn, dim3 grid, dim3 block, A& a, hip
   return FE_OK;
 }
 
-int dec_replay(const char* who, const DecKernels& kn, bool vec, DecArgs& a, hipStream_t stream) {
-  // as many blocks as the card holds at once, of at least a tile a wave
-  const long long tiles = (long long)a.BH * ((a.C + 31) / 32 + (a.A + 31) / 32);
-  a.nb = (int)std::max<long long>(1, std::min<long long>(kn.dp > 128 ? 512 : 768, (tiles + 3) / 4));
-  return dec_launch(who, kn.replay[vec], dim3((unsigned)a.nb), dim3(256), a, stream);
+// st: strides of q, k, v and the K cache.
+int dec_replay(const char* who, const DecKernels& kn, bool vec, DecArgs& a, int64_t B, const long long (*st)[4], hipStream_t stream) {
+  const long long max_tiles = (a.C + 31) / 32 + (a.A + 31) / 32;
+  if (vec && std::max({st[1][2], st[2][2], st[3][2]}) <= 0x7fffffffLL && a.Hkv <= 65535 && B <= 65535) {
+    DecReplayArgs r = {};
+    r.q = a.q;
+    r.k = a.k;
+    r.v = a.v;
+    r.kc = a.kc;
+    r.length = a.length;
+    r.path = a.path;
+    r.lse = a.lse_in;
+    r.imp = a.imp;
+    r.norm = a.norm;
+    r.imp_out = a.imp_out;
+    r.new_imp = a.new_imp;
+    r.qb = st[0][0], r.qh = st[0][1], r.qn = st[0][2];
+    r.kb = st[1][0], r.kh = st[1][1], r.kn = (u32)st[1][2];
+    r.vb = st[2][0], r.vh = st[2][1], r.vn = (u32)st[2][2];
+    r.kcb = st[3][0], r.kch = st[3][1], r.kcn = (u32)st[3][2];
+    r.imp_stride = a.imp_stride;
+    r.norm_stride = a.norm_stride;
+    r.impo_stride = a.impo_stride;
+    r.T = a.T;
+    r.C = a.C;
+    r.D = a.D;
+    r.G = a.G;
+    r.A = a.A;
+    r.qand = a.qand;
+    r.qxor = a.qxor;
+    r.scale_log2 = a.scale_log2;
+    r.decay_log2 = a.decay_log2;
+    // as many blocks as the card holds at once, of at least a tile a wave
+    r.S = (int)std::max<long long>(1, std::min<long long>((kn.dp > 128 ? 256 : 512) / a.BH, (max_tiles + 3) / 4));
+    return dec_launch(who, kn.replay[1], dim3((unsigned)r.S, (unsigned)a.Hkv, (unsigned)B), dim3(256), r, stream);
+  }
+  a.nb = (int)std::max<long long>(1, std::min<long long>(512, ((long long)a.BH * max_tiles + 3) / 4));
+  return dec_launch(who, kn.replay[0], dim3((unsigned)a.nb), dim3(256), a, stream);
 }
 
 }  // namespace
@@ -1945,7 +2155,7 @@ extern "C" int fe_decode_attention(const void* q, const void* k, const void* v, 
   if (int rc = dec_launch(who, kn.join, dim3((unsigned)blocks), dim3(256), o, stream)) return rc;
   if (!importance || logits) return FE_OK;
   dec_set(a.lse_in, lse);
-  return dec_replay(who, kn, vec, a, stream);
+  return dec_replay(who, kn, vec, a, B, st, stream);
 }
 
 extern "C" int fe_replay_path(const void* q, const void* k, const void* v, const void* k_cache, const int32_t* length,
@@ -1988,5 +2198,5 @@ extern "C" int fe_replay_path(const void* q, const void* k, const void* v, const
   dec_set(a.imp_out, importance_out);
   a.impo_stride = importance_out_stride;
   dec_set(a.new_imp, new_importance);
-  return dec_replay(who, kn, vec, a, (hipStream_t)hip_stream);
+  return dec_replay(who, kn, vec, a, B, st, (hipStream_t)hip_stream);
 }
