@@ -112,6 +112,21 @@ struct DecFewArgs {
 };
 static_assert(offsetof(DecFewArgs, pad) <= 4 * 64 && sizeof(DecFewArgs) >= 4 * 64, "argument window");
 
+struct DecWideArgs {
+  DecIn q, k, v, kc, vc;
+  DecI32In length;
+  const FE_GLOBAL unsigned char* tree;
+  DecF32 part_o, part_ml;
+  FE_GLOBAL int* seg;
+  long long qb, qh, qn, kb, kh, vb, vh, kcb, kch, vcb, vch, tree_stride;   // strides of batch, head, (q) row
+  u32 kn, vn, kcn, vcn;    // row strides
+  int T, C, D, G, Hkv, BH, R, RB, RW, nb;
+  u32 qand, qxor;
+  float scale_log2;
+  int pad[3];
+};
+static_assert(offsetof(DecWideArgs, pad) <= 4 * 64 && sizeof(DecWideArgs) >= 4 * 64, "argument window");
+
 struct DecReplayArgs {
   DecIn q, k, v, kc;
   DecI32In length, path;   // path: or null, all T
@@ -191,7 +206,8 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kDecNegInf = -__builtin_huge_valf();
 
 // Rows of the (b, j) cache, within the tensor whatever the caller's length says.
-__device__ __forceinline__ int dec_len(const DecArgs& a, int bh) { return min(max(a.length[bh], 0), a.C); }
+template <typename A>
+__device__ __forceinline__ int dec_len(const A& a, int bh) { return min(max(a.length[bh], 0), a.C); }
 
 // Orders a wave's own LDS writes and reads (the hardware keeps them in order; the compiler is told).
 __device__ __forceinline__ void dec_wave_order() {
@@ -275,8 +291,8 @@ struct DecShare {
   int pos, hi, base, bh;
   int len;                 // lane i: rows of head (bh & ~63) + i
 };
-template <int KT, int PER>
-__device__ __forceinline__ DecShare dec_share(const DecArgs& a, int segs, int fresh) {
+template <int KT, int PER, typename A>
+__device__ __forceinline__ DecShare dec_share(const A& a, int segs, int fresh) {
   const int lane = threadIdx.x & 63;
   auto tiles = [&](int len, int bh) { return bh < a.BH ? segs * dec_tiles<KT>(len, fresh) : 0; };
   auto length = [&](int bh) { return bh < a.BH ? dec_len(a, bh) : 0; };
@@ -313,7 +329,8 @@ __device__ __forceinline__ DecShare dec_share(const DecArgs& a, int segs, int fr
 // Rows of the share's current head.
 __device__ __forceinline__ int dec_share_len(const DecShare& s) { return __builtin_amdgcn_readlane(s.len, s.bh & 63); }
 // On to the next head.
-__device__ __forceinline__ void dec_share_next(const DecArgs& a, DecShare& s) {
+template <typename A>
+__device__ __forceinline__ void dec_share_next(const A& a, DecShare& s) {
   s.base = s.pos;
   ++s.bh;
   if ((s.bh & 63) == 0) {
@@ -324,7 +341,8 @@ __device__ __forceinline__ void dec_share_next(const DecArgs& a, DecShare& s) {
 
 // Which of a lane's 16 keys of 32 from kb (bit i: key kb + 8 (i / 4) + 4 hh + i % 4) query token tq sees, among the
 // cache's rows (fresh false) or the new ones.
-__device__ __forceinline__ u32 dec_visible(const DecArgs& a, int b, int tq, int kb, int rows, bool fresh) {
+template <typename A>
+__device__ __forceinline__ u32 dec_visible(const A& a, int b, int tq, int kb, int rows, bool fresh) {
   const int k0 = kb + 4 * (int)((threadIdx.x >> 5) & 1);
   const FE_GLOBAL unsigned char* row = a.tree + b * a.tree_stride + tq * a.T;
   u32 bits = 0;
@@ -438,7 +456,8 @@ __device__ __forceinline__ void dec_set_q(const DecArgs& a, bool valid, u32x4 (&
 
 // The segment's place in the tables, and its first and last slot, by the blocks that hold its ends. A block's
 // segments follow each other, so block + segment numbers every (block, segment) pair apart.
-__device__ __forceinline__ int dec_slot(const DecArgs& a, int seg, bool head, bool end) {
+template <typename A>
+__device__ __forceinline__ int dec_slot(const A& a, int seg, bool head, bool end) {
   const int slot = (int)blockIdx.x + seg;
   if (threadIdx.x == 0) {
     if (head) a.seg[2 * seg] = slot;
@@ -1047,17 +1066,20 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_rows_kernel(cons
 // What bounds it: vector work beside the products (an exponential a logit); at 256 rows a tile takes about as long as
 // its bytes from HBM.
 template <typename E, int DP, int NW>
-__global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void decode_wide_kernel(const DecArgs args) {
+__global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void decode_wide_kernel(const DecWideArgs args) {
   constexpr int NDC = DP / 16, NDT = DP / 32, CPR = DP / 8, TILE = 128 * DP;   // bytes of 64 rows
   constexpr int NT = NW * 64, NL = (64 * CPR + NT - 1) / NT;
   __shared__ __attribute__((aligned(1024))) unsigned char lds_k[2][TILE], lds_v[2][TILE];
   __shared__ u32 s_odd[2][2];            // keys of a tile of new rows with a value that is not finite
   __shared__ float s_row[NW][DP];        // such a value, by each wave
+  const DecWideArgs a = dec_hold<0, 4>(args);
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  u32 ones2;
+  asm volatile("s_mov_b32 %0, %1" : "=s"(ones2) : "i"(E::kOnes2));
 
-  const DecArgs a = dec_hold<kDecAttnArgs, 5>(args);
   DecShare sh = dec_share<64, 1>(a, a.RB, a.T);
+#pragma unroll 1
   while (sh.pos < sh.hi) {
     const int bh = sh.bh, b = bh / a.Hkv, hkv = bh - b * a.Hkv;
     const int n = dec_share_len(sh);
@@ -1071,162 +1093,199 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void decode_wide_kernel(
     const bool live = wv < a.RW && (rb * a.RW + wv) * 32 < a.R;   // the wave has rows
     const bool rv = live && r < a.R;
     const int g = rv ? r / a.T : 0, tq = rv ? r - g * a.T : 0;
-    const DecRows hr = dec_rows(a, b, hkv);
+    const DecIn kc = a.kc + b * a.kcb + hkv * a.kch, vc = a.vc + b * a.vcb + hkv * a.vch;
+    const DecIn kn = a.k + b * a.kb + hkv * a.kh, vn = a.v + b * a.vb + hkv * a.vh;
     u32x4 qf[NDC];
-    dec_read_q<DP, 1>(a, b, hkv * a.G + g, tq, qf);
+    {
+      const DecIn qp = a.q + b * a.qb + (long long)(hkv * a.G + g) * a.qh + tq * a.qn;
+      int D = a.D;
+      asm volatile("" : "+s"(D));
+#pragma unroll
+      for (int c = 0; c < NDC; ++c) qf[c] = *(const FE_GLOBAL u32x4*)(qp + (16 * c + 8 * hh < D ? 16 * c + 8 * hh : 0));
+    }
     f32x16 o[NDT];
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) o[dt] = (f32x16){};
     float m = kDecNegInf, nm = 0.f, l = 0.f, lr = 0.f;   // lane-wise sums (half of a row's keys each)
-    u32 ones2;
-    asm volatile("s_mov_b32 %0, %1" : "=s"(ones2) : "i"(E::kOnes2));
-
     u32x4 kx[NL] = {}, vx[NL] = {};
+    // a tile's rows on their way (past the last, the last), and into LDS
     auto load = [&](int t) __attribute__((always_inline)) {
-      const DecTile at = dec_tile<64>(hr, n, nc, a.T, t);
-      dec_load_rows<DP, 64, NT>(at.k, at.krs, at.kb, at.rows, a.D, tid, kx);
-      dec_load_rows<DP, 64, NT>(at.v, at.vrs, at.kb, at.rows, a.D, tid, vx);
-    };
-    auto store = [&](int t, int buf) __attribute__((always_inline)) {
-      const DecTile at = dec_tile<64>(hr, n, nc, a.T, t);
-      if (at.kb + 64 > at.rows) dec_cut_rows<DP, NT>(at.kb, at.rows, tid, vx);
+      const bool nt = t >= nc;
+      const int kb = (nt ? t - nc : t) * 64, last = (nt ? a.T : n) - 1;
+      const DecIn kp = nt ? kn : kc, vp = nt ? vn : vc;
+      const u32 ks = nt ? a.kn : a.kcn, vs = nt ? a.vn : a.vcn;
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
-        const int e = i * NT + tid, key = e / CPR, ch = e % CPR;
-        if (64 * CPR % NT == 0 || key < 64) {
-          *(u32x4*)(lds_k[buf] + dec_k_at<DP>(key, ch)) = kx[i];
-          *(u32x4*)(lds_v[buf] + dec_v_at<DP>(key, ch)) = vx[i];
+        const int e = i * NT + tid, ch = 8 * (e % CPR);
+        const u32 row = (u32)min(kb + e / CPR, last);
+        const int cc = ch < a.D ? ch : 0;
+        kx[i] = *(const FE_GLOBAL u32x4*)(kp + (unsigned long long)row * ks + cc);
+        vx[i] = *(const FE_GLOBAL u32x4*)(vp + (unsigned long long)row * vs + cc);
+      }
+    };
+    auto store = [&](int t) __attribute__((always_inline)) {
+      const int buf = t & 1;
+      const bool nt = t >= nc;
+      const int kb = (nt ? t - nc : t) * 64, rows = nt ? a.T : n;
+      if (kb + 64 > rows) dec_cut_rows<DP, NT>(kb, rows, tid, vx);
+      if (a.D != DP) {
+        int D = a.D;
+        asm volatile("" : "+s"(D));
+#pragma unroll
+        for (int i = 0; i < NL; ++i)
+          if (8 * ((i * NT + tid) % CPR) >= D) kx[i] = (u32x4){0u, 0u, 0u, 0u};
+      }
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const int e = i * NT + tid;
+        if (64 * CPR % NT == 0 || e < 64 * CPR) {
+          *(u32x4*)(lds_k[buf] + dec_k_at<DP>(e / CPR, e % CPR)) = kx[i];
+          *(u32x4*)(lds_v[buf] + dec_v_at<DP>(e / CPR, e % CPR)) = vx[i];
         }
       }
-      if (t >= nc) {
+      if (nt) {
         if (tid < 2) s_odd[buf][tid] = 0u;
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
           const int key = (i * NT + tid) / CPR;
-          if (dec_nonfinite<E>(vx[i])) atomicOr(&s_odd[buf][key >> 5], 1u << (key & 31));
+          if (key < 64 && dec_nonfinite<E>(vx[i])) atomicOr(&s_odd[buf][key >> 5], 1u << (key & 31));
         }
       }
     };
     load(t0);
-    dec_set_q<DP>(a, rv, qf);
-    store(t0, t0 & 1);
+    // (unconditionally: fragments changed in a branch cost 250 spilled registers)
+#pragma unroll
+    for (int c = 0; c < NDC; ++c) {
+      const u32 keep = rv && 16 * c + 8 * hh < a.D ? a.qand : 0u, flip = keep ? a.qxor : 0u;
+      qf[c] = (qf[c] & keep) ^ flip;
+    }
+    store(t0);
     __syncthreads();
+#pragma unroll 1
     for (int t = t0; t < t1; ++t) {
-      const int buf = t & 1;
-      const bool tail = t >= nc;
-      const int kb = tail ? (t - nc) * 64 : t * 64, rows = tail ? a.T : n;
-      unsigned char* kt = lds_k[buf];
-      unsigned char* vt = lds_v[buf];
       if (t + 1 < t1) load(t + 1);
-      unsigned long long odd = 0;
-      if (tail) {
-        odd = ((unsigned long long)s_odd[buf][1] << 32) | s_odd[buf][0];
-        if (odd) {
-          for (int e = tid; e < 64 * CPR; e += NT)
-            if ((odd >> (e / CPR)) & 1u) *(u32x4*)(vt + dec_v_at<DP>(e / CPR, e % CPR)) = (u32x4){0u, 0u, 0u, 0u};
-          __syncthreads();
+      {
+        const int buf = t & 1;
+        const bool tail = t >= nc;
+        const int kb = (tail ? t - nc : t) * 64, rows = tail ? a.T : n;
+        unsigned char* kt = lds_k[buf];
+        unsigned char* vt = lds_v[buf];
+        unsigned long long odd = 0;
+        if (tail) {
+          odd = ((unsigned long long)s_odd[buf][1] << 32) | s_odd[buf][0];
+          if (odd) {
+            for (int e = tid; e < 64 * CPR; e += NT)
+              if ((odd >> (e / CPR)) & 1u) *(u32x4*)(vt + dec_v_at<DP>(e / CPR, e % CPR)) = (u32x4){0u, 0u, 0u, 0u};
+            __syncthreads();
+          }
         }
-      }
-      if (live) {
-        u32 vis[2] = {~0u, ~0u};
-        const bool masked = tail || kb + 64 > rows;
-        if (masked) {
-          vis[0] = dec_visible(a, b, tq, kb, rows, tail);
-          vis[1] = dec_visible(a, b, tq, kb + 32, rows, tail);
-        }
-        f32x16 x[2];                       // logits, then probabilities
-        auto logits = [&]() __attribute__((always_inline)) {
-#pragma unroll
-          for (int s = 0; s < 2; ++s) {
-#pragma unroll
-            for (int c = 0; c < NDC; ++c)
-              x[s] = c == 0 ? E::mfma(dec_kfrag<DP>(kt, 32 * s, 0), qf[0], (f32x16){}) : E::mfma(dec_kfrag<DP>(kt, 32 * s, c), qf[c], x[s]);
-            if (masked) {
-#pragma unroll
-              for (int i = 0; i < 16; ++i) x[s][i] = (vis[s] >> i) & 1u ? x[s][i] : kDecNegInf;
+        if (live) {
+          u32 vis[2] = {~0u, ~0u};
+          const bool masked = tail || kb + 64 > rows;
+          if (masked) {
+#pragma unroll 1
+            for (int s = 0; s < 2; ++s) {
+              const u32 x = dec_visible(a, b, tq, kb + 32 * s, rows, tail);
+              vis[0] = s ? vis[0] : x;
+              vis[1] = x;
             }
           }
-        };
-        float ls;
-        auto exponentials = [&]() __attribute__((always_inline)) {
-          ls = 0.f;
+          f32x16 x[2];                     // logits, then probabilities
+          auto logits = [&]() __attribute__((always_inline)) {
 #pragma unroll
-          for (int s = 0; s < 2; ++s)
+            for (int s = 0; s < 2; ++s) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              x[s][i] = fast_exp2(x[s][i] * a.scale_log2 + nm);
-              ls += x[s][i];
+              for (int c = 0; c < NDC; ++c) {
+                if (c % 4 == 0) __builtin_amdgcn_sched_barrier(0);   // four fragments in flight
+                x[s] = c == 0 ? E::mfma(dec_kfrag<DP>(kt, 32 * s, 0), qf[0], (f32x16){}) : E::mfma(dec_kfrag<DP>(kt, 32 * s, c), qf[c], x[s]);
+              }
             }
-        };
-        logits();
-        exponentials();
-        const bool over = !(ls <= E::kMaxTileSum) || m == kDecNegInf;
-        if (__ballot(over)) {
-          // a new reference for rows without one, and for those whose probabilities grew too large
+            if (masked) {
+#pragma unroll
+              for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[s][i] = (vis[s] >> i) & 1u ? x[s][i] : kDecNegInf;
+            }
+          };
+          float ls;
+          auto exponentials = [&]() __attribute__((always_inline)) {
+            ls = 0.f;
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                x[s][i] = fast_exp2(x[s][i] * a.scale_log2 + nm);
+                ls += x[s][i];
+              }
+          };
           logits();
-          float mx = kDecNegInf;
+          exponentials();
+          const bool over = !(ls <= E::kMaxTileSum) || m == kDecNegInf;
+          if (__ballot(over)) {
+            // a new reference for rows without one, and for those whose probabilities grew too large
+            logits();
+            float mx = kDecNegInf;
 #pragma unroll
-          for (int s = 0; s < 2; ++s)
+            for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x[s][i]);
-          mx = half_swap_max(mx) * a.scale_log2;
-          if (half_swap_max(over ? 1.f : 0.f) > 0.f && mx > m) {
-            const float alpha = m == kDecNegInf ? 0.f : fast_exp2(m - mx);
-            m = mx;
-            nm = -mx;
+              for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x[s][i]);
+            mx = half_swap_max(mx) * a.scale_log2;
+            const bool take = half_swap_max(over ? 1.f : 0.f) > 0.f && mx > m;
+            const float alpha = !take ? 1.f : m == kDecNegInf ? 0.f : fast_exp2(m - mx);
+            m = take ? mx : m;
+            nm = take ? -mx : nm;
             l *= alpha;
             lr *= alpha;
 #pragma unroll
             for (int dt = 0; dt < NDT; ++dt) o[dt] *= alpha;
+            exponentials();
           }
-          exponentials();
-        }
-        if (odd) {
-          const DecIn vp = hr.v;
+          if (odd) {
 #pragma unroll 1
-          for (unsigned long long left = odd; left; left &= left - 1) {
-            const int key = __ffsll(left) - 1;
-            // the register and half that hold the key, where the lane's query sees it
-            float mine = -1.f;
+            for (unsigned long long left = odd; left; left &= left - 1) {
+              const int key = __ffsll(left) - 1;
+              // the register and half that hold the key, where the lane's query sees it
+              float mine = -1.f;
 #pragma unroll
-            for (int s = 0; s < 2; ++s)
+              for (int s = 0; s < 2; ++s)
 #pragma unroll
-              for (int i = 0; i < 16; ++i)
-                if (key == 32 * s + 8 * (i >> 2) + 4 * hh + (i & 3) && ((vis[s] >> i) & 1u)) mine = x[s][i];
-            const float pk = half_swap_max(mine);      // probabilities are not negative
-            const float nan = half_swap_max(mine != mine ? 1.f : 0.f);
-            const float pr = nan > 0.f ? __builtin_nanf("") : pk;
-            const bool sees = pk >= 0.f || nan > 0.f;
-            const DecIn row = vp + (long long)(kb + key) * hr.vs;
-            for (int ch = lane; ch < DP; ch += 64) s_row[wv][ch] = ch < a.D ? E::to_f32(row[ch]) : 0.f;
-            dec_wave_order();
+                for (int i = 0; i < 16; ++i)
+                  if (key == 32 * s + 8 * (i >> 2) + 4 * hh + (i & 3) && ((vis[s] >> i) & 1u)) mine = x[s][i];
+              const float pk = half_swap_max(mine);      // probabilities are not negative
+              const float nan = half_swap_max(mine != mine ? 1.f : 0.f);
+              const float pr = nan > 0.f ? __builtin_nanf("") : pk;
+              const bool sees = pk >= 0.f || nan > 0.f;
+              const DecIn row = vn + (unsigned long long)(kb + key) * a.vn;
+              for (int ch = lane; ch < DP; ch += 64) s_row[wv][ch] = ch < a.D ? E::to_f32(row[ch]) : 0.f;
+              dec_wave_order();
 #pragma unroll
-            for (int dt = 0; dt < NDT; ++dt)
+              for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const float y = s_row[wv][32 * dt + 8 * (i >> 2) + 4 * hh + (i & 3)];
-                if (sees) o[dt][i] += pr * y;
-              }
-            dec_wave_order();
-          }
-        }
-        l += ls;
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-          for (int c4 = 0; c4 < 2; ++c4) {
-            u32x4 pf;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              pf[i] = E::pack2(x[s][8 * c4 + 2 * i], x[s][8 * c4 + 2 * i + 1]);
-              lr = E::sum2(pf[i], ones2, lr);
+                for (int i = 0; i < 16; ++i) {
+                  const float y = s_row[wv][32 * dt + 8 * (i >> 2) + 4 * hh + (i & 3)];
+                  if (sees) o[dt][i] += pr * y;
+                }
+              dec_wave_order();
             }
-#pragma unroll
-            for (int dt = 0; dt < NDT; ++dt) o[dt] = E::mfma(dec_vfrag<DP>(vt, 32 * s + 16 * c4, dt), pf, o[dt]);
           }
+          l += ls;
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int c4 = 0; c4 < 2; ++c4) {
+              u32x4 pf;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                pf[i] = E::pack2(x[s][8 * c4 + 2 * i], x[s][8 * c4 + 2 * i + 1]);
+                lr = E::sum2(pf[i], ones2, lr);
+              }
+#pragma unroll
+              for (int dt = 0; dt < NDT; ++dt) o[dt] = E::mfma(dec_vfrag<DP>(vt, 32 * s + 16 * c4, dt), pf, o[dt]);
+            }
+        }
       }
-      if (t + 1 < t1) store(t + 1, buf ^ 1);
+      if (t + 1 < t1) store(t + 1);
       __syncthreads();
     }
 
@@ -1236,12 +1295,12 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void decode_wide_kernel(
     if (rv) {
       const float inv = lr == 0.f ? 0.f : 1.f / lr;
       const int row = wv * 32 + l32;
-      const DecF32 po = a.part_o + ((long long)slot * a.RW * 32 + row) * DP;
+      const DecF32 po = a.part_o + ((long long)slot * a.RW * 32 + row) * DP + 4 * hh;
 #pragma unroll
       for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          *(FE_GLOBAL f32x4*)(po + 32 * dt + 8 * i + 4 * hh) =
+          *(FE_GLOBAL f32x4*)(po + 32 * dt + 8 * i) =
               (f32x4){o[dt][4 * i] * inv, o[dt][4 * i + 1] * inv, o[dt][4 * i + 2] * inv, o[dt][4 * i + 3] * inv};
       if (hh == 0) {
         a.part_ml[(long long)slot * 64 * a.RW + row] = m;
@@ -1861,7 +1920,7 @@ DecPlan dec_plan(int64_t BH, int64_t R, int64_t C, int64_t T, int64_t DP, bool v
   DecPlan p = {};
   const int64_t RT = (R + 31) / 32;
   p.few = vec && near && R <= 16;
-  p.wide = vec && RT > 1;
+  p.wide = vec && near && RT > 1;
   if (p.wide) {
     p.waves = DP > 128 || RT <= 4 ? 4 : 8;
     p.RB = (int)((RT + p.waves - 1) / p.waves);
@@ -2033,7 +2092,7 @@ extern "C" int fe_decode_attention(const void* q, const void* k, const void* v, 
   dec_set(a.tree, tree);
   a.tree_stride = tree_batch_stride;
   a.R = a.G * a.T;
-  // the few-rows kernel takes 32-bit row strides, and heads and batch rows as grid axes
+  // the few-rows and wide kernels take 32-bit row strides, the former heads and batch rows as grid axes
   const bool near = std::max({st[1][2], st[2][2], st[3][2], st[4][2]}) <= 0x7fffffffLL && Hkv <= 65535 && B <= 65535;
   const DecPlan p = dec_plan(a.BH, a.R, C, T, kn.dp, vec, near, importance != nullptr);
   const bool logits = importance && a.R <= kDecLogitRows;
@@ -2104,7 +2163,37 @@ extern "C" int fe_decode_attention(const void* q, const void* k, const void* v, 
     return dec_launch(who, kn.few[1], dim3((unsigned)(a.R + per), (unsigned)Hkv, (unsigned)B), dim3(256), o, stream);
   }
   if (p.wide) {
-    if (int rc = dec_launch(who, kn.wide[p.waves == 8], dim3((unsigned)p.nb), dim3(64 * p.waves), a, stream)) return rc;
+    DecWideArgs f = {};
+    f.q = a.q;
+    f.k = a.k;
+    f.v = a.v;
+    f.kc = a.kc;
+    f.vc = a.vc;
+    f.length = a.length;
+    f.tree = a.tree;
+    f.part_o = a.part_o;
+    f.part_ml = a.part_ml;
+    f.seg = a.seg;
+    f.qb = st[0][0], f.qh = st[0][1], f.qn = st[0][2];
+    f.kb = st[1][0], f.kh = st[1][1], f.kn = (u32)st[1][2];
+    f.vb = st[2][0], f.vh = st[2][1], f.vn = (u32)st[2][2];
+    f.kcb = st[3][0], f.kch = st[3][1], f.kcn = (u32)st[3][2];
+    f.vcb = st[4][0], f.vch = st[4][1], f.vcn = (u32)st[4][2];
+    f.tree_stride = tree_batch_stride;
+    f.T = a.T;
+    f.C = a.C;
+    f.D = a.D;
+    f.G = a.G;
+    f.Hkv = a.Hkv;
+    f.BH = a.BH;
+    f.R = a.R;
+    f.RB = a.RB;
+    f.RW = a.RW;
+    f.nb = a.nb;
+    f.qand = a.qand;
+    f.qxor = a.qxor;
+    f.scale_log2 = a.scale_log2;
+    if (int rc = dec_launch(who, kn.wide[p.waves == 8], dim3((unsigned)p.nb), dim3(64 * p.waves), f, stream)) return rc;
   } else {
     if (int rc = dec_launch(who, kn.rows[vec], dim3((unsigned)p.nb), dim3(256), a, stream)) return rc;
   }
