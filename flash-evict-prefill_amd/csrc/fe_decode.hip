@@ -12,20 +12,22 @@
 // Counting recency back from the newest token, a prompt's importance continued chunk by chunk is the
 // importance of the whole (fe_prefill's).
 //
-//   decode_few_kernel      up to 16 query rows r = g * T + t of a group, the steps of one token: each wave takes 32 keys at
-//                          a time for all of them; the code of a call is short, as most of a small call is its reading
-//   decode_rows_kernel     up to 32 query rows r = g * T + t of a group: each wave takes 32 keys at a time for all of
-//                          them, S^T = K Q^T and O^T = V^T P^T on MFMA, with the rows' running maximum and sum
+//   decode_few_kernel      up to 32 query rows r = g * T + t of a group, the steps of one or a few tokens: each wave takes
+//                          32 keys at a time for all of them, S^T = K Q^T and O^T = V^T P^T on MFMA, with the rows' running
+//                          maximum and sum
 //   decode_wide_kernel     more rows: each wave holds 32 of them, the block's waves share tiles of 64 keys in LDS
+//   decode_elements_kernel any layout of rows that 16-byte loads cannot read
 //   decode_join_kernel     joins the splits of the keys: out and lse; and, where the first kernel left its logits
 //                          (few rows), the importance, whose probabilities need the joined lse
 //   decode_replay_kernel   the importance otherwise: S = Q K^T for the rows that stay, lanes holding keys, so that a
 //                          key's sum over the rows is in-lane: p = exp2(x log2e - bias), the bias holding lse and w
 //                          (decode_replay_elements_kernel for rows that do not allow 16-byte loads)
 //
-// Lengths are known on the device only, and differ from head to head, so a launch has as many blocks as the card
-// holds at once, and each takes an equal share of all tiles of all heads, in order (dec_share); the few-rows kernel's
-// blocks divide each head's tiles instead, which takes less code.
+// Lengths are known on the device only: a launch's grid comes from the cache's size, and a head's blocks divide the
+// tiles that its length has. Short calls are bound by the reading of code and arguments and by trips to memory one after
+// the other, so the kernels read their arguments at once (dec_hold), have the loads of a tile in the code once, read
+// rows past the end as the last, and divide little: the first version of this file, which did none of that, took 15.4 +
+// 11.0 us for a step over 1024 rows of 8 heads, against 6.4 + 4.6 us.
 #include <math.h>
 #include <stddef.h>
 #include <algorithm>
@@ -33,7 +35,6 @@
 
 #include "fe_attn.h"
 #include "fe_internal.h"
-#include "fe_radix.h"
 #include "../../include/flash_evict.h"
 
 namespace fe {
@@ -48,7 +49,6 @@ constexpr int kDecMaxTokens = 256;   // new tokens of a call
 // read, against the 2 D of reading K again.
 constexpr int kDecLogitRows = 16;
 constexpr int kDecJoinBlocks = 1024;   // blocks that share the importance of all heads
-
 // Pointers to global memory, said to be: a pointer that the compiler loses sight of (dec_hold) would be read with flat
 // instructions, which wait for LDS too.
 #define FE_GLOBAL __attribute__((address_space(1)))
@@ -56,76 +56,25 @@ typedef const FE_GLOBAL u16* DecIn;
 typedef FE_GLOBAL float* DecF32;
 typedef const FE_GLOBAL float* DecF32In;
 typedef const FE_GLOBAL int* DecI32In;
-typedef FE_GLOBAL u32x4* DecVec;
 
-// In the order of their use, so that what a kernel needs at once lies together (dec_hold).
+// Attention. Slots are ((b * Hkv + j) * RB + row block) * S + split.
 struct DecArgs {
-  // replay
-  DecF32In imp;            // [B * Hkv] rows of imp_stride
-  DecF32In norm;
-  DecF32 imp_out;
-  DecF32 new_imp;          // [B * Hkv, A]
-  DecF32In lse_in;
-  DecI32In path;           // [B, A] nodes of the accepted path, or null: all T
-  long long imp_stride, norm_stride, impo_stride;
-  int A;
-  float decay_log2;
-  // all
-  DecIn q, k, v, kc;       // queries, new rows, the cache's K
+  DecIn q, k, v, kc, vc;   // queries, new rows, the cache
   DecI32In length;         // [B * Hkv]
-  long long qs[3], ks[3], vs[3], kcs[3];   // strides of batch, head, row
-  int T, C, D, G, Hkv, BH;
-  int nb;                  // blocks that share the tiles
+  const FE_GLOBAL unsigned char* tree;   // [T, T] or [B, T, T], or null: causal
+  DecF32 part_o;           // [slot][RS][DP]: normalised partial outputs
+  DecF32 part_ml;          // [slot][2][RS]: maximum (log2 units), sum
+  DecF32 logits;           // [B * Hkv][tile of 32 keys][R][32] in log2 units, or null
+  long long qb, qh, qn, kb, kh, vb, vh, kcb, kch, vcb, vch, tree_stride;   // strides of batch, head, (q) row
+  u32 kn, vn, kcn, vcn;    // row strides
+  int T, C, D, R, RB, RS, S, max_tiles;   // R rows of a group in RB blocks of RS; splits; tiles of a full cache
   u32 qand, qxor;          // Q's sign for a negative scale, Q's zeros for a zero one
   float scale_log2;
-  // attention
-  DecIn vc;
-  const FE_GLOBAL unsigned char* tree;   // [T, T] or [B, T, T], or null: causal
-  DecF32 part_o;           // [slot][32 * RW][DP]: normalised partial outputs
-  DecF32 part_ml;          // [slot][2][32 * RW]: maximum (log2 units), sum
-  FE_GLOBAL int* seg;      // [segment][2]: first and last slot
-  DecF32 logits;           // [B * Hkv][tile][R][32] in log2 units, or null
-  long long vcs[3], tree_stride;
-  int R, RB, RW;           // rows of a group; segments of a group, 32-row tiles of a segment
-  int max_tiles;           // tiles of 32 keys of a full cache and T new rows
-  // element loads
-  long long qc, kcc, vcc, knc, vnc;      // channel strides of q, the cache and the new rows
-  int pad[4];
-};
-constexpr int kDecReplayArgs = 0, kDecAttnArgs = 80;   // offsets of what the kernels hold
-static_assert(offsetof(DecArgs, q) == kDecAttnArgs && offsetof(DecArgs, qc) <= kDecAttnArgs + 5 * 64 && offsetof(DecArgs, vc) <= 5 * 64 &&
-                  sizeof(DecArgs) >= kDecAttnArgs + 5 * 64, "argument windows");
-
-struct DecFewArgs {
-  DecIn q, k, v, kc, vc;
-  DecI32In length;
-  const FE_GLOBAL unsigned char* tree;
-  DecF32 part_o;           // [B * Hkv * S][16][DP]
-  DecF32 part_ml;          // [B * Hkv * S][2][16]
-  DecF32 logits;           // or null
-  long long qb, qh, qn, kb, kh, vb, vh, kcb, kch, vcb, vch, tree_stride;   // strides of batch, head, (q) row
-  u32 kn, vn, kcn, vcn;    // row strides
-  int T, C, D, R, S, max_tiles;
-  u32 qand, qxor;
-  float scale_log2;
-  int pad[9];
-};
-static_assert(offsetof(DecFewArgs, pad) <= 4 * 64 && sizeof(DecFewArgs) >= 4 * 64, "argument window");
-
-struct DecWideArgs {
-  DecIn q, k, v, kc, vc;
-  DecI32In length;
-  const FE_GLOBAL unsigned char* tree;
-  DecF32 part_o, part_ml;
-  FE_GLOBAL int* seg;
-  long long qb, qh, qn, kb, kh, vb, vh, kcb, kch, vcb, vch, tree_stride;   // strides of batch, head, (q) row
-  u32 kn, vn, kcn, vcn;    // row strides
-  int T, C, D, G, Hkv, BH, R, RB, RW, nb;
-  u32 qand, qxor;
-  float scale_log2;
   int pad[3];
+  // element loads: 64-bit row strides, channel strides
+  long long kn64, vn64, kcn64, vcn64, qc, kd, vd, kcd, vcd;
 };
-static_assert(offsetof(DecWideArgs, pad) <= 4 * 64 && sizeof(DecWideArgs) >= 4 * 64, "argument window");
+static_assert(offsetof(DecArgs, pad) <= 4 * 64 && sizeof(DecArgs) >= 4 * 64, "argument window");
 
 struct DecReplayArgs {
   DecIn q, k, v, kc;
@@ -139,10 +88,12 @@ struct DecReplayArgs {
   u32 qand, qxor;
   float scale_log2, decay_log2;
   int pad[6];
+  // element loads: 64-bit row strides, channel strides
+  long long kn64, vn64, kcn64, qc, kd, vd, kcd;
 };
 static_assert(offsetof(DecReplayArgs, pad) <= 4 * 64 && sizeof(DecReplayArgs) >= 4 * 64, "argument window");
 
-struct DecFewJoinArgs {
+struct DecJoinArgs {
   DecF32In part_o, part_ml, logits;
   DecI32In length;
   FE_GLOBAL u16* out;      // [B, Hq, T, D]
@@ -150,26 +101,11 @@ struct DecFewJoinArgs {
   DecF32In imp, norm;
   DecF32 imp_out, new_imp;
   DecIn v;
-  long long imp_stride, norm_stride, impo_stride, vb, vh;
-  u32 vn;
-  int T, C, D, R, S, max_tiles;
-  float decay_log2;
-  int pad[8];
-};
-static_assert(offsetof(DecFewJoinArgs, pad) <= 3 * 64 && sizeof(DecFewJoinArgs) >= 3 * 64, "argument window");
-
-struct DecJoinArgs {
-  DecF32In part_o, part_ml, logits;
-  DecI32In seg, length;
-  FE_GLOBAL u16* out;      // [B, Hq, T, D]
-  DecF32 lse;              // [B, Hq, T]
-  DecF32In imp, norm;
-  DecF32 imp_out, new_imp;
-  DecIn v;
-  long long imp_stride, norm_stride, impo_stride, vs[3], vnc;
-  int T, C, D, G, Hkv, BH, R, RB, RS, max_tiles;   // RS: rows of a slot
-  int out_blocks, split;   // blocks of the output; 32-lane groups that share a row
-  int per_head;            // blocks of a head's importance
+  long long imp_stride, norm_stride, impo_stride, vb, vh, vn, vd;
+  int T, C, D, R, RB, RS, S, max_tiles;
+  int wide;                // tiles of 64 keys
+  int rows;                // output rows of a block: 1, all its threads on it, or a group of threads on each
+  int out_blocks;          // of a head
   float decay_log2;
   int pad[16];
 };
@@ -177,7 +113,7 @@ static_assert(offsetof(DecJoinArgs, pad) <= 4 * 64 && sizeof(DecJoinArgs) >= 4 *
 
 // The kernel's arguments, NV * 64 bytes of them from byte FIRST on read at once and kept in registers. Left to the
 // compiler, each is read where it is first used and again wherever that saves registers; arguments lie in host memory,
-// and a wave waited some 2000 cycles for every such read (step of one token over 1024 rows: 15.4 us of which 10 so).
+// and a wave waited some 2000 cycles for every such read .
 template <int FIRST, int NV, typename A>
 __device__ __forceinline__ A dec_hold(const A& arg) {
   static_assert(sizeof(A) >= FIRST + NV * 64, "argument window");
@@ -188,8 +124,6 @@ __device__ __forceinline__ A dec_hold(const A& arg) {
   u32x16 v[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) v[i] = p[i];
-  if constexpr (NV == 5) asm volatile("" : "+s"(v[0]), "+s"(v[1]), "+s"(v[2]), "+s"(v[3]), "+s"(v[4]));
-  if constexpr (NV == 3) asm volatile("" : "+s"(v[0]), "+s"(v[1]), "+s"(v[2]));
   if constexpr (NV == 4) asm volatile("" : "+s"(v[0]), "+s"(v[1]), "+s"(v[2]), "+s"(v[3]));
   // from here on word by word: a spilled register of 16 words would come back whole for each word of it
   u32 w[NV * 16];
@@ -204,10 +138,6 @@ __device__ __forceinline__ A dec_hold(const A& arg) {
 
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kDecNegInf = -__builtin_huge_valf();
-
-// Rows of the (b, j) cache, within the tensor whatever the caller's length says.
-template <typename A>
-__device__ __forceinline__ int dec_len(const A& a, int bh) { return min(max(a.length[bh], 0), a.C); }
 
 // Orders a wave's own LDS writes and reads (the hardware keeps them in order; the compiler is told).
 __device__ __forceinline__ void dec_wave_order() {
@@ -279,191 +209,19 @@ __device__ __forceinline__ bool dec_nonfinite<BF16>(u32x4 x) { return dec_expone
 template <>
 __device__ __forceinline__ bool dec_nonfinite<F16>(u32x4 x) { return dec_exponent_full<0x7c00u>(x); }
 
-// The tiles of KT keys of a head: its cache's, then those of `fresh` new rows.
+// Tiles of KT keys of a head: its cache's, then those of `fresh` new rows.
 template <int KT>
 __device__ __forceinline__ int dec_tiles(int n, int fresh) { return (n + KT - 1) / KT + (fresh + KT - 1) / KT; }
+// A split's tiles: whole rounds of PER.
+template <int PER>
+__device__ __forceinline__ int dec_split(int tiles, int S) { return ((tiles + PER * S - 1) / (PER * S)) * PER; }
 
-// Block blockIdx.x's share [pos, hi) of the tiles of all segments, numbered head by head and, within a head, segment
-// by segment of all its tiles; the head that holds pos and the head's first tile. Only as many blocks share as there
-// are PER tiles for each, so no block between two others is without a tile. Every wave computes it. (The launch
-// keeps the number of tiles below 2^31.)
-struct DecShare {
-  int pos, hi, base, bh;
-  int len;                 // lane i: rows of head (bh & ~63) + i
-};
-template <int KT, int PER, typename A>
-__device__ __forceinline__ DecShare dec_share(const A& a, int segs, int fresh) {
-  const int lane = threadIdx.x & 63;
-  auto tiles = [&](int len, int bh) { return bh < a.BH ? segs * dec_tiles<KT>(len, fresh) : 0; };
-  auto length = [&](int bh) { return bh < a.BH ? dec_len(a, bh) : 0; };
-  DecShare s;
-  const int len0 = length(lane), scan0 = wave_inclusive_scan(tiles(len0, lane));
-  u32 W = (u32)__builtin_amdgcn_readlane(scan0, 63);
-  for (int c0 = 64; c0 < a.BH; c0 += 64) W += (u32)__builtin_amdgcn_readlane(wave_inclusive_scan(tiles(length(c0 + lane), c0 + lane)), 63);
-  const u32 nb = min((u32)a.nb, (W + PER - 1) / PER), q = W / nb, rest = W - q * nb, i = blockIdx.x;
-  s.pos = s.hi = 0;
-  if (i < nb) {
-    s.pos = (int)(q * i + min(i, rest));
-    s.hi = s.pos + (int)(q + (i < rest ? 1u : 0u));
-  }
-  s.base = 0;
-  s.bh = 0;
-  s.len = len0;
-  int x = scan0;
-  for (int c0 = 0;;) {
-    const unsigned long long past = __ballot(s.base + x > s.pos);
-    if (past) {
-      const int at = __ffsll(past) - 1;
-      s.bh = c0 + at;
-      if (at) s.base += __builtin_amdgcn_readlane(x, at - 1);
-      break;
-    }
-    s.base += __builtin_amdgcn_readlane(x, 63);
-    c0 += 64;
-    if (c0 >= a.BH) break;
-    s.len = length(c0 + lane);
-    x = wave_inclusive_scan(tiles(s.len, c0 + lane));
-  }
-  return s;
-}
-// Rows of the share's current head.
-__device__ __forceinline__ int dec_share_len(const DecShare& s) { return __builtin_amdgcn_readlane(s.len, s.bh & 63); }
-// On to the next head.
-template <typename A>
-__device__ __forceinline__ void dec_share_next(const A& a, DecShare& s) {
-  s.base = s.pos;
-  ++s.bh;
-  if ((s.bh & 63) == 0) {
-    const int bh = s.bh + (int)(threadIdx.x & 63);
-    s.len = bh < a.BH ? dec_len(a, bh) : 0;
-  }
-}
-
-// Which of a lane's 16 keys of 32 from kb (bit i: key kb + 8 (i / 4) + 4 hh + i % 4) query token tq sees, among the
-// cache's rows (fresh false) or the new ones.
-template <typename A>
-__device__ __forceinline__ u32 dec_visible(const A& a, int b, int tq, int kb, int rows, bool fresh) {
-  const int k0 = kb + 4 * (int)((threadIdx.x >> 5) & 1);
-  const FE_GLOBAL unsigned char* row = a.tree + b * a.tree_stride + tq * a.T;
-  u32 bits = 0;
-#pragma unroll 1
-  for (int i = 0; i < 16; i += 4) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int key = k0 + 2 * i + j;
-      bool see = key < rows;
-      if (fresh) see = see && (a.tree ? row[see ? key : 0] != 0 : key <= tq);
-      bits |= (see ? 1u : 0u) << (i + j);
-    }
-  }
-  return bits;
-}
-
-// The rows of a head: its cache's and its new ones'.
-struct DecRows {
-  DecIn kc, vc, k, v;
-  long long kcs, vcs, ks, vs;   // row strides
-};
-__device__ __forceinline__ DecRows dec_rows(const DecArgs& a, int b, int hkv) {
-  return {a.kc + b * a.kcs[0] + hkv * a.kcs[1], a.vc + b * a.vcs[0] + hkv * a.vcs[1], a.k + b * a.ks[0] + hkv * a.ks[1],
-          a.v + b * a.vs[0] + hkv * a.vs[1], a.kcs[2], a.vcs[2], a.ks[2], a.vs[2]};
-}
-
-// Where a tile of KT keys lies: tile t of nc of the cache, then of the new rows.
-struct DecTile {
-  DecIn k, v;
-  long long krs, vrs;
-  int kb, rows;
-  bool tail;
-};
-template <int KT>
-__device__ __forceinline__ DecTile dec_tile(const DecRows& r, int n, int nc, int fresh, int t) {
-  DecTile x;
-  x.tail = t >= nc;
-  x.kb = (x.tail ? t - nc : t) * KT;
-  x.rows = x.tail ? fresh : n;
-  x.krs = x.tail ? r.ks : r.kcs;
-  x.vrs = x.tail ? r.vs : r.vcs;
-  x.k = x.tail ? r.k : r.kc;
-  x.v = x.tail ? r.v : r.vc;
-  return x;
-}
-
-// NT threads' 16-byte chunks of KT rows of D channels: thread tid's chunk i is e = i * NT + tid in row order. Loads
-// go out together, without a branch or a wait between them: a chunk past channel D is not loaded and keeps its zeros
-// (x starts as zeros), rows past the last are read as the last.
-template <int DP, int KT, int NT, int NL>
-__device__ __forceinline__ void dec_load_rows(DecIn p, long long rs, int kb, int rows, int D, int tid, u32x4 (&x)[NL]) {
-  constexpr int CPR = DP / 8;
-  if constexpr (NT % CPR == 0) {
-    const int key = tid / CPR, ch = 8 * (tid % CPR);
-    if (ch < D) {
-      if (kb + KT <= rows) {
-        DecIn lp = p + (long long)(kb + key) * rs + ch;
-        const long long step = (long long)(NT / CPR) * rs;
-#pragma unroll
-        for (int i = 0; i < NL; ++i) {
-          x[i] = *(const FE_GLOBAL u32x4*)lp;
-          lp += step;
-          asm volatile("" : "+v"(lp));   // one address at a time, no table of multiples of the stride
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < NL; ++i) x[i] = *(const FE_GLOBAL u32x4*)(p + (long long)min(kb + key + i * (NT / CPR), rows - 1) * rs + ch);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int e = i * NT + tid, key = e / CPR, ch = 8 * (e % CPR);
-      if (ch < D) x[i] = *(const FE_GLOBAL u32x4*)(p + (long long)min(kb + key, rows - 1) * rs + ch);
-    }
-  }
-}
 // Zeros in place of the rows past the last (V: 0 * inf is not 0).
 template <int DP, int NT, int NL>
 __device__ __forceinline__ void dec_cut_rows(int kb, int rows, int tid, u32x4 (&x)[NL]) {
 #pragma unroll
   for (int i = 0; i < NL; ++i)
     if (kb + (i * NT + tid) / (DP / 8) >= rows) x[i] = (u32x4){0u, 0u, 0u, 0u};
-}
-
-// A lane's fragments of its query row: read, then (once the tile behind them is on its way too) with the scale's sign
-// and zeros past D and for a row that is none.
-template <int DP, int VEC>
-__device__ __forceinline__ void dec_read_q(const DecArgs& a, int b, int head, int tq, u32x4 (&qf)[DP / 16]) {
-  const int hh = (threadIdx.x >> 5) & 1;
-  const DecIn qp = a.q + b * a.qs[0] + head * a.qs[1] + tq * a.qs[2];   // a real row in any case
-#pragma unroll
-  for (int c = 0; c < DP / 16; ++c) {
-    if constexpr (VEC) {
-      qf[c] = *(const FE_GLOBAL u32x4*)(qp + (16 * c + 8 * hh < a.D ? 16 * c + 8 * hh : 0));
-    } else {
-      qf[c] = dec_load8(qp, a.qc, 2 * c + hh, a.D);
-      __builtin_amdgcn_sched_barrier(0);   // element loads: one chunk's addresses at a time
-    }
-  }
-}
-template <int DP>
-__device__ __forceinline__ void dec_set_q(const DecArgs& a, bool valid, u32x4 (&qf)[DP / 16]) {
-  const int hh = (threadIdx.x >> 5) & 1;
-#pragma unroll
-  for (int c = 0; c < DP / 16; ++c) {
-    const u32 keep = valid && 16 * c + 8 * hh < a.D ? a.qand : 0u, flip = keep ? a.qxor : 0u;
-    qf[c] = (qf[c] & keep) ^ flip;
-  }
-}
-
-// The segment's place in the tables, and its first and last slot, by the blocks that hold its ends. A block's
-// segments follow each other, so block + segment numbers every (block, segment) pair apart.
-template <typename A>
-__device__ __forceinline__ int dec_slot(const A& a, int seg, bool head, bool end) {
-  const int slot = (int)blockIdx.x + seg;
-  if (threadIdx.x == 0) {
-    if (head) a.seg[2 * seg] = slot;
-    if (end) a.seg[2 * seg + 1] = slot;
-  }
-  return slot;
 }
 
 template <typename E>
@@ -487,54 +245,66 @@ __device__ __forceinline__ float dec_quad_sum(float x) {
   return half_swap_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
-// Tiles of a block of the few-rows kernel: whole rounds of its four waves.
-__device__ __forceinline__ int dec_few_share(int tiles, int S) { return ((tiles + 4 * S - 1) / (4 * S)) * 4; }
-
-// Block (split, KV head, batch row). S^T = K Q^T and O^T = V^T P^T with 16 queries in the lanes' low four bits: 32 keys
-// are two accumulators of S^T, whose registers (keys 4 (lane / 16) + i of each) are P^T's operand as they are; V^T's comes
-// from transposing reads in that key order.
+// Block (split, KV head, batch row), QT tiles of 16 rows. S^T = K Q^T and O^T = V^T P^T with 16 queries in the lanes' low
+// four bits: 32 keys are two accumulators of S^T, whose registers (keys 4 (lane / 16) + i of each) are P^T's operand as
+// they are; V^T's comes from transposing reads in that key order.
 // What bounds it: HBM where the cache is long (the next 32 keys' K and V are on their way to registers while a wave
 // works on these); where it is short, the reading of its own code and the one round trip to memory, so the loads of
 // a tile appear in the code once, rows past the end are read as the last, and nothing is divided that need not be.
-template <typename E, int DP>
-__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_few_kernel(const DecFewArgs args) {
-  constexpr int NC = DP / 32, NT16 = DP / 16, CPR = DP / 8, NL = DP / 16, TILE = 64 * DP, OST = DP + 4;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[4][2 * TILE];
-  __shared__ float sm[3][4][16];
-  static_assert(2 * TILE >= 16 * OST * 4 && 2 * TILE >= (32 * 16 + DP) * 4, "output, or probabilities and a value, in a wave's tiles");
-  const DecFewArgs a = dec_hold<0, 4>(args);
+template <typename E, int DP, int QT>
+__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_few_kernel(const DecArgs args) {
+  constexpr int NC = DP / 32, NT16 = DP / 16, CPR = DP / 8, NL = DP / 16, TILE = 64 * DP, OST = DP + 4, RS = 16 * QT;
+  constexpr int WLDS = QT == 1 ? 2 * TILE : 32 * OST * 4;   // a wave's LDS: a K and a V tile, then its output
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[4][WLDS];
+  __shared__ float sm[3][4][RS];
+  static_assert(WLDS >= 2 * TILE && WLDS >= RS * OST * 4 && WLDS >= (32 * RS + DP) * 4, "output, or probabilities and a value, in a wave's tiles");
+  const DecArgs a = dec_hold<0, 4>(args);
   const int lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hkv = (int)blockIdx.y, b = (int)blockIdx.z, bh = b * (int)gridDim.y + hkv;
   int n = a.length[bh];
-  // this lane's query row (row 0 where there is none: its results go nowhere)
-  const int r = l16 < a.R ? l16 : 0;
-  const int g = a.T == 1 ? r : r / a.T, tq = r - g * a.T;
-  const DecIn qp = a.q + b * a.qb + (long long)(hkv * (a.R / a.T) + g) * a.qh + tq * a.qn;
-  u32x4 qf[NC];
+  // this lane's query rows (row 0 where there is none: its results go nowhere)
+  int tq[QT];
+  u32x4 qf[QT][NC];
 #pragma unroll
-  for (int c = 0; c < NC; ++c) qf[c] = *(const FE_GLOBAL u32x4*)(qp + (DP == a.D || 32 * c + 8 * lq < a.D ? 32 * c + 8 * lq : 0));
+  for (int q = 0; q < QT; ++q) {
+    const int r = 16 * q + l16 < a.R ? 16 * q + l16 : 0, g = a.T == 1 ? r : r / a.T;
+    tq[q] = r - g * a.T;
+    const DecIn qp = a.q + b * a.qb + (long long)(hkv * (a.R / a.T) + g) * a.qh + tq[q] * a.qn;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) qf[q][c] = *(const FE_GLOBAL u32x4*)(qp + (DP == a.D || 32 * c + 8 * lq < a.D ? 32 * c + 8 * lq : 0));
+  }
+  if (a.D != DP) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int q = 0; q < QT; ++q) qf[q][c] &= 32 * c + 8 * lq < a.D ? ~0u : 0u;
+  }
   const DecIn kc = a.kc + b * a.kcb + hkv * a.kch, vc = a.vc + b * a.vcb + hkv * a.vch;
   const DecIn kn = a.k + b * a.kb + hkv * a.kh, vn = a.v + b * a.vb + hkv * a.vh;
   n = __builtin_amdgcn_readfirstlane(min(max(n, 0), a.C));
-  const int nc = (n + 31) / 32, tiles = nc + (a.T + 31) / 32, share = dec_few_share(tiles, a.S);
+  const int nc = (n + 31) / 32, tiles = nc + (a.T + 31) / 32, share = dec_split<4>(tiles, a.S);
   const int t0 = (int)blockIdx.x * share, t1 = min(tiles, t0 + share);
   if (t0 >= t1) return;
 
   unsigned char* kt = lds[wv];
   unsigned char* vt = lds[wv] + TILE;
-  f32x4 o[NT16];
+  f32x4 o[QT][NT16];
+  float m[QT], l[QT], lr[QT];              // l, lr: of the lane's keys
 #pragma unroll
-  for (int i = 0; i < NT16; ++i) o[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  float m = kDecNegInf, l = 0.f, lr = 0.f;   // l, lr: of the lane's keys
+  for (int q = 0; q < QT; ++q) {
+    m[q] = kDecNegInf;
+    l[q] = lr[q] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NT16; ++i) o[q][i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  }
   u32x4 kx[NL] = {}, vx[NL] = {};
   int t = -1, next = t0 + wv;
-  bool set = false;
 #pragma unroll 1
   while (true) {
     const bool tail = t >= nc;
     const int kb = (tail ? t - nc : t) * 32, rows = tail ? a.T : n;
-    u32 odd = 0;                           // keys of new rows with a value that is not finite (as in decode_rows_kernel)
+    u32 odd = 0;                           // keys of new rows whose value has an infinity or a NaN
     if (t >= 0) {
       if (kb + 32 > rows) dec_cut_rows<DP, 64>(kb, rows, lane, vx);
       if (a.D != DP) {
@@ -573,101 +343,106 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_few_kernel(const
         }
       }
     }
-    if (!set) {
-      set = true;
-      if (a.qand != ~0u || a.qxor != 0u || a.D != DP) {
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          const u32 keep = 32 * c + 8 * lq < a.D ? a.qand : 0u, flip = keep ? a.qxor : 0u;
-          qf[c] = (qf[c] & keep) ^ flip;
-        }
-      }
-    }
     if (t >= 0) {
+      // 0 * inf would reach the rows that do not see such a key, so its value is taken out of the product, and
+      // added to the rows that do
       if (odd) {
         dec_wave_order();
         for (int e = lane; e < 32 * CPR; e += 64)
           if ((odd >> (e / CPR)) & 1u) *(u32x4*)(vt + dec_v_at<DP>(e / CPR, e % CPR)) = (u32x4){0u, 0u, 0u, 0u};
       }
       dec_wave_order();
-      f32x4 x[2];
+      f32x4 x[QT][2];
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
+          if (QT > 1 && c % 4 == 0) __builtin_amdgcn_sched_barrier(0);   // four fragments in flight
           const u32x4 kf = *(const u32x4*)(kt + dec_k_at<DP>(16 * s + l16, 4 * c + lq));
-          x[s] = dec_mfma16<E>(kf, qf[c], c == 0 ? (f32x4){0.f, 0.f, 0.f, 0.f} : x[s]);
+#pragma unroll
+          for (int q = 0; q < QT; ++q) x[q][s] = dec_mfma16<E>(kf, qf[q][c], c == 0 ? (f32x4){0.f, 0.f, 0.f, 0.f} : x[q][s]);
         }
-      u32 vis = 0xffu;                      // bit 4 s + i: register i of x[s], key kb + 16 s + 4 lq + i, is visible
-      if (tail || kb + 32 > rows) {
-        const FE_GLOBAL unsigned char* row = a.tree + b * a.tree_stride + tq * a.T;
-        vis = 0;
+      u32x4 pf[QT];
+      u32 vis[QT];                          // bit 4 s + i: register i of x[s], key kb + 16 s + 4 lq + i, is visible
+#pragma unroll
+      for (int q = 0; q < QT; ++q) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[q][i >> 2][i & 3] *= a.scale_log2;
+        vis[q] = 0xffu;
+        if (tail || kb + 32 > rows) {
+          const FE_GLOBAL unsigned char* row = a.tree + b * a.tree_stride + tq[q] * a.T;
+          vis[q] = 0;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int key = kb + 16 * (i >> 2) + 4 * lq + (i & 3);
+            bool see = key < rows;
+            if (tail) see = see && (a.tree ? row[see ? key : 0] != 0 : key <= tq[q]);
+            vis[q] |= (see ? 1u : 0u) << i;
+            x[q][i >> 2][i & 3] = see ? x[q][i >> 2][i & 3] : kDecNegInf;
+          }
+        }
+        float mn = kDecNegInf;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mn = fmaxf(mn, x[q][i >> 2][i & 3]);
+        if (QT == 1 && a.logits && l16 < a.R) {
+          const DecF32 lp = a.logits + (((long long)bh * a.max_tiles + t) * a.R + l16) * 32 + 4 * lq;
+          *(FE_GLOBAL f32x4*)lp = x[q][0];
+          *(FE_GLOBAL f32x4*)(lp + 16) = x[q][1];
+        }
+        mn = fmaxf(m[q], dec_quad_max(mn));
+        const float ref = mn == kDecNegInf ? 0.f : mn;
+        const float alpha = fast_exp2(m[q] - ref);
+        m[q] = mn;
+        float ls = 0.f, lrs = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int key = kb + 16 * (i >> 2) + 4 * lq + (i & 3);
-          bool see = key < rows;
-          if (tail) see = see && (a.tree ? row[see ? key : 0] != 0 : key <= tq);
-          vis |= (see ? 1u : 0u) << i;
-          x[i >> 2][i & 3] = see ? x[i >> 2][i & 3] : kDecNegInf;
+          x[q][i >> 2][i & 3] = fast_exp2(x[q][i >> 2][i & 3] - ref);
+          ls += x[q][i >> 2][i & 3];
         }
-      }
-      float mn = kDecNegInf;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[i >> 2][i & 3] *= a.scale_log2;
-        mn = fmaxf(mn, x[i >> 2][i & 3]);
-      }
-      if (a.logits && l16 < a.R) {
-        const DecF32 lp = a.logits + (((long long)bh * a.max_tiles + t) * a.R + l16) * 32 + 4 * lq;
-        *(FE_GLOBAL f32x4*)lp = x[0];
-        *(FE_GLOBAL f32x4*)(lp + 16) = x[1];
-      }
-      mn = fmaxf(m, dec_quad_max(mn));
-      const float ref = mn == kDecNegInf ? 0.f : mn;
-      const float alpha = fast_exp2(m - ref);
-      m = mn;
-      float ls = 0.f, lrs = 0.f;
-      u32x4 pf;
+        for (int i = 0; i < 4; ++i) {
+          pf[q][i] = E::pack2(x[q][i >> 1][2 * (i & 1)], x[q][i >> 1][2 * (i & 1) + 1]);
+          lrs += E::to_f32((u16)pf[q][i]) + E::to_f32((u16)(pf[q][i] >> 16));
+        }
+        l[q] = l[q] * alpha + ls;
+        lr[q] = lr[q] * alpha + lrs;
+        if (__ballot(alpha != 1.f)) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x[i >> 2][i & 3] = fast_exp2(x[i >> 2][i & 3] - ref);
-        ls += x[i >> 2][i & 3];
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        pf[i] = E::pack2(x[i >> 1][2 * (i & 1)], x[i >> 1][2 * (i & 1) + 1]);
-        lrs += E::to_f32((u16)pf[i]) + E::to_f32((u16)(pf[i] >> 16));
-      }
-      l = l * alpha + ls;
-      lr = lr * alpha + lrs;
-      if (__ballot(alpha != 1.f)) {
-#pragma unroll
-        for (int i = 0; i < NT16; ++i) o[i] *= alpha;
+          for (int i = 0; i < NT16; ++i) o[q][i] *= alpha;
+        }
       }
 #pragma unroll
       for (int i = 0; i < NT16; ++i) {
+        if (QT > 1 && i % 4 == 0) __builtin_amdgcn_sched_barrier(0);
         // channels 16 i + l16: keys 4 lq .. + 3, then 16 + 4 lq .. + 3
         const int row = 4 * lq + (l16 >> 2);
         unsigned char* p = vt + row * (DP * 2) + ((i >> 1) ^ dec_vswz<DP>(row)) * 64 + 32 * (i & 1) + 8 * (l16 & 3);
         const u32x2 ux = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((dec_lds_s16x4*)(dec_lds_ptr)p));
         const u32x2 uy = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((dec_lds_s16x4*)(dec_lds_ptr)(p + 16 * DP * 2)));
-        o[i] = dec_mfma16<E>((u32x4){ux[0], ux[1], uy[0], uy[1]}, pf, o[i]);
+#pragma unroll
+        for (int q = 0; q < QT; ++q) o[q][i] = dec_mfma16<E>((u32x4){ux[0], ux[1], uy[0], uy[1]}, pf[q], o[q][i]);
       }
       if (odd) {
         dec_wave_order();
-        float* sp = (float*)kt;             // [32 keys][16 rows] probabilities (-1: hidden)
-        float* val = sp + 32 * 16;          // a value's channels
+        float* sp = (float*)kt;             // [32 keys][RS rows] probabilities (-1: hidden)
+        float* val = sp + 32 * RS;          // a value's channels
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sp[(16 * (i >> 2) + 4 * lq + (i & 3)) * 16 + l16] = (vis >> i) & 1u ? x[i >> 2][i & 3] : -1.f;
+        for (int q = 0; q < QT; ++q)
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            sp[(16 * (i >> 2) + 4 * lq + (i & 3)) * RS + 16 * q + l16] = (vis[q] >> i) & 1u ? x[q][i >> 2][i & 3] : -1.f;
         for (u32 left = odd; left; left &= left - 1) {
           const int key = __ffs((int)left) - 1;
           for (int ch = lane; ch < DP; ch += 64) val[ch] = ch < a.D ? E::to_f32(vn[(unsigned long long)(kb + key) * a.vn + ch]) : 0.f;
           dec_wave_order();
-          const float p = sp[key * 16 + l16];
 #pragma unroll
-          for (int i = 0; i < NT16; ++i) {
-            const f32x4 y = *(const f32x4*)(val + 16 * i + 4 * lq);
-            if (p >= 0.f || p != p) o[i] += p * y;
+          for (int q = 0; q < QT; ++q) {
+            const float p = sp[key * RS + 16 * q + l16];
+#pragma unroll
+            for (int i = 0; i < NT16; ++i) {
+              const f32x4 y = *(const f32x4*)(val + 16 * i + 4 * lq);
+              if (p >= 0.f || p != p) o[q][i] += p * y;
+            }
           }
           dec_wave_order();
         }
@@ -680,16 +455,18 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_few_kernel(const
   }
 
   // join the four waves (waves without a tile have a maximum of -inf and zeros)
-  l = dec_quad_sum(l);
-  lr = dec_quad_sum(lr);
-  if (lq == 0) {
-    sm[0][wv][l16] = m;
-    sm[1][wv][l16] = l;
-    sm[2][wv][l16] = lr;
-  }
   float* mine = (float*)lds[wv];
 #pragma unroll
-  for (int i = 0; i < NT16; ++i) *(f32x4*)(mine + l16 * OST + 16 * i + 4 * lq) = o[i];
+  for (int q = 0; q < QT; ++q) {
+    const float ls = dec_quad_sum(l[q]), lrs = dec_quad_sum(lr[q]);
+    if (lq == 0) {
+      sm[0][wv][16 * q + l16] = m[q];
+      sm[1][wv][16 * q + l16] = ls;
+      sm[2][wv][16 * q + l16] = lrs;
+    }
+#pragma unroll
+    for (int i = 0; i < NT16; ++i) *(f32x4*)(mine + (16 * q + l16) * OST + 16 * i + 4 * lq) = o[q][i];
+  }
   __syncthreads();
   const long long slot = (long long)bh * a.S + blockIdx.x;
 #pragma unroll 1
@@ -708,164 +485,302 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_few_kernel(const
     }
     // partials are normalised by the sum of the rounded probabilities, and weighted by the exact one: so a row
     // that one key dominates returns that key's value whatever the split
-    *(FE_GLOBAL f32x4*)(a.part_o + (slot * 16 + row) * DP + ch) = s * (lrt == 0.f ? 0.f : __builtin_amdgcn_rcpf(lrt));
+    *(FE_GLOBAL f32x4*)(a.part_o + (slot * RS + row) * DP + ch) = s * (lrt == 0.f ? 0.f : __builtin_amdgcn_rcpf(lrt));
     if (ch == 0) {
-      a.part_ml[slot * 32 + row] = mx;
-      a.part_ml[slot * 32 + 16 + row] = lt;
+      a.part_ml[slot * 2 * RS + row] = mx;
+      a.part_ml[slot * 2 * RS + RS + row] = lt;
     }
   }
 }
 
-// Joins the splits of decode_few_kernel. Blocks below R of a head: an output row, DP / 4 threads on each slot's values,
-// each merging its slots as it reads them (maximum, sum, values), and the groups of threads through LDS. The others:
-// the head's importance, a tile of 32 keys to 32 lanes.
-// What bounds it: two round trips to memory and the reading of its code; on long caches the logits' and weights' bytes.
-template <typename E, int DP>
-__global__ __launch_bounds__(256) void decode_few_join_kernel(const DecFewJoinArgs args) {
-  constexpr int LPR = DP / 4, NG = 256 / LPR, PF = 4;   // threads on a slot, groups of them; loads in flight
-  __shared__ float sm[16][16], sl[16][16], bias[16];
-  __shared__ f32x4 so[NG * LPR];
-  const DecFewJoinArgs a = dec_hold<0, 3>(args);
-  const int tid = threadIdx.x, hkv = (int)blockIdx.y, b = (int)blockIdx.z, bh = b * (int)gridDim.y + hkv;
+// Block (split, KV head, row block of a batch row). A wave holds 32 of its rows; the block's waves share tiles of 64 keys,
+// whose loads are on the way to registers during the tile before. A row keeps its reference maximum until a tile's
+// probabilities could overflow (E::kMaxTileSum), as in the prefill kernels, so most tiles spend nothing on maxima and
+// rescaling. The two waves of a SIMD run half a tile apart: one multiplies a tile's probabilities by V right away, the
+// other at the next tile, while the first is at its exponentials.
+// What bounds it: the matrix pipe and the vector work beside it (an exponential a logit); at 256 rows a tile takes
+// about as long as its bytes from HBM.
+template <typename E, int DP, int NW>
+__global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void decode_wide_kernel(const DecArgs args) {
+  constexpr int NDC = DP / 16, NDT = DP / 32, CPR = DP / 8, TILE = 128 * DP;   // bytes of 64 rows
+  constexpr int NT = NW * 64, NL = (64 * CPR + NT - 1) / NT, OST = DP + 4;
+  // eight waves: two on a SIMD. K of two tiles; V of three then: waves that run late read the tile before while the
+  // next one comes in
+  constexpr int VB = NW == 8 ? 3 : 2;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[(2 + VB) * TILE];
+  __shared__ u32 s_odd[2][2];            // keys of a tile of new rows with a value that is not finite
+  __shared__ u32 s_tree[kDecMaxTokens][2];   // what each query token sees of a tile of new rows
+  __shared__ float s_row[NW][DP];        // a value that is not finite, by each wave
+  static_assert((2 + VB) * TILE >= NW * 16 * OST * 4, "16 rows of each wave's output");
+  const DecArgs a = dec_hold<0, 4>(args);
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const bool late = VB == 3 && wv >= 4;
+  u32 ones2;
+  asm volatile("s_mov_b32 %0, %1" : "=s"(ones2) : "i"(E::kOnes2));
+  const int hkv = (int)blockIdx.y, z = (int)blockIdx.z, b = a.RB == 1 ? z : z / a.RB, rb = z - b * a.RB;
+  const int bh = b * (int)gridDim.y + hkv;
   const int n = __builtin_amdgcn_readfirstlane(min(max(a.length[bh], 0), a.C));
-  const int nc = (n + 31) / 32, tiles = nc + (a.T + 31) / 32, share = dec_few_share(tiles, a.S), count = (tiles + share - 1) / share;
-  const long long first = (long long)bh * a.S;
-  if ((int)blockIdx.x < a.R) {
-    const int row = (int)blockIdx.x, grp = tid / LPR, c4 = tid - grp * LPR;
-    const DecF32In ml = a.part_ml + first * 32 + row;
-    const DecF32In po = a.part_o + (first * 16 + row) * DP + 4 * c4;
-    float m = kDecNegInf, l = 0.f;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-    for (int s0 = grp; s0 < count && grp < NG; s0 += PF * NG) {
-      float ms[PF], ls[PF];
-      f32x4 x[PF];
-#pragma unroll
-      for (int i = 0; i < PF; ++i) {
-        const int s = min(s0 + i * NG, count - 1);
-        ms[i] = ml[s * 32];
-        ls[i] = ml[s * 32 + 16];
-        x[i] = *(const FE_GLOBAL f32x4*)(po + (long long)s * 16 * DP);
-      }
-#pragma unroll
-      for (int i = 0; i < PF; ++i)
-        if (i && s0 + i * NG >= count) ms[i] = kDecNegInf, ls[i] = 0.f, x[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
-      float mn = m;
-#pragma unroll
-      for (int i = 0; i < PF; ++i) mn = fmaxf(mn, ms[i]);
-      const float ref = mn == kDecNegInf ? 0.f : mn, keep = fast_exp2(m - ref);
-      l *= keep;
-      acc *= keep;
-#pragma unroll
-      for (int i = 0; i < PF; ++i) {
-        // a split that this row sees nothing of has a weight of 0 and values of 0
-        const float w = ls[i] * fast_exp2(ms[i] - ref);
-        l += w;
-        acc += w * x[i];
-      }
-      m = mn;
-    }
-    if (grp < NG) {
-      so[tid] = acc;
-      if (c4 == 0) sm[0][grp] = m, sl[0][grp] = l;
-    }
-    __syncthreads();
-    if (grp) return;
-    float mx = m;
-#pragma unroll
-    for (int i = 1; i < NG; ++i) mx = fmaxf(mx, sm[0][i]);
-    const float ref = mx == kDecNegInf ? 0.f : mx, keep = fast_exp2(m - ref);
-    l *= keep;
-    acc *= keep;
-#pragma unroll
-    for (int i = 1; i < NG; ++i) {
-      const float w = fast_exp2(sm[0][i] - ref);
-      l += w * sl[0][i];
-      acc += w * so[i * LPR + c4];
-    }
-    acc *= l == 0.f ? 0.f : 1.f / l;
-    const long long at = (long long)bh * a.R + row;       // [B, Hkv, G, T]
-    if (4 * c4 < a.D) *(FE_GLOBAL u32x2*)(a.out + at * a.D + 4 * c4) = (u32x2){E::pack2(acc[0], acc[1]), E::pack2(acc[2], acc[3])};
-    if (c4 == 0) a.lse[at] = l == 0.f ? kDecNegInf : (ref + fast_log2(l)) * kLn2;
-    return;
-  }
-
-  const int part = (int)blockIdx.x - a.R, step = 8 * ((int)gridDim.x - a.R), l32 = tid & 31;
-  int t = part * 8 + (tid >> 5);
-  if (part * 8 >= tiles) return;
-  float x[PF], old = 0.f, w = 1.f;          // a tile's first rows of logits; its keys' importance and norms
+  const int nc = (n + 63) / 64, tiles = dec_tiles<64>(n, a.T), share = dec_split<1>(tiles, a.S);
+  const int t0 = (int)blockIdx.x * share, t1 = min(tiles, t0 + share);
+  if (t0 >= t1) return;
   {
-    const int row = tid & 15, grp = tid >> 4;
-    const DecF32In ml = a.part_ml + first * 32 + row;
-    float m = kDecNegInf, l = 0.f;
-    if (row < a.R) {
-#pragma unroll 1
-      for (int s = grp; s < count; s += 16) {
-        const float ms = ml[s * 32], ls = ml[s * 32 + 16];
-        const float mn = fmaxf(m, ms), ref = mn == kDecNegInf ? 0.f : mn;
-        l = l * fast_exp2(m - ref) + ls * fast_exp2(ms - ref);
-        m = mn;
+    const int r = rb * a.RS + wv * 32 + l32;
+    const bool live = wv * 32 < a.RS && rb * a.RS + wv * 32 < a.R;   // the wave has rows
+    const bool rv = live && r < a.R;
+    const int g = rv ? r / a.T : 0, tq = rv ? r - g * a.T : 0;
+    const DecIn kc = a.kc + b * a.kcb + hkv * a.kch, vc = a.vc + b * a.vcb + hkv * a.vch;
+    const DecIn kn = a.k + b * a.kb + hkv * a.kh, vn = a.v + b * a.vb + hkv * a.vh;
+    u32x4 qf[NDC];
+    {
+      const DecIn qp = a.q + b * a.qb + (long long)(hkv * (a.R / a.T) + g) * a.qh + tq * a.qn;
+      int D = a.D;
+      asm volatile("" : "+s"(D));
+#pragma unroll
+      for (int c = 0; c < NDC; ++c) qf[c] = *(const FE_GLOBAL u32x4*)(qp + (16 * c + 8 * hh < D ? 16 * c + 8 * hh : 0));
+    }
+    f32x16 o[NDT];
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) o[dt] = (f32x16){};
+    float m = kDecNegInf, nm = 0.f, l = 0.f, lr = 0.f;   // lane-wise sums (half of a row's keys each)
+    u32x4 kx[NL] = {}, vx[NL] = {};
+    // a tile's rows on their way (past the last, the last), and into LDS
+    auto load = [&](int t) __attribute__((always_inline)) {
+      const bool nt = t >= nc;
+      const int kb = (nt ? t - nc : t) * 64, last = (nt ? a.T : n) - 1;
+      const DecIn kp = nt ? kn : kc, vp = nt ? vn : vc;
+      const u32 ks = nt ? a.kn : a.kcn, vs = nt ? a.vn : a.vcn;
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const int e = i * NT + tid, ch = 8 * (e % CPR);
+        const u32 row = (u32)min(kb + e / CPR, last);
+        const int cc = ch < a.D ? ch : 0;
+        kx[i] = *(const FE_GLOBAL u32x4*)(kp + (unsigned long long)row * ks + cc);
+        vx[i] = *(const FE_GLOBAL u32x4*)(vp + (unsigned long long)row * vs + cc);
       }
-    }
-    sm[grp][row] = m;
-    sl[grp][row] = l;
-    __syncthreads();
-    if (tid < 16) {
-#pragma unroll 4
-      for (int i = 1; i < 16; ++i) m = fmaxf(m, sm[i][row]);
-      const float ref = m == kDecNegInf ? 0.f : m;
-      l = 0.f;
-#pragma unroll 4
-      for (int i = 0; i < 16; ++i) l += sl[i][row] * fast_exp2(sm[i][row] - ref);
-      // log2 of l and of w = 2^(-decay (T - 1 - t)); rows that see nothing, or are none, give no weight
-      bias[row] = l == 0.f || row >= a.R ? -kDecNegInf : ref + fast_log2(l) + a.decay_log2 * (float)(a.T - 1 - row % a.T);
-    }
-    __syncthreads();
-  }
-  const float keep = fast_exp2(-a.decay_log2 * (float)a.T);
-#pragma unroll 1
-  for (; t < tiles; t += step) {
-    const DecF32In lp = a.logits + ((long long)bh * a.max_tiles + t) * a.R * 32 + l32;
-    const int key = t * 32 + l32;
+    };
+    auto kbuf = [&](int t) -> unsigned char* { return lds + (t & 1) * TILE; };
+    auto vbuf = [&](int t) -> unsigned char* { return lds + (2 + t % VB) * TILE; };
+    auto store = [&](int t) __attribute__((always_inline)) {
+      const int buf = t & 1;
+      unsigned char* kt = kbuf(t);
+      unsigned char* vt = vbuf(t);
+      const bool nt = t >= nc;
+      const int kb = (nt ? t - nc : t) * 64, rows = nt ? a.T : n;
+      if (kb + 64 > rows) dec_cut_rows<DP, NT>(kb, rows, tid, vx);
+      if (a.D != DP) {
+        int D = a.D;
+        asm volatile("" : "+s"(D));
 #pragma unroll
-    for (int i = 0; i < PF; ++i) x[i] = lp[min(i, a.R - 1) * 32];
-    if (key < n) {
-      old = a.imp[bh * a.imp_stride + key];
-      if (a.norm) w = a.norm[bh * a.norm_stride + key];
-    }
-    float sum = 0.f;
+        for (int i = 0; i < NL; ++i)
+          if (8 * ((i * NT + tid) % CPR) >= D) kx[i] = (u32x4){0u, 0u, 0u, 0u};
+      }
 #pragma unroll
-    for (int i = 0; i < PF; ++i) sum += fast_exp2(x[i] - bias[i]);
-#pragma unroll 1
-    for (int r0 = PF; r0 < a.R; r0 += PF) {
-#pragma unroll
-      for (int i = 0; i < PF; ++i) x[i] = lp[min(r0 + i, a.R - 1) * 32];
-#pragma unroll
-      for (int i = 0; i < PF; ++i) sum += fast_exp2(x[i] - bias[r0 + i]);
-    }
-    if (t < nc) {
-      if (key < n) a.imp_out[bh * a.impo_stride + key] = old * keep + w * sum;
-    } else if (key - nc * 32 < a.T) {
-      const int u = key - nc * 32;
-      float nu = 1.f;
-      if (a.norm) {
-        const FE_GLOBAL u32x4* vp = (const FE_GLOBAL u32x4*)(a.v + b * a.vb + hkv * a.vh + (unsigned long long)u * a.vn);
-        nu = 0.f;
-        for (int d = 0; d < a.D / 8; ++d) {
-          const u32x4 y = vp[d];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) nu += fabsf(E::to_f32((u16)y[i])) + fabsf(E::to_f32((u16)(y[i] >> 16)));
+      for (int i = 0; i < NL; ++i) {
+        const int e = i * NT + tid;
+        if (64 * CPR % NT == 0 || e < 64 * CPR) {
+          *(u32x4*)(kt + dec_k_at<DP>(e / CPR, e % CPR)) = kx[i];
+          *(u32x4*)(vt + dec_v_at<DP>(e / CPR, e % CPR)) = vx[i];
         }
       }
-      a.new_imp[(long long)bh * a.T + u] = nu * sum;
+      if (nt) {
+        if (tid < 2) s_odd[buf][tid] = 0u;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+          const int key = (i * NT + tid) / CPR;
+          if (key < 64 && dec_nonfinite<E>(vx[i])) atomicOr(&s_odd[buf][key >> 5], 1u << (key & 31));
+        }
+      }
+    };
+    load(t0);
+    // (unconditionally: fragments changed in a branch cost 250 spilled registers)
+#pragma unroll
+    for (int c = 0; c < NDC; ++c) {
+      const u32 keep = rv && 16 * c + 8 * hh < a.D ? a.qand : 0u, flip = keep ? a.qxor : 0u;
+      qf[c] = (qf[c] & keep) ^ flip;
+    }
+    store(t0);
+    __syncthreads();
+    u32x4 pf[4];                           // a tile's probabilities, as the product takes them
+    auto product = [&](int t) __attribute__((always_inline)) {
+      unsigned char* vt = vbuf(t);
+#pragma unroll
+      for (int c4 = 0; c4 < 4; ++c4)
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) o[dt] = E::mfma(dec_vfrag<DP>(vt, 16 * c4, dt), pf[c4], o[dt]);
+    };
+#pragma unroll 1
+    for (int t = t0; t < t1; ++t) {
+      if (t + 1 < t1) load(t + 1);
+      {
+        const int buf = t & 1;
+        const bool tail = t >= nc;
+        const int kb = (tail ? t - nc : t) * 64, rows = tail ? a.T : n;
+        unsigned char* kt = kbuf(t);
+        unsigned long long odd = 0;
+        if (tail) {
+          if (a.tree) {
+            // the tile's columns of the mask, a query token a ballot
+            const FE_GLOBAL unsigned char* row = a.tree + b * a.tree_stride + min(kb + lane, a.T - 1);
+#pragma unroll 4
+            for (int u = wv; u < a.T; u += NW) {
+              const unsigned long long sees = __ballot(row[u * a.T] != 0);
+              if (lane < 2) s_tree[u][lane] = (u32)(sees >> (32 * lane));
+            }
+          }
+          odd = ((unsigned long long)s_odd[buf][1] << 32) | s_odd[buf][0];
+          if (odd)
+            for (int e = tid; e < 64 * CPR; e += NT)
+              if ((odd >> (e / CPR)) & 1u) *(u32x4*)(vbuf(t) + dec_v_at<DP>(e / CPR, e % CPR)) = (u32x4){0u, 0u, 0u, 0u};
+          __syncthreads();
+        }
+        if (live) {
+          if (late && t > t0) product(t - 1);
+          u32 vis[2] = {~0u, ~0u};         // bit 8 (i / 4) + i % 4 of word s: register i of x[s] is of a visible key
+          const bool masked = tail || kb + 64 > rows;
+          if (masked) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+              const int left = rows - kb - 32 * s, own = tq - kb - 32 * s + 1;
+              u32 x = left >= 32 ? ~0u : left > 0 ? (1u << left) - 1u : 0u;
+              if (tail) x &= a.tree ? s_tree[tq][s] : own >= 32 ? ~0u : own > 0 ? (1u << own) - 1u : 0u;
+              vis[s] = x >> (4 * hh);
+            }
+          }
+          f32x16 x[2];                     // logits, then probabilities
+          auto logits = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+#pragma unroll
+              for (int c = 0; c < NDC; ++c) {
+                if (c % 4 == 0) __builtin_amdgcn_sched_barrier(0);   // four fragments in flight
+                x[s] = c == 0 ? E::mfma(dec_kfrag<DP>(kt, 32 * s, 0), qf[0], (f32x16){}) : E::mfma(dec_kfrag<DP>(kt, 32 * s, c), qf[c], x[s]);
+              }
+            }
+            if (masked) {
+#pragma unroll
+              for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  const u32 on = (u32)((int)(vis[s] << (31 - 8 * (i >> 2) - (i & 3))) >> 31);
+                  x[s][i] = __uint_as_float((__float_as_uint(x[s][i]) & on) | (0xff800000u & ~on));
+                }
+            }
+          };
+          float ls;
+          auto exponentials = [&]() __attribute__((always_inline)) {
+            ls = 0.f;
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                x[s][i] = fast_exp2(x[s][i] * a.scale_log2 + nm);
+                ls += x[s][i];
+              }
+          };
+          logits();
+          exponentials();
+          const bool over = !(ls <= E::kMaxTileSum) || m == kDecNegInf;
+          if (__ballot(over)) {
+            // a new reference for rows without one, and for those whose probabilities grew too large
+            logits();
+            float mx = kDecNegInf;
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x[s][i]);
+            mx = half_swap_max(mx) * a.scale_log2;
+            const bool take = half_swap_max(over ? 1.f : 0.f) > 0.f && mx > m;
+            const float alpha = !take ? 1.f : m == kDecNegInf ? 0.f : fast_exp2(m - mx);
+            m = take ? mx : m;
+            nm = take ? -mx : nm;
+            l *= alpha;
+            lr *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt) o[dt] *= alpha;
+            exponentials();
+          }
+          if (odd) {
+#pragma unroll 1
+            for (unsigned long long left = odd; left; left &= left - 1) {
+              const int key = __ffsll(left) - 1;
+              // the register that holds the key, in the lanes whose half it is and whose query sees it
+              const int s = key >> 5, reg = 16 * s + 4 * ((key >> 3) & 3) + (key & 3), bit = 8 * ((key >> 3) & 3) + (key & 3);
+              const bool in = ((key >> 2) & 1) == hh && (((s ? vis[1] : vis[0]) >> bit) & 1u);
+              float mine = 0.f;
+#pragma unroll
+              for (int i = 0; i < 32; ++i) mine = i == reg ? x[i >> 4][i & 15] : mine;
+              if (!in) mine = -1.f;
+              const float pk = half_swap_max(mine);      // probabilities are not negative
+              const float nan = half_swap_max(mine != mine ? 1.f : 0.f);
+              const float pr = nan > 0.f ? __builtin_nanf("") : pk;
+              const bool sees = pk >= 0.f || nan > 0.f;
+              const DecIn row = vn + (unsigned long long)(kb + key) * a.vn;
+              for (int ch = lane; ch < DP; ch += 64) s_row[wv][ch] = ch < a.D ? E::to_f32(row[ch]) : 0.f;
+              dec_wave_order();
+#pragma unroll
+              for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  const float y = s_row[wv][32 * dt + 8 * (i >> 2) + 4 * hh + (i & 3)];
+                  if (sees) o[dt][i] += pr * y;
+                }
+              dec_wave_order();
+            }
+          }
+          l += ls;
+#pragma unroll
+          for (int c4 = 0; c4 < 4; ++c4)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              pf[c4][i] = E::pack2(x[c4 >> 1][8 * (c4 & 1) + 2 * i], x[c4 >> 1][8 * (c4 & 1) + 2 * i + 1]);
+              lr = E::sum2(pf[c4][i], ones2, lr);
+            }
+          if (!late) product(t);
+        }
+      }
+      if (t + 1 < t1) store(t + 1);
+      __syncthreads();
+    }
+
+    if (live && late) product(t1 - 1);
+    __syncthreads();                       // LDS is the outputs' from here on
+    l = half_swap_sum(l);
+    lr = half_swap_sum(lr);
+    const long long slot = ((long long)bh * a.RB + rb) * a.S + blockIdx.x;
+    if (live) {
+      const float inv = lr == 0.f ? 0.f : 1.f / lr;
+      if (rv && hh == 0) {
+        a.part_ml[slot * 2 * a.RS + wv * 32 + l32] = m;
+        a.part_ml[slot * 2 * a.RS + a.RS + wv * 32 + l32] = l;
+      }
+      // 16 rows at a time through LDS, so that rows are stored whole
+      float* mine = (float*)lds + wv * 16 * OST;
+#pragma unroll 1
+      for (int half = 0; half < 2; ++half) {
+        if ((l32 >> 4) == half) {
+#pragma unroll
+          for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              *(f32x4*)(mine + (l32 & 15) * OST + 32 * dt + 8 * i + 4 * hh) =
+                  (f32x4){o[dt][4 * i] * inv, o[dt][4 * i + 1] * inv, o[dt][4 * i + 2] * inv, o[dt][4 * i + 3] * inv};
+        }
+        dec_wave_order();
+        const int row0 = wv * 32 + 16 * half, rows = min(16, a.R - rb * a.RS - row0);
+#pragma unroll 4
+        for (int e = lane; e < rows * (DP / 4); e += 64)
+          *(FE_GLOBAL f32x4*)(a.part_o + (slot * a.RS + row0) * DP + 4 * e) = *(const f32x4*)(mine + e / (DP / 4) * OST + 4 * (e % (DP / 4)));
+        dec_wave_order();
+      }
     }
   }
 }
 
-// What bounds it: HBM. Few rows leave the matrix and vector units mostly idle, so every wave keeps the next 32 keys'
-// K and V on the way to registers while it works on these.
-template <typename E, int DP, int VEC>
-__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_rows_kernel(const DecArgs args) {
+// 32 rows a block, keys to its waves 32 at a time, everything read element by element.
+template <typename E, int DP>
+__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_elements_kernel(const DecArgs a) {
   constexpr int NDC = DP / 16, NDT = DP / 32, CPR = DP / 8, TILE = 64 * DP;   // bytes of 32 rows
   constexpr int OST = 33;                // floats of a channel's 32 rows in LDS, and one against bank conflicts
   constexpr int WLDS = DP * OST * 4;     // a wave's LDS: a K and a V tile, then its output
@@ -876,68 +791,48 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_rows_kernel(cons
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   unsigned char* kt = lds[wv];
   unsigned char* vt = lds[wv] + TILE;
-  const DecArgs a = dec_hold<kDecAttnArgs, 5>(args);
 
-  DecShare sh = dec_share<32, 4>(a, a.RB, a.T);
-  while (sh.pos < sh.hi) {
-    const int bh = sh.bh, b = bh / a.Hkv, hkv = bh - b * a.Hkv;
-    const int n = dec_share_len(sh);
-    const int nc = (n + 31) / 32, tiles = dec_tiles<32>(n, a.T);
-    const int rb = a.RB == 1 ? 0 : (sh.pos - sh.base) / tiles, t0 = sh.pos - sh.base - rb * tiles;
-    const int t1 = min(tiles, t0 + sh.hi - sh.pos);
-    sh.pos += t1 - t0;
-    if (t1 == tiles && rb == a.RB - 1) dec_share_next(a, sh);
-
+  const int hkv = (int)blockIdx.y, z = (int)blockIdx.z, b = z / a.RB, rb = z - b * a.RB, bh = b * (int)gridDim.y + hkv;
+  const int n = __builtin_amdgcn_readfirstlane(min(max(a.length[bh], 0), a.C));
+  const int nc = (n + 31) / 32, tiles = dec_tiles<32>(n, a.T), share = dec_split<4>(tiles, a.S);
+  const int t0 = (int)blockIdx.x * share, t1 = min(tiles, t0 + share);
+  if (t0 >= t1) return;
+  {
     const int r = rb * 32 + l32;         // this lane's query row
     const bool rv = r < a.R;
     const int g = rv ? r / a.T : 0, tq = rv ? r - g * a.T : 0;
-    const DecRows hr = dec_rows(a, b, hkv);
+    const DecIn kc = a.kc + b * a.kcb + hkv * a.kch, vc = a.vc + b * a.vcb + hkv * a.vch;
+    const DecIn kn = a.k + b * a.kb + hkv * a.kh, vn = a.v + b * a.vb + hkv * a.vh;
     u32x4 qf[NDC];
-    dec_read_q<DP, VEC>(a, b, hkv * a.G + g, tq, qf);
+    {
+      const DecIn qp = a.q + b * a.qb + (long long)(hkv * (a.R / a.T) + g) * a.qh + tq * a.qn;   // a real row in any case
+#pragma unroll
+      for (int c = 0; c < NDC; ++c) {
+        qf[c] = (dec_load8(qp, a.qc, 2 * c + hh, a.D) & a.qand) ^ a.qxor;
+        __builtin_amdgcn_sched_barrier(0);   // one chunk's addresses at a time
+      }
+    }
     f32x16 o[NDT];
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) o[dt] = (f32x16){};
     float m = kDecNegInf, l = 0.f, lr = 0.f;   // sums of the probabilities, and of these as rounded for the product
 
-    u32x4 kx[VEC ? NDC : 1] = {}, vx[VEC ? NDC : 1] = {};
-    auto load = [&](int t) __attribute__((always_inline)) {
-      const DecTile at = dec_tile<32>(hr, n, nc, a.T, t);
-      dec_load_rows<DP, 32, 64>(at.k, at.krs, at.kb, at.rows, a.D, lane, kx);
-      dec_load_rows<DP, 32, 64>(at.v, at.vrs, at.kb, at.rows, a.D, lane, vx);
-    };
-    if (VEC && t0 + wv < t1) load(t0 + wv);
-    dec_set_q<DP>(a, rv, qf);
     for (int t = t0 + wv; t < t1; t += 4) {
-      const DecTile at = dec_tile<32>(hr, n, nc, a.T, t);
-      const bool tail = at.tail;
-      const int kb = at.kb, rows = at.rows;
-      const long long vcs = VEC ? 1 : tail ? a.vnc : a.vcc;
+      const bool tail = t >= nc;
+      const int kb = (tail ? t - nc : t) * 32, rows = tail ? a.T : n;
+      const DecIn kp = tail ? kn : kc, vp = tail ? vn : vc;
+      const long long krs = tail ? a.kn64 : a.kcn64, vrs = tail ? a.vn64 : a.vcn64, kcs = tail ? a.kd : a.kcd, vcs = tail ? a.vd : a.vcd;
       // keys of the tail whose value has an infinity or a NaN: 0 * inf would reach the rows that do not see
       // them, so their values are taken out of the product and added to the rows that do
       u32 odd = 0;
-      if (VEC) {
-        if (kb + 32 > rows) dec_cut_rows<DP, 64>(kb, rows, lane, vx);
-#pragma unroll
-        for (int i = 0; i < NDC; ++i) {
-          const int e = i * 64 + lane;
-          *(u32x4*)(kt + dec_k_at<DP>(e / CPR, e % CPR)) = kx[i];
-          *(u32x4*)(vt + dec_v_at<DP>(e / CPR, e % CPR)) = vx[i];
-        }
-        if (tail) {
-#pragma unroll
-          for (int i = 0; i < NDC; ++i)
-            for (unsigned long long bl = __ballot(dec_nonfinite<E>(vx[i])); bl; bl &= bl - 1) odd |= 1u << ((i * 64 + __ffsll(bl) - 1) / CPR);
-        }
-        if (t + 4 < t1) load(t + 4);
-      } else {
-        const long long kcs = tail ? a.knc : a.kcc;
+      {
 #pragma unroll 1
         for (int i = 0; i < NDC; ++i) {
           const int e = i * 64 + lane, row = kb + e / CPR, ch = e % CPR;
-          const u32x4 x = row < rows ? dec_load8(at.k + row * at.krs, kcs, ch, a.D) : (u32x4){0u, 0u, 0u, 0u};
+          const u32x4 x = row < rows ? dec_load8(kp + row * krs, kcs, ch, a.D) : (u32x4){0u, 0u, 0u, 0u};
           *(u32x4*)(kt + dec_k_at<DP>(e / CPR, ch)) = x;
           __builtin_amdgcn_sched_barrier(0);
-          const u32x4 y = row < rows ? dec_load8(at.v + row * at.vrs, vcs, ch, a.D) : (u32x4){0u, 0u, 0u, 0u};
+          const u32x4 y = row < rows ? dec_load8(vp + row * vrs, vcs, ch, a.D) : (u32x4){0u, 0u, 0u, 0u};
           *(u32x4*)(vt + dec_v_at<DP>(e / CPR, ch)) = y;
           if (tail)
             for (unsigned long long bl = __ballot(dec_nonfinite<E>(y)); bl; bl &= bl - 1) odd |= 1u << ((i * 64 + __ffsll(bl) - 1) / CPR);
@@ -955,7 +850,14 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_rows_kernel(cons
       for (int c = 0; c < NDC; ++c) x = c == 0 ? E::mfma(dec_kfrag<DP>(kt, 0, 0), qf[0], (f32x16){}) : E::mfma(dec_kfrag<DP>(kt, 0, c), qf[c], x);
       u32 vis = ~0u;
       if (tail || kb + 32 > rows) {
-        vis = dec_visible(a, b, tq, kb, rows, tail);
+        vis = 0;
+#pragma unroll 1
+        for (int i = 0; i < 16; ++i) {
+          const int key = kb + 8 * (i >> 2) + 4 * hh + (i & 3);
+          bool see = key < rows;
+          if (tail) see = see && (a.tree ? a.tree[b * a.tree_stride + tq * a.T + (see ? key : 0)] != 0 : key <= tq);
+          vis |= (see ? 1u : 0u) << i;
+        }
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] = (vis >> i) & 1u ? x[i] : kDecNegInf;
       }
@@ -1006,7 +908,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_rows_kernel(cons
         for (int i = 0; i < 16; ++i) sp[(8 * (i >> 2) + 4 * hh + (i & 3)) * 32 + l32] = (vis >> i) & 1u ? x[i] : -1.f;
         for (u32 left = odd; left; left &= left - 1) {
           const int key = __ffs((int)left) - 1;
-          for (int ch = lane; ch < DP; ch += 64) row[ch] = ch < a.D ? E::to_f32(at.v[(kb + key) * at.vrs + ch * vcs]) : 0.f;
+          for (int ch = lane; ch < DP; ch += 64) row[ch] = ch < a.D ? E::to_f32(vp[(kb + key) * vrs + ch * vcs]) : 0.f;
           dec_wave_order();
           const float p = sp[key * 32 + l32];
 #pragma unroll
@@ -1034,7 +936,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_rows_kernel(cons
 #pragma unroll
       for (int i = 0; i < 16; ++i) mine[(32 * dt + 8 * (i >> 2) + 4 * hh + (i & 3)) * OST + l32] = o[dt][i];
     __syncthreads();
-    const int slot = dec_slot(a, bh * a.RB + rb, t0 == 0, t1 == tiles);
+    const long long slot = ((long long)bh * a.RB + rb) * a.S + blockIdx.x;
     const int rows = min(32, a.R - rb * 32);
     for (int e = threadIdx.x; e < rows * DP; e += 256) {
       const int row = e / DP, ch = e % DP;
@@ -1050,464 +952,177 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_rows_kernel(cons
       }
       // partials are normalised by the sum of the rounded probabilities, and weighted by the exact one: so a row
       // that one key dominates returns that key's value whatever the split
-      a.part_o[((long long)slot * 32 + row) * DP + ch] = lrt == 0.f ? 0.f : s * (1.f / lrt);
+      a.part_o[(slot * 32 + row) * DP + ch] = lrt == 0.f ? 0.f : s * (1.f / lrt);
       if (ch == 0) {
         a.part_ml[slot * 64 + row] = mx;
         a.part_ml[slot * 64 + 32 + row] = lt;
       }
     }
-    __syncthreads();                        // the next segment's tiles follow these reads
   }
 }
 
-// A wave holds 32 of the segment's rows; the block's waves share tiles of 64 keys, double-buffered, whose loads are on
-// the way to registers during the tile before. A row keeps its reference maximum until a tile's probabilities could
-// overflow (E::kMaxTileSum), as in the prefill kernels, so most tiles spend nothing on maxima and rescaling.
-// What bounds it: vector work beside the products (an exponential a logit); at 256 rows a tile takes about as long as
-// its bytes from HBM.
-template <typename E, int DP, int NW>
-__global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void decode_wide_kernel(const DecWideArgs args) {
-  constexpr int NDC = DP / 16, NDT = DP / 32, CPR = DP / 8, TILE = 128 * DP;   // bytes of 64 rows
-  constexpr int NT = NW * 64, NL = (64 * CPR + NT - 1) / NT;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds_k[2][TILE], lds_v[2][TILE];
-  __shared__ u32 s_odd[2][2];            // keys of a tile of new rows with a value that is not finite
-  __shared__ float s_row[NW][DP];        // such a value, by each wave
-  const DecWideArgs a = dec_hold<0, 4>(args);
-  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
-  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  u32 ones2;
-  asm volatile("s_mov_b32 %0, %1" : "=s"(ones2) : "i"(E::kOnes2));
-
-  DecShare sh = dec_share<64, 1>(a, a.RB, a.T);
-#pragma unroll 1
-  while (sh.pos < sh.hi) {
-    const int bh = sh.bh, b = bh / a.Hkv, hkv = bh - b * a.Hkv;
-    const int n = dec_share_len(sh);
-    const int nc = (n + 63) / 64, tiles = dec_tiles<64>(n, a.T);
-    const int rb = a.RB == 1 ? 0 : (sh.pos - sh.base) / tiles, t0 = sh.pos - sh.base - rb * tiles;
-    const int t1 = min(tiles, t0 + sh.hi - sh.pos);
-    sh.pos += t1 - t0;
-    if (t1 == tiles && rb == a.RB - 1) dec_share_next(a, sh);
-
-    const int r = (rb * a.RW + wv) * 32 + l32;
-    const bool live = wv < a.RW && (rb * a.RW + wv) * 32 < a.R;   // the wave has rows
-    const bool rv = live && r < a.R;
-    const int g = rv ? r / a.T : 0, tq = rv ? r - g * a.T : 0;
-    const DecIn kc = a.kc + b * a.kcb + hkv * a.kch, vc = a.vc + b * a.vcb + hkv * a.vch;
-    const DecIn kn = a.k + b * a.kb + hkv * a.kh, vn = a.v + b * a.vb + hkv * a.vh;
-    u32x4 qf[NDC];
-    {
-      const DecIn qp = a.q + b * a.qb + (long long)(hkv * a.G + g) * a.qh + tq * a.qn;
-      int D = a.D;
-      asm volatile("" : "+s"(D));
-#pragma unroll
-      for (int c = 0; c < NDC; ++c) qf[c] = *(const FE_GLOBAL u32x4*)(qp + (16 * c + 8 * hh < D ? 16 * c + 8 * hh : 0));
-    }
-    f32x16 o[NDT];
-#pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) o[dt] = (f32x16){};
-    float m = kDecNegInf, nm = 0.f, l = 0.f, lr = 0.f;   // lane-wise sums (half of a row's keys each)
-    u32x4 kx[NL] = {}, vx[NL] = {};
-    // a tile's rows on their way (past the last, the last), and into LDS
-    auto load = [&](int t) __attribute__((always_inline)) {
-      const bool nt = t >= nc;
-      const int kb = (nt ? t - nc : t) * 64, last = (nt ? a.T : n) - 1;
-      const DecIn kp = nt ? kn : kc, vp = nt ? vn : vc;
-      const u32 ks = nt ? a.kn : a.kcn, vs = nt ? a.vn : a.vcn;
-#pragma unroll
-      for (int i = 0; i < NL; ++i) {
-        const int e = i * NT + tid, ch = 8 * (e % CPR);
-        const u32 row = (u32)min(kb + e / CPR, last);
-        const int cc = ch < a.D ? ch : 0;
-        kx[i] = *(const FE_GLOBAL u32x4*)(kp + (unsigned long long)row * ks + cc);
-        vx[i] = *(const FE_GLOBAL u32x4*)(vp + (unsigned long long)row * vs + cc);
-      }
-    };
-    auto store = [&](int t) __attribute__((always_inline)) {
-      const int buf = t & 1;
-      const bool nt = t >= nc;
-      const int kb = (nt ? t - nc : t) * 64, rows = nt ? a.T : n;
-      if (kb + 64 > rows) dec_cut_rows<DP, NT>(kb, rows, tid, vx);
-      if (a.D != DP) {
-        int D = a.D;
-        asm volatile("" : "+s"(D));
-#pragma unroll
-        for (int i = 0; i < NL; ++i)
-          if (8 * ((i * NT + tid) % CPR) >= D) kx[i] = (u32x4){0u, 0u, 0u, 0u};
-      }
-#pragma unroll
-      for (int i = 0; i < NL; ++i) {
-        const int e = i * NT + tid;
-        if (64 * CPR % NT == 0 || e < 64 * CPR) {
-          *(u32x4*)(lds_k[buf] + dec_k_at<DP>(e / CPR, e % CPR)) = kx[i];
-          *(u32x4*)(lds_v[buf] + dec_v_at<DP>(e / CPR, e % CPR)) = vx[i];
-        }
-      }
-      if (nt) {
-        if (tid < 2) s_odd[buf][tid] = 0u;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < NL; ++i) {
-          const int key = (i * NT + tid) / CPR;
-          if (key < 64 && dec_nonfinite<E>(vx[i])) atomicOr(&s_odd[buf][key >> 5], 1u << (key & 31));
-        }
-      }
-    };
-    load(t0);
-    // (unconditionally: fragments changed in a branch cost 250 spilled registers)
-#pragma unroll
-    for (int c = 0; c < NDC; ++c) {
-      const u32 keep = rv && 16 * c + 8 * hh < a.D ? a.qand : 0u, flip = keep ? a.qxor : 0u;
-      qf[c] = (qf[c] & keep) ^ flip;
-    }
-    store(t0);
-    __syncthreads();
-#pragma unroll 1
-    for (int t = t0; t < t1; ++t) {
-      if (t + 1 < t1) load(t + 1);
-      {
-        const int buf = t & 1;
-        const bool tail = t >= nc;
-        const int kb = (tail ? t - nc : t) * 64, rows = tail ? a.T : n;
-        unsigned char* kt = lds_k[buf];
-        unsigned char* vt = lds_v[buf];
-        unsigned long long odd = 0;
-        if (tail) {
-          odd = ((unsigned long long)s_odd[buf][1] << 32) | s_odd[buf][0];
-          if (odd) {
-            for (int e = tid; e < 64 * CPR; e += NT)
-              if ((odd >> (e / CPR)) & 1u) *(u32x4*)(vt + dec_v_at<DP>(e / CPR, e % CPR)) = (u32x4){0u, 0u, 0u, 0u};
-            __syncthreads();
-          }
-        }
-        if (live) {
-          u32 vis[2] = {~0u, ~0u};
-          const bool masked = tail || kb + 64 > rows;
-          if (masked) {
-#pragma unroll 1
-            for (int s = 0; s < 2; ++s) {
-              const u32 x = dec_visible(a, b, tq, kb + 32 * s, rows, tail);
-              vis[0] = s ? vis[0] : x;
-              vis[1] = x;
-            }
-          }
-          f32x16 x[2];                     // logits, then probabilities
-          auto logits = [&]() __attribute__((always_inline)) {
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-#pragma unroll
-              for (int c = 0; c < NDC; ++c) {
-                if (c % 4 == 0) __builtin_amdgcn_sched_barrier(0);   // four fragments in flight
-                x[s] = c == 0 ? E::mfma(dec_kfrag<DP>(kt, 32 * s, 0), qf[0], (f32x16){}) : E::mfma(dec_kfrag<DP>(kt, 32 * s, c), qf[c], x[s]);
-              }
-            }
-            if (masked) {
-#pragma unroll
-              for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) x[s][i] = (vis[s] >> i) & 1u ? x[s][i] : kDecNegInf;
-            }
-          };
-          float ls;
-          auto exponentials = [&]() __attribute__((always_inline)) {
-            ls = 0.f;
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                x[s][i] = fast_exp2(x[s][i] * a.scale_log2 + nm);
-                ls += x[s][i];
-              }
-          };
-          logits();
-          exponentials();
-          const bool over = !(ls <= E::kMaxTileSum) || m == kDecNegInf;
-          if (__ballot(over)) {
-            // a new reference for rows without one, and for those whose probabilities grew too large
-            logits();
-            float mx = kDecNegInf;
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-              for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x[s][i]);
-            mx = half_swap_max(mx) * a.scale_log2;
-            const bool take = half_swap_max(over ? 1.f : 0.f) > 0.f && mx > m;
-            const float alpha = !take ? 1.f : m == kDecNegInf ? 0.f : fast_exp2(m - mx);
-            m = take ? mx : m;
-            nm = take ? -mx : nm;
-            l *= alpha;
-            lr *= alpha;
-#pragma unroll
-            for (int dt = 0; dt < NDT; ++dt) o[dt] *= alpha;
-            exponentials();
-          }
-          if (odd) {
-#pragma unroll 1
-            for (unsigned long long left = odd; left; left &= left - 1) {
-              const int key = __ffsll(left) - 1;
-              // the register and half that hold the key, where the lane's query sees it
-              float mine = -1.f;
-#pragma unroll
-              for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                  if (key == 32 * s + 8 * (i >> 2) + 4 * hh + (i & 3) && ((vis[s] >> i) & 1u)) mine = x[s][i];
-              const float pk = half_swap_max(mine);      // probabilities are not negative
-              const float nan = half_swap_max(mine != mine ? 1.f : 0.f);
-              const float pr = nan > 0.f ? __builtin_nanf("") : pk;
-              const bool sees = pk >= 0.f || nan > 0.f;
-              const DecIn row = vn + (unsigned long long)(kb + key) * a.vn;
-              for (int ch = lane; ch < DP; ch += 64) s_row[wv][ch] = ch < a.D ? E::to_f32(row[ch]) : 0.f;
-              dec_wave_order();
-#pragma unroll
-              for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                  const float y = s_row[wv][32 * dt + 8 * (i >> 2) + 4 * hh + (i & 3)];
-                  if (sees) o[dt][i] += pr * y;
-                }
-              dec_wave_order();
-            }
-          }
-          l += ls;
-#pragma unroll
-          for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int c4 = 0; c4 < 2; ++c4) {
-              u32x4 pf;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                pf[i] = E::pack2(x[s][8 * c4 + 2 * i], x[s][8 * c4 + 2 * i + 1]);
-                lr = E::sum2(pf[i], ones2, lr);
-              }
-#pragma unroll
-              for (int dt = 0; dt < NDT; ++dt) o[dt] = E::mfma(dec_vfrag<DP>(vt, 32 * s + 16 * c4, dt), pf, o[dt]);
-            }
-        }
-      }
-      if (t + 1 < t1) store(t + 1);
-      __syncthreads();
-    }
-
-    const int slot = dec_slot(a, bh * a.RB + rb, t0 == 0, t1 == tiles);
-    l = half_swap_sum(l);
-    lr = half_swap_sum(lr);
-    if (rv) {
-      const float inv = lr == 0.f ? 0.f : 1.f / lr;
-      const int row = wv * 32 + l32;
-      const DecF32 po = a.part_o + ((long long)slot * a.RW * 32 + row) * DP + 4 * hh;
-#pragma unroll
-      for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *(FE_GLOBAL f32x4*)(po + 32 * dt + 8 * i) =
-              (f32x4){o[dt][4 * i] * inv, o[dt][4 * i + 1] * inv, o[dt][4 * i + 2] * inv, o[dt][4 * i + 3] * inv};
-      if (hh == 0) {
-        a.part_ml[(long long)slot * 64 * a.RW + row] = m;
-        a.part_ml[(long long)slot * 64 * a.RW + 32 * a.RW + row] = l;
-      }
-    }
-  }
-}
-
-// A segment's first slot and its number of slots.
-__device__ __forceinline__ void dec_slots(const DecJoinArgs& a, int sg, int& first, int& count) {
-  first = a.seg[2 * sg];
-  count = a.seg[2 * sg + 1] - first + 1;
-}
-
-// Blocks below out_blocks: out = sum_s w_s O_s / sum w_s with w_s = l_s 2^(m_s - m), eight 32-lane groups a block,
-// `split` of them (1 or 8) on each row. Later blocks, where there are logits: importance_out and new_importance, tiles
-// of 32 keys of a head, per_head blocks on each.
-// What bounds it: waits. Its few loads depend on each other (slots, maxima, values), so what can be is read before.
+// Joins the splits. Blocks below out_blocks of a head: output rows, DP / 4 threads on a slot's values, merging slots as
+// they are read (maximum, sum, values); where a row has many slots all of a block's groups of threads are on one row.
+// The others, where there are logits: the head's importance, a tile of 32 keys to 32 lanes.
+// What bounds it: two trips to memory and the reading of its code; on long caches the logits' and weights' bytes.
 template <typename E, int DP>
 __global__ __launch_bounds__(256) void decode_join_kernel(const DecJoinArgs args) {
-  constexpr int NV = (DP + 127) / 128;      // float4 of a lane
-  constexpr int PF = 4;                     // splits, or rows of logits, in flight
-  __shared__ float sm[8][32], sl[8][32];
-  __shared__ float bias[32];
-  __shared__ f32x4 so[8][32 * NV];
+  constexpr int LPR = DP / 4, NG = 256 / LPR, PF = 4;   // threads on a slot, groups of them; loads in flight
+  __shared__ float sm[16][16], sl[16][16], bias[16];
+  __shared__ f32x4 so[NG * LPR];
   const DecJoinArgs a = dec_hold<0, 4>(args);
-  const int l32 = threadIdx.x & 31, grp = threadIdx.x >> 5;
+  const int tid = threadIdx.x, hkv = (int)blockIdx.y, b = (int)blockIdx.z, bh = b * (int)gridDim.y + hkv;
+  const int n = __builtin_amdgcn_readfirstlane(min(max(a.length[bh], 0), a.C));
   const int RS = a.RS;
   if ((int)blockIdx.x < a.out_blocks) {
-    const int split = a.split, per = 8 / split, sub = grp % split;
-    const int gr = (int)blockIdx.x * per + grp / split;   // row of all heads' rows
-    const bool rv = gr < a.BH * a.R;
-    const int bh = rv ? gr / a.R : 0, r = rv ? gr - bh * a.R : 0;
-    const int sgr = a.RB == 1 ? 0 : r / RS, row = r - sgr * RS;
-    int first, count;
-    dec_slots(a, bh * a.RB + sgr, first, count);
-    if (!rv) count = 0;
-    const DecF32In ml = a.part_ml + (long long)first * 2 * RS + row;
-    const DecF32In po = a.part_o + ((long long)first * RS + row) * DP + 4 * l32;
-    auto values = [&](int s, f32x4 (&x)[NV]) __attribute__((always_inline)) {
-#pragma unroll
-      for (int v = 0; v < NV; ++v)
-        x[v] = 128 * v + 4 * l32 < DP ? *(const FE_GLOBAL f32x4*)(po + (long long)s * RS * DP + 128 * v) : (f32x4){0.f, 0.f, 0.f, 0.f};
-    };
-    f32x4 x[PF][NV];
-#pragma unroll
-    for (int i = 0; i < PF; ++i)
-      if (sub + i * split < count) values(sub + i * split, x[i]);
+    const int grp = tid / LPR, c4 = tid - grp * LPR;
+    const int all = a.wide ? dec_tiles<64>(n, a.T) : dec_tiles<32>(n, a.T);
+    const int share = a.wide ? dec_split<1>(all, a.S) : dec_split<4>(all, a.S), count = (all + share - 1) / share;
+    const int row = (int)blockIdx.x * a.rows + (a.rows > 1 ? grp : 0), step = a.rows > 1 ? 1 : NG;
+    const bool rv = grp < NG && row < a.R;
+    const int rb = a.RB == 1 ? 0 : row / RS;
+    const long long first = ((long long)bh * a.RB + rb) * a.S;
+    const DecF32In ml = a.part_ml + first * 2 * RS + (row - rb * RS);
+    const DecF32In po = a.part_o + (first * RS + (row - rb * RS)) * DP + 4 * c4;
     float m = kDecNegInf, l = 0.f;
-    for (int s = l32; s < count; s += 32) {
-      const float ms = ml[(long long)s * 2 * RS], ls = ml[(long long)s * 2 * RS + RS];
-      const float mn = fmaxf(m, ms), ref = mn == kDecNegInf ? 0.f : mn;
-      l = l * fast_exp2(m - ref) + ls * fast_exp2(ms - ref);
-      m = mn;
-    }
-    float mx = m;
-#pragma unroll
-    for (int d = 16; d; d /= 2) mx = fmaxf(mx, __shfl_xor(mx, d));
-    const float ref = mx == kDecNegInf ? 0.f : mx;
-    l *= fast_exp2(m - ref);
-    m = mx;
-#pragma unroll
-    for (int d = 16; d; d /= 2) l += __shfl_xor(l, d);
-    f32x4 acc[NV];
-#pragma unroll
-    for (int v = 0; v < NV; ++v) acc[v] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    for (int s0 = sub; s0 < count; s0 += PF * split) {
-      if (s0 != sub) {
-#pragma unroll
-        for (int i = 0; i < PF; ++i)
-          if (s0 + i * split < count) values(s0 + i * split, x[i]);
-      }
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int s0 = a.rows > 1 ? 0 : grp; s0 < count && rv; s0 += PF * step) {
+      float ms[PF], ls[PF];
+      f32x4 x[PF];
 #pragma unroll
       for (int i = 0; i < PF; ++i) {
-        const int s = s0 + i * split;
-        if (s < count) {
-          // a split that this row sees nothing of has a weight of 0 and values of 0
-          const float w = ml[(long long)s * 2 * RS + RS] * fast_exp2(ml[(long long)s * 2 * RS] - ref);
-#pragma unroll
-          for (int v = 0; v < NV; ++v) acc[v] += w * x[i][v];
-        }
+        const int s = min(s0 + i * step, count - 1);
+        ms[i] = ml[(long long)s * 2 * RS];
+        ls[i] = ml[(long long)s * 2 * RS + RS];
+        x[i] = *(const FE_GLOBAL f32x4*)(po + (long long)s * RS * DP);
       }
+#pragma unroll
+      for (int i = 0; i < PF; ++i)
+        if (i && s0 + i * step >= count) ms[i] = kDecNegInf, ls[i] = 0.f, x[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      float mn = m;
+#pragma unroll
+      for (int i = 0; i < PF; ++i) mn = fmaxf(mn, ms[i]);
+      const float ref = mn == kDecNegInf ? 0.f : mn, keep = fast_exp2(m - ref);
+      l *= keep;
+      acc *= keep;
+#pragma unroll
+      for (int i = 0; i < PF; ++i) {
+        // a split that this row sees nothing of has a weight of 0 and values of 0
+        const float w = ls[i] * fast_exp2(ms[i] - ref);
+        l += w;
+        acc += w * x[i];
+      }
+      m = mn;
     }
-    if (split > 1) {
-#pragma unroll
-      for (int v = 0; v < NV; ++v) so[grp][v * 32 + l32] = acc[v];
+    if (a.rows == 1) {
+      if (grp < NG) {
+        so[tid] = acc;
+        if (c4 == 0) sm[0][grp] = m, sl[0][grp] = l;
+      }
       __syncthreads();
-      if (sub) return;
-      for (int i = 1; i < split; ++i)
+      if (grp) return;
+      float mx = m;
 #pragma unroll
-        for (int v = 0; v < NV; ++v) acc[v] += so[grp + i][v * 32 + l32];
+      for (int i = 1; i < NG; ++i) mx = fmaxf(mx, sm[0][i]);
+      const float ref = mx == kDecNegInf ? 0.f : mx, keep = fast_exp2(m - ref);
+      l *= keep;
+      acc *= keep;
+      m = mx;
+#pragma unroll
+      for (int i = 1; i < NG; ++i) {
+        const float w = fast_exp2(sm[0][i] - ref);
+        l += w * sl[0][i];
+        acc += w * so[i * LPR + c4];
+      }
     }
     if (!rv) return;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const int b = bh / a.Hkv, hkv = bh - b * a.Hkv, g = r / a.T, t = r - g * a.T;
-    const long long at = ((long long)b * a.Hkv * a.G + hkv * a.G + g) * a.T + t;
+    acc *= l == 0.f ? 0.f : 1.f / l;
+    const long long at = (long long)bh * a.R + row;       // [B, Hkv, G, T]
+    const u32 w0 = E::pack2(acc[0], acc[1]), w1 = E::pack2(acc[2], acc[3]);
+    FE_GLOBAL u16* op = a.out + at * a.D + 4 * c4;
+    if (a.D % 4 == 0) {
+      if (4 * c4 < a.D) *(FE_GLOBAL u32x2*)op = (u32x2){w0, w1};
+    } else {
+      const u16 h[4] = {(u16)w0, (u16)(w0 >> 16), (u16)w1, (u16)(w1 >> 16)};
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int d = 128 * v + 4 * l32;
-      const u32 w0 = E::pack2(acc[v][0] * inv, acc[v][1] * inv), w1 = E::pack2(acc[v][2] * inv, acc[v][3] * inv);
-      FE_GLOBAL u16* op = a.out + at * a.D + d;
-      if (a.D % 4 == 0) {
-        if (d < a.D) *(FE_GLOBAL u32x2*)op = (u32x2){w0, w1};
-      } else {
-        const u16 h[4] = {(u16)w0, (u16)(w0 >> 16), (u16)w1, (u16)(w1 >> 16)};
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (d + i < a.D) op[i] = h[i];
-      }
+      for (int i = 0; i < 4; ++i)
+        if (4 * c4 + i < a.D) op[i] = h[i];
     }
-    if (l32 == 0) a.lse[at] = l == 0.f ? kDecNegInf : (m + fast_log2(l)) * kLn2;
+    if (c4 == 0) a.lse[at] = l == 0.f ? kDecNegInf : (m + fast_log2(l)) * kLn2;
     return;
   }
 
-  // importance: a head's R <= kDecLogitRows rows are one segment
-  const int blk = (int)blockIdx.x - a.out_blocks, bh = blk / a.per_head, part = blk - bh * a.per_head;
-  const int b = bh / a.Hkv, hkv = bh - b * a.Hkv;
-  int first, count;
-  dec_slots(a, bh, first, count);
-  const int n = min(max(a.length[bh], 0), a.C), nc = (n + 31) / 32, tiles = dec_tiles<32>(n, a.T);
-  int t = part * 8 + grp;
+  // a head's R <= kDecLogitRows rows, one row block; tiles of 32 keys
+  const int nc = (n + 31) / 32, tiles = dec_tiles<32>(n, a.T), share = dec_split<4>(tiles, a.S), count = (tiles + share - 1) / share;
+  const long long first = (long long)bh * a.S;
+  const int part = (int)blockIdx.x - a.out_blocks, step = 8 * ((int)gridDim.x - a.out_blocks), l32 = tid & 31;
+  int t = part * 8 + (tid >> 5);
+  if (part * 8 >= tiles) return;
   float x[PF], old = 0.f, w = 1.f;          // a tile's first rows of logits; its keys' importance and norms
-  auto fetch = [&]() __attribute__((always_inline)) {
-    if (t >= tiles) return;
-    const DecF32In lp = a.logits + ((long long)bh * a.max_tiles + t) * a.R * 32 + l32;
-#pragma unroll
-    for (int i = 0; i < PF; ++i) x[i] = lp[min(i, a.R - 1) * 32];
-    const int key = t * 32 + l32;
-    if (key < n) {
-      old = a.imp[bh * a.imp_stride + key];
-      if (a.norm) w = a.norm[bh * a.norm_stride + key];
-    }
-  };
-  fetch();
   {
-    const DecF32In ml = a.part_ml + (long long)first * 2 * RS + l32;
-    const bool rv = l32 < a.R;
+    const int row = tid & 15, grp = tid >> 4;
+    const DecF32In ml = a.part_ml + first * 2 * RS + row;
     float m = kDecNegInf, l = 0.f;
-    for (int s = grp; s < count; s += 8) {
-      const float ms = rv ? ml[s * 2 * RS] : kDecNegInf, ls = rv ? ml[s * 2 * RS + RS] : 0.f;
-      const float mn = fmaxf(m, ms), ref = mn == kDecNegInf ? 0.f : mn;
-      l = l * fast_exp2(m - ref) + ls * fast_exp2(ms - ref);
-      m = mn;
+    if (row < a.R) {
+#pragma unroll 1
+      for (int s = grp; s < count; s += 16) {
+        const float ms = ml[(long long)s * 2 * RS], ls = ml[(long long)s * 2 * RS + RS];
+        const float mn = fmaxf(m, ms), ref = mn == kDecNegInf ? 0.f : mn;
+        l = l * fast_exp2(m - ref) + ls * fast_exp2(ms - ref);
+        m = mn;
+      }
     }
-    sm[grp][l32] = m;
-    sl[grp][l32] = l;
+    sm[grp][row] = m;
+    sl[grp][row] = l;
     __syncthreads();
-    if (grp == 0) {
-#pragma unroll
-      for (int i = 1; i < 8; ++i) m = fmaxf(m, sm[i][l32]);
+    if (tid < 16) {
+#pragma unroll 4
+      for (int i = 1; i < 16; ++i) m = fmaxf(m, sm[i][row]);
       const float ref = m == kDecNegInf ? 0.f : m;
       l = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) l += sl[i][l32] * fast_exp2(sm[i][l32] - ref);
+#pragma unroll 4
+      for (int i = 0; i < 16; ++i) l += sl[i][row] * fast_exp2(sm[i][row] - ref);
       // log2 of l and of w = 2^(-decay (T - 1 - t)); rows that see nothing, or are none, give no weight
-      bias[l32] = l == 0.f || !rv ? -kDecNegInf : ref + fast_log2(l) + a.decay_log2 * (float)(a.T - 1 - l32 % a.T);
+      bias[row] = l == 0.f || row >= a.R ? -kDecNegInf : ref + fast_log2(l) + a.decay_log2 * (float)(a.T - 1 - row % a.T);
     }
     __syncthreads();
   }
   const float keep = fast_exp2(-a.decay_log2 * (float)a.T);
-  while (t < tiles) {
+#pragma unroll 1
+  for (; t < tiles; t += step) {
+    const DecF32In lp = a.logits + ((long long)bh * a.max_tiles + t) * a.R * 32 + l32;
+    const int key = t * 32 + l32;
+#pragma unroll
+    for (int i = 0; i < PF; ++i) x[i] = lp[min(i, a.R - 1) * 32];
+    if (key < n) {
+      old = a.imp[bh * a.imp_stride + key];
+      if (a.norm) w = a.norm[bh * a.norm_stride + key];
+    }
     float sum = 0.f;
-    const float o = old, nw = w;
 #pragma unroll
     for (int i = 0; i < PF; ++i) sum += fast_exp2(x[i] - bias[i]);
-    const DecF32In lp = a.logits + ((long long)bh * a.max_tiles + t) * a.R * 32 + l32;
+#pragma unroll 1
     for (int r0 = PF; r0 < a.R; r0 += PF) {
 #pragma unroll
       for (int i = 0; i < PF; ++i) x[i] = lp[min(r0 + i, a.R - 1) * 32];
 #pragma unroll
       for (int i = 0; i < PF; ++i) sum += fast_exp2(x[i] - bias[r0 + i]);
     }
-    const int now = t;
-    t += 8 * a.per_head;
-    fetch();
-    if (now < nc) {
-      const int key = now * 32 + l32;
-      if (key < n) a.imp_out[bh * a.impo_stride + key] = o * keep + (a.norm ? nw : 1.f) * sum;
-    } else {
-      const int u = (now - nc) * 32 + l32;
-      if (u < a.T) {
-        float nu = 1.f;
-        if (a.norm) {
-          const DecIn vp = a.v + b * a.vs[0] + hkv * a.vs[1] + u * a.vs[2];
-          nu = 0.f;
-          for (int d = 0; d < a.D; ++d) nu += fabsf(E::to_f32(vp[d * a.vnc]));
-        }
-        a.new_imp[(long long)bh * a.T + u] = nu * sum;
+    if (t < nc) {
+      if (key < n) a.imp_out[bh * a.impo_stride + key] = old * keep + w * sum;
+    } else if (key - nc * 32 < a.T) {
+      const int u = key - nc * 32;
+      float nu = 1.f;
+      if (a.norm) {
+        const DecIn vp = a.v + b * a.vb + hkv * a.vh + u * a.vn;
+        nu = 0.f;
+#pragma unroll 4
+        for (int d = 0; d < a.D; ++d) nu += fabsf(E::to_f32(vp[d * a.vd]));
       }
+      a.new_imp[(long long)bh * a.T + u] = nu * sum;
     }
   }
-}
-
-// Leading nodes of batch row b's path that name one of the T tokens.
-__device__ __forceinline__ int dec_path_len(const DecArgs& a, int b) {
-  if (!a.path) return a.A;
-  int len = 0;
-  for (int i0 = 0; i0 < a.A; i0 += 64) {
-    const int i = i0 + (int)(threadIdx.x & 63);
-    const int node = i < a.A ? a.path[(long long)b * a.A + i] : -1;
-    const unsigned long long ok = __ballot(node >= 0 && node < a.T);
-    const int run = ok == ~0ull ? 64 : __ffsll(~ok) - 1;
-    len += run;
-    if (run < 64) break;
-  }
-  return __builtin_amdgcn_readfirstlane(len);
 }
 
 // Block (split, KV head, batch row), as decode_few_kernel. Rows r = g * A_b + i of the path, 64 at a time, with their Q in
@@ -1537,7 +1152,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_replay_kernel(co
     }
   }
   n = __builtin_amdgcn_readfirstlane(min(max(n, 0), a.C));
-  const int nc = (n + 31) / 32, tiles = nc + (a.A + 31) / 32, share = dec_few_share(tiles, a.S);
+  const int nc = (n + 31) / 32, tiles = nc + (a.A + 31) / 32, share = dec_split<4>(tiles, a.S);
   const int t0 = (int)blockIdx.x * share, t1 = min(tiles, t0 + share);
   if (t0 >= t1) return;
   const int rend = a.G * na;
@@ -1696,11 +1311,26 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_replay_kernel(co
 template <int DP>
 constexpr int dec_replay_rows() { return DP > 128 ? 32 : 64; }
 
+// Leading nodes of batch row b's path that name one of the T tokens.
+__device__ __forceinline__ int dec_path_len(const DecReplayArgs& a, int b) {
+  if (!a.path) return a.A;
+  int len = 0;
+  for (int i0 = 0; i0 < a.A; i0 += 64) {
+    const int i = i0 + (int)(threadIdx.x & 63);
+    const int node = i < a.A ? a.path[(long long)b * a.A + i] : -1;
+    const unsigned long long ok = __ballot(node >= 0 && node < a.T);
+    const int run = ok == ~0ull ? 64 : __ffsll(~ok) - 1;
+    len += run;
+    if (run < 64) break;
+  }
+  return __builtin_amdgcn_readfirstlane(len);
+}
+
 // Any layout, element by element: a wave takes 32 keys at a time through its own LDS into registers, against the rows'
 // Q in LDS. More rows than that has room for take K again, adding to what the rows before left.
 template <typename E, int DP>
-__global__ __launch_bounds__(256, 2) void decode_replay_elements_kernel(const DecArgs args) {
-  constexpr int NDC = DP / 16, CPR = DP / 8, TILE = 64 * DP, CH = dec_replay_rows<DP>();
+__global__ __launch_bounds__(256, 2) void decode_replay_elements_kernel(const DecReplayArgs a) {
+  constexpr int NDC = DP / 16, CPR = DP / 8, TILE = 64 * DP, CH = DP > 128 ? 32 : 64;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[4][TILE];
   __shared__ __attribute__((aligned(1024))) unsigned char lds_q[CH * DP * 2];
   __shared__ __attribute__((aligned(16))) float bias[CH];
@@ -1708,20 +1338,17 @@ __global__ __launch_bounds__(256, 2) void decode_replay_elements_kernel(const De
   const int lane = threadIdx.x & 63, l32 = lane & 31, hh = lane >> 5;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
-  const DecArgs a = dec_hold<kDecReplayArgs, 5>(args);
-  DecShare sh = dec_share<32, 4>(a, 1, a.A);
-  while (sh.pos < sh.hi) {
-    const int bh = sh.bh, b = bh / a.Hkv, hkv = bh - b * a.Hkv;
-    const int n = dec_share_len(sh);
-    const int nc = (n + 31) / 32, tiles = dec_tiles<32>(n, a.A);
-    const int t0 = sh.pos - sh.base, t1 = min(tiles, t0 + sh.hi - sh.pos);
-    sh.pos += t1 - t0;
-    if (t1 == tiles) dec_share_next(a, sh);
+  const int hkv = (int)blockIdx.y, b = (int)blockIdx.z, bh = b * (int)gridDim.y + hkv;
+  const int n = __builtin_amdgcn_readfirstlane(min(max(a.length[bh], 0), a.C));
+  const int nc = (n + 31) / 32, tiles = dec_tiles<32>(n, a.A), share = dec_split<4>(tiles, a.S);
+  const int t0 = (int)blockIdx.x * share, t1 = min(tiles, t0 + share);
+  if (t0 >= t1) return;
+  {
     const int na = dec_path_len(a, b), rows = a.G * na;
     const DecI32In path = a.path ? a.path + (long long)b * a.A : (DecI32In) nullptr;
     const float keep = fast_exp2(-a.decay_log2 * (float)na);
 
-    const DecRows hr = dec_rows(a, b, hkv);
+    const DecIn kc = a.kc + b * a.kcb + hkv * a.kch, kn = a.k + b * a.kb + hkv * a.kh, vn = a.v + b * a.vb + hkv * a.vh;
     for (int r0 = 0; r0 == 0 || r0 < rows; r0 += CH) {
       __syncthreads();                      // the rows before are done with
       for (int i = threadIdx.x; i < CH; i += 256) {
@@ -1731,7 +1358,7 @@ __global__ __launch_bounds__(256, 2) void decode_replay_elements_kernel(const De
         if (r < rows) {
           const int g = r / na, node = path ? path[r - g * na] : r - g * na;
           at = r - g * na;
-          const float z = a.lse_in[((long long)b * a.Hkv * a.G + hkv * a.G + g) * a.T + node];
+          const float z = a.lse[((long long)bh * a.G + g) * a.T + node];
           // nothing visible (lse = -inf): the row gives no weight
           if (z != kDecNegInf) bs = z * (1.f / kLn2) + a.decay_log2 * (float)(na - 1 - at);
         }
@@ -1744,7 +1371,7 @@ __global__ __launch_bounds__(256, 2) void decode_replay_elements_kernel(const De
         u32x4 x = {0u, 0u, 0u, 0u};
         if (r < rows) {
           const int g = r / na, node = path ? path[r - g * na] : r - g * na;
-          const DecIn qp = a.q + b * a.qs[0] + (hkv * a.G + g) * a.qs[1] + node * a.qs[2];
+          const DecIn qp = a.q + b * a.qb + (long long)(hkv * a.G + g) * a.qh + node * a.qn;
           x = (dec_load8(qp, a.qc, ch, a.D) & a.qand) ^ a.qxor;
         }
         *(u32x4*)(lds_q + dec_k_at<DP>(e / CPR, ch)) = x;
@@ -1756,8 +1383,8 @@ __global__ __launch_bounds__(256, 2) void decode_replay_elements_kernel(const De
         const bool tail = t >= nc;
         const int kb = tail ? (t - nc) * 32 : t * 32, krows = tail ? na : n;
         {
-          const DecIn kp = tail ? hr.k : hr.kc;
-          const long long krs = tail ? hr.ks : hr.kcs, kcs = tail ? a.knc : a.kcc;
+          const DecIn kp = tail ? kn : kc;
+          const long long krs = tail ? a.kn64 : a.kcn64, kcs = tail ? a.kd : a.kcd;
 #pragma unroll 1
           for (int i = 0; i < NDC; ++i) {
             const int e = i * 64 + lane, key = kb + e / CPR, ch = e % CPR;
@@ -1801,9 +1428,9 @@ __global__ __launch_bounds__(256, 2) void decode_replay_elements_kernel(const De
           if (key < na) {
             w = 1.f;
             if (a.norm) {
-              const DecIn vp = hr.v + (path ? path[key] : key) * hr.vs;
+              const DecIn vp = vn + (path ? path[key] : key) * a.vn64;
               w = 0.f;
-              for (int d = 0; d < a.D; ++d) w += fabsf(E::to_f32(vp[d * a.vnc]));
+              for (int d = 0; d < a.D; ++d) w += fabsf(E::to_f32(vp[d * a.vd]));
             }
           }
           const DecF32 to = a.new_imp + (long long)bh * a.A + key;
@@ -1816,18 +1443,17 @@ __global__ __launch_bounds__(256, 2) void decode_replay_elements_kernel(const De
 
 #define FE_DEC_DIMS(X) X(64) X(96) X(128) X(192) X(256)
 #define FE_DEC_ROW(DP, E, T)                                                                                            \
-  {DP, T, {(const void*)decode_few_kernel<E, DP>, (const void*)decode_few_join_kernel<E, DP>}, {(const void*)decode_rows_kernel<E, DP, 0>, (const void*)decode_rows_kernel<E, DP, 1>},                       \
-   {(const void*)decode_wide_kernel<E, DP, 4>, (const void*)decode_wide_kernel<E, DP, (DP > 128 ? 4 : 8)>},              \
-   (const void*)decode_join_kernel<E, DP>,                                                                              \
+  {DP, T, {(const void*)decode_few_kernel<E, DP, 1>, (const void*)decode_few_kernel<E, DP, 2>},                         \
+   {(const void*)decode_wide_kernel<E, DP, 4>, (const void*)decode_wide_kernel<E, DP, (DP > 128 ? 4 : 8)>},             \
+   (const void*)decode_elements_kernel<E, DP>, (const void*)decode_join_kernel<E, DP>,                                  \
    {(const void*)decode_replay_elements_kernel<E, DP>, (const void*)decode_replay_kernel<E, DP>}},
 #define FE_DEC_ROWS(DP) FE_DEC_ROW(DP, F16, FE_DTYPE_F16) FE_DEC_ROW(DP, BF16, FE_DTYPE_BF16)
-// Kernels by tile dim. rows and replay: the second takes operands whose rows all allow 16-byte loads. wide: of four
-// waves, and of eight where their registers allow it.
+// Kernels by tile dim: few of up to 16 and 32 rows, wide of four waves, and of eight where their registers allow it.
 struct DecKernels {
   int dp, dtype;
-  const void* few[2];          // and its join
-  const void* rows[2];
+  const void* few[2];
   const void* wide[2];
+  const void* elements;
   const void* join;
   const void* replay[2];
 };
@@ -1841,10 +1467,10 @@ const DecKernels& dec_kernels(int64_t D, int dtype) {
 
 void append_decode_resources(std::string& out) {
   for (const auto& e : kDecKernels) {
-    const void* fns[9] = {e.rows[1], e.wide[0], e.wide[1], e.join, e.replay[1], e.rows[0], e.replay[0], e.few[0], e.few[1]};
-    const char* names[9] = {"decode_rows", "decode_wide4", "decode_wide8", "decode_join", "decode_replay", "decode_rows_elements", "decode_replay_elements", "decode_few", "decode_few_join"};
-    for (int i = 0; i < 9; ++i) {
-      if (i == 2 && e.dp > 128) continue;
+    const void* fns[8] = {e.few[0], e.few[1], e.wide[0], e.wide[1], e.join, e.replay[1], e.elements, e.replay[0]};
+    const char* names[8] = {"decode_few16", "decode_few32", "decode_wide4", "decode_wide8", "decode_join", "decode_replay", "decode_elements", "decode_replay_elements"};
+    for (int i = 0; i < 8; ++i) {
+      if (i == 3 && e.dp > 128) continue;
       hipFuncAttributes attr;
       if (hipFuncGetAttributes(&attr, fns[i]) != hipSuccess) continue;
       char buf[512];
@@ -1860,10 +1486,11 @@ void append_decode_resources(std::string& out) {
 
 namespace {
 
-// 16-byte loads of rows: unit channel stride, channels in whole 16-byte chunks, every row on a 16-byte boundary.
+// 16-byte loads of rows: unit channel stride, channels in whole 16-byte chunks, every row on a 16-byte boundary, and
+// row strides of 31 bits.
 bool vec_ok(const void* p, const long long (&st)[4], int64_t B, int64_t H, int64_t N, int64_t D) {
   return D % 8 == 0 && st[3] == 1 && (uintptr_t)p % 16 == 0 && (B <= 1 || st[0] % 8 == 0) && (H <= 1 || st[1] % 8 == 0) &&
-         (N <= 1 || st[2] % 8 == 0);
+         (N <= 1 || (st[2] % 8 == 0 && st[2] <= 0x7fffffffLL));
 }
 
 int dec_check(const char* who, int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t C, int64_t D, int dtype, float scale,
@@ -1881,9 +1508,8 @@ int dec_check(const char* who, int64_t B, int64_t Hq, int64_t Hkv, int64_t T, in
     set_error(w + ": scale must be finite, recency_decay finite and nonnegative");
     return FE_ERR_INVALID;
   }
-  const int64_t most = std::max<int64_t>((Hq / Hkv * T + 31) / 32, 1);   // segments of a head
-  if (C > (1LL << 30) || Hq / Hkv > 32767 || B > (1LL << 30) || Hkv > (1LL << 30) || B * Hkv > (1LL << 24) ||
-      B * Hkv * most > 0x7fffffLL || (double)(B * Hkv * most) * (double)((C + 31) / 32 + (T + 31) / 32) > 2147483647.) {
+  // grid axes: KV heads, and batch rows times blocks of at least 32 rows
+  if (C > (1LL << 30) || Hkv > 65535 || B > 65535 || Hq / Hkv > 32767 || B * ((Hq / Hkv * T + 31) / 32) > 65535) {
     set_error(w + ": sizes exceed the supported range");
     return FE_ERR_UNSUPPORTED;
   }
@@ -1907,48 +1533,31 @@ int dec_strides(const char* who, const int64_t* const* in, long long (*out)[4], 
   return FE_OK;
 }
 
-// How an attention launch is laid out; the same for the workspace's size and the call, whatever the layout of rows.
+// How an attention launch is laid out; the same for the workspace's size and the call.
 struct DecPlan {
-  bool few, wide;
-  int S;                       // splits of a head (few)
-  int RS;                      // rows of a slot
-  int waves, RB, RW, nb;       // waves of a wide block; segments of a head, 32-row tiles of one, blocks
-  long long slots;
-  size_t o, ml, seg, logits, bytes;   // offsets
+  int kind;                    // 0: elements, 1: few, 2: wide
+  int waves, RB, RS, S;        // waves of a wide block; row blocks of a head, rows of one, splits
+  size_t o, ml, logits, bytes; // offsets
 };
-DecPlan dec_plan(int64_t BH, int64_t R, int64_t C, int64_t T, int64_t DP, bool vec, bool near, bool weights) {
+DecPlan dec_plan(int64_t BH, int64_t R, int64_t C, int64_t T, int64_t DP, bool vec, bool weights) {
   DecPlan p = {};
   const int64_t RT = (R + 31) / 32;
-  p.few = vec && near && R <= 16;
-  p.wide = vec && near && RT > 1;
-  if (p.wide) {
-    p.waves = DP > 128 || RT <= 4 ? 4 : 8;
-    p.RB = (int)((RT + p.waves - 1) / p.waves);
-    p.RW = (int)((RT + p.RB - 1) / p.RB);
-  } else {
-    p.RB = (int)RT;
-    p.RW = 1;
-  }
-  // As many blocks as the card holds at once, of at least a tile a wave.
-  const int64_t KT = p.wide ? 64 : 32, tiles = BH * p.RB * ((C + KT - 1) / KT + (T + KT - 1) / KT);
-  const int64_t resident = p.wide ? (p.waves == 8 || DP > 128 ? 256 : 512) : (DP > 128 ? 256 : 512);
-  p.nb = (int)std::max<int64_t>(1, std::min(resident, p.wide ? tiles : (tiles + 3) / 4));
-  p.slots = p.nb + BH * p.RB;
-  p.RS = 32 * p.RW;
-  if (p.few) {
-    p.S = (int)std::max<int64_t>(1, std::min(resident / BH, (tiles / BH + 3) / 4));
-    p.nb = (int)(p.S * BH);
-    p.slots = p.nb;
-    p.RS = 16;
-  }
+  p.kind = !vec ? 0 : RT == 1 ? 1 : 2;
+  p.waves = DP > 128 || RT <= 4 ? 4 : 8;
+  p.RB = (int)(p.kind == 2 ? (RT + p.waves - 1) / p.waves : RT);
+  p.RS = (int)(p.kind == 2 ? 32 * ((RT + p.RB - 1) / p.RB) : p.kind == 1 && R <= 16 ? 16 : 32);
+  // as many blocks as the card holds at once, of at least a tile a wave
+  const int64_t KT = p.kind == 2 ? 64 : 32, tiles = (C + KT - 1) / KT + (T + KT - 1) / KT;
+  const int64_t resident = DP > 128 || (p.kind == 2 && p.waves == 8) ? 256 : 512;
+  p.S = (int)std::max<int64_t>(1, std::min(resident / (BH * p.RB), p.kind == 2 ? tiles : (tiles + 3) / 4));
   auto area = [&](size_t elems) {
     const size_t at = p.bytes;
     p.bytes += (elems * 4 + 255) / 256 * 256;
     return at;
   };
-  p.o = area((size_t)p.slots * p.RS * DP);
-  p.ml = area((size_t)p.slots * p.RS * 2);
-  p.seg = area((size_t)BH * p.RB * 2);
+  const size_t slots = (size_t)BH * p.RB * p.S;
+  p.o = area(slots * p.RS * DP);
+  p.ml = area(slots * p.RS * 2);
   p.logits = p.bytes;
   if (weights && R <= kDecLogitRows) area((size_t)BH * ((C + 31) / 32 + (T + 31) / 32) * R * 32);
   return p;
@@ -1965,44 +1574,44 @@ int dec_launch(const char* who, const void* fn, dim3 grid, dim3 block, A& a, hip
   return FE_OK;
 }
 
-// st: strides of q, k, v and the K cache.
-int dec_replay(const char* who, const DecKernels& kn, bool vec, DecArgs& a, int64_t B, const long long (*st)[4], hipStream_t stream) {
-  const long long max_tiles = (a.C + 31) / 32 + (a.A + 31) / 32;
-  if (vec && std::max({st[1][2], st[2][2], st[3][2]}) <= 0x7fffffffLL && a.Hkv <= 65535 && B <= 65535) {
-    DecReplayArgs r = {};
-    r.q = a.q;
-    r.k = a.k;
-    r.v = a.v;
-    r.kc = a.kc;
-    r.length = a.length;
-    r.path = a.path;
-    r.lse = a.lse_in;
-    r.imp = a.imp;
-    r.norm = a.norm;
-    r.imp_out = a.imp_out;
-    r.new_imp = a.new_imp;
-    r.qb = st[0][0], r.qh = st[0][1], r.qn = st[0][2];
-    r.kb = st[1][0], r.kh = st[1][1], r.kn = (u32)st[1][2];
-    r.vb = st[2][0], r.vh = st[2][1], r.vn = (u32)st[2][2];
-    r.kcb = st[3][0], r.kch = st[3][1], r.kcn = (u32)st[3][2];
-    r.imp_stride = a.imp_stride;
-    r.norm_stride = a.norm_stride;
-    r.impo_stride = a.impo_stride;
-    r.T = a.T;
-    r.C = a.C;
-    r.D = a.D;
-    r.G = a.G;
-    r.A = a.A;
-    r.qand = a.qand;
-    r.qxor = a.qxor;
-    r.scale_log2 = a.scale_log2;
-    r.decay_log2 = a.decay_log2;
-    // as many blocks as the card holds at once, of at least a tile a wave
-    r.S = (int)std::max<long long>(1, std::min<long long>((kn.dp > 128 ? 256 : 512) / a.BH, (max_tiles + 3) / 4));
-    return dec_launch(who, kn.replay[1], dim3((unsigned)r.S, (unsigned)a.Hkv, (unsigned)B), dim3(256), r, stream);
-  }
-  a.nb = (int)std::max<long long>(1, std::min<long long>(512, ((long long)a.BH * max_tiles + 3) / 4));
-  return dec_launch(who, kn.replay[0], dim3((unsigned)a.nb), dim3(256), a, stream);
+template <typename P, typename Q>
+void dec_set(P& to, Q* from) { to = (P)(uintptr_t)from; }
+
+// A negative scale runs as |scale| on -Q, a zero one as 1 on zeros (a masked logit, -inf, times a zero scale would be
+// NaN).
+template <typename A>
+void dec_scale(A& a, float scale) {
+  a.qand = scale == 0.f ? 0u : ~0u;
+  a.qxor = scale < 0.f ? 0x80008000u : 0u;
+  a.scale_log2 = scale == 0.f ? 1.f : (float)(fabs((double)scale) * 1.4426950408889634);
+}
+
+// st: strides of q, k, v and the K cache; a's path, lse, importance and norms set by the caller.
+int dec_replay(const char* who, const DecKernels& kn, DecReplayArgs& a, const void* q, const void* k, const void* v, const void* k_cache,
+               const int32_t* length, const long long (*st)[4], int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t A, int64_t C,
+               int64_t D, float scale, float decay, hipStream_t stream) {
+  const bool vec = vec_ok(q, st[0], B, Hq, T, D) && vec_ok(k, st[1], B, Hkv, T, D) && vec_ok(v, st[2], B, Hkv, T, D) &&
+                   vec_ok(k_cache, st[3], B, Hkv, C, D);
+  dec_set(a.q, q);
+  dec_set(a.k, k);
+  dec_set(a.v, v);
+  dec_set(a.kc, k_cache);
+  dec_set(a.length, length);
+  a.qb = st[0][0], a.qh = st[0][1], a.qn = st[0][2], a.qc = st[0][3];
+  a.kb = st[1][0], a.kh = st[1][1], a.kn = (u32)st[1][2], a.kn64 = st[1][2], a.kd = st[1][3];
+  a.vb = st[2][0], a.vh = st[2][1], a.vn = (u32)st[2][2], a.vn64 = st[2][2], a.vd = st[2][3];
+  a.kcb = st[3][0], a.kch = st[3][1], a.kcn = (u32)st[3][2], a.kcn64 = st[3][2], a.kcd = st[3][3];
+  a.T = (int)T;
+  a.C = (int)C;
+  a.D = (int)D;
+  a.G = (int)(Hq / Hkv);
+  a.A = (int)A;
+  dec_scale(a, scale);
+  a.decay_log2 = (float)((double)decay * 1.4426950408889634);
+  // as many blocks as the card holds at once, of at least a tile a wave
+  const int64_t tiles = (C + 31) / 32 + (A + 31) / 32;
+  a.S = (int)std::max<int64_t>(1, std::min<int64_t>((kn.dp > 128 ? 256 : 512) / (B * Hkv), (tiles + 3) / 4));
+  return dec_launch(who, kn.replay[vec], dim3((unsigned)a.S, (unsigned)Hkv, (unsigned)B), dim3(256), a, stream);
 }
 
 }  // namespace
@@ -2011,47 +1620,12 @@ int dec_replay(const char* who, const DecKernels& kn, bool vec, DecArgs& a, int6
 using namespace fe;
 
 extern "C" size_t fe_decode_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t C, int64_t D, int weights) {
-  if (B < 1 || Hkv < 1 || Hq < Hkv || T < 1 || C < 1 || D < 1 || D > 256 || T > kDecMaxTokens || B > (1LL << 24) ||
-      Hkv > (1LL << 24) || Hq > (1LL << 24) || C > (1LL << 30) || B * Hkv > (1LL << 24) ||
-      B * Hkv * ((Hq / Hkv * T + 31) / 32) > 0x7fffffLL)
+  if (B < 1 || Hkv < 1 || Hq < Hkv || T < 1 || C < 1 || D < 1 || D > 256 || T > kDecMaxTokens || B > 65535 || Hkv > 65535 ||
+      Hq / Hkv > 32767 || C > (1LL << 30) || B * ((Hq / Hkv * T + 31) / 32) > 65535)
     return 0;
   const int64_t dp = dec_kernels(D, 0).dp;
-  size_t bytes = 0;
-  for (int i = 0; i < 3; ++i) bytes = std::max(bytes, dec_plan(B * Hkv, Hq / Hkv * T, C, T, dp, i > 0, i > 1, weights != 0).bytes);
-  return bytes;
-}
-
-template <typename P, typename Q>
-static void dec_set(P& to, Q* from) { to = (P)(uintptr_t)from; }
-
-// What every launch needs. A negative scale runs as |scale| on -Q, a zero one as 1 on zeros (a masked logit, -inf,
-// times a zero scale would be NaN).
-static void dec_common(DecArgs& a, const void* q, const void* k, const void* v, const void* k_cache, const int32_t* length,
-                       const long long (*st)[4], int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t C, int64_t D, float scale,
-                       float decay) {
-  dec_set(a.q, q);
-  dec_set(a.k, k);
-  dec_set(a.v, v);
-  dec_set(a.kc, k_cache);
-  dec_set(a.length, length);
-  std::copy(st[0], st[0] + 3, a.qs);
-  std::copy(st[1], st[1] + 3, a.ks);
-  std::copy(st[2], st[2] + 3, a.vs);
-  std::copy(st[3], st[3] + 3, a.kcs);
-  a.qc = st[0][3];
-  a.knc = st[1][3];
-  a.vnc = st[2][3];
-  a.kcc = st[3][3];
-  a.T = a.A = (int)T;
-  a.C = (int)C;
-  a.D = (int)D;
-  a.G = (int)(Hq / Hkv);
-  a.Hkv = (int)Hkv;
-  a.BH = (int)(B * Hkv);
-  a.qand = scale == 0.f ? 0u : ~0u;
-  a.qxor = scale < 0.f ? 0x80008000u : 0u;
-  a.scale_log2 = scale == 0.f ? 1.f : (float)(fabs((double)scale) * 1.4426950408889634);
-  a.decay_log2 = (float)((double)decay * 1.4426950408889634);
+  return std::max(dec_plan(B * Hkv, Hq / Hkv * T, C, T, dp, false, weights != 0).bytes,
+                  dec_plan(B * Hkv, Hq / Hkv * T, C, T, dp, true, weights != 0).bytes);
 }
 
 extern "C" int fe_decode_attention(const void* q, const void* k, const void* v, const void* k_cache, const void* v_cache,
@@ -2084,167 +1658,88 @@ extern "C" int fe_decode_attention(const void* q, const void* k, const void* v, 
   }
   const bool vec = vec_ok(q, st[0], B, Hq, T, D) && vec_ok(k, st[1], B, Hkv, T, D) && vec_ok(v, st[2], B, Hkv, T, D) &&
                    vec_ok(k_cache, st[3], B, Hkv, C, D) && vec_ok(v_cache, st[4], B, Hkv, C, D);
-  DecArgs a = {};
-  dec_common(a, q, k, v, k_cache, length, st, B, Hq, Hkv, T, C, D, scale, recency_decay);
-  dec_set(a.vc, v_cache);
-  std::copy(st[4], st[4] + 3, a.vcs);
-  a.vcc = st[4][3];
-  dec_set(a.tree, tree);
-  a.tree_stride = tree_batch_stride;
-  a.R = a.G * a.T;
-  // the few-rows and wide kernels take 32-bit row strides, the former heads and batch rows as grid axes
-  const bool near = std::max({st[1][2], st[2][2], st[3][2], st[4][2]}) <= 0x7fffffffLL && Hkv <= 65535 && B <= 65535;
-  const DecPlan p = dec_plan(a.BH, a.R, C, T, kn.dp, vec, near, importance != nullptr);
-  const bool logits = importance && a.R <= kDecLogitRows;
+  const int64_t BH = B * Hkv, R = Hq / Hkv * T;
+  const DecPlan p = dec_plan(BH, R, C, T, kn.dp, vec, importance != nullptr);
+  const bool logits = importance && R <= kDecLogitRows;
   char* ws = (char*)workspace;
-  a.RB = p.RB;
-  a.RW = p.RW;
-  a.nb = p.nb;
-  a.max_tiles = (int)((C + 31) / 32 + (T + 31) / 32);
+  hipStream_t stream = (hipStream_t)hip_stream;
+  DecArgs a = {};
+  dec_set(a.q, q);
+  dec_set(a.k, k);
+  dec_set(a.v, v);
+  dec_set(a.kc, k_cache);
+  dec_set(a.vc, v_cache);
+  dec_set(a.length, length);
+  dec_set(a.tree, tree);
   dec_set(a.part_o, ws + p.o);
   dec_set(a.part_ml, ws + p.ml);
-  dec_set(a.seg, ws + p.seg);
   if (logits) dec_set(a.logits, ws + p.logits);
-  hipStream_t stream = (hipStream_t)hip_stream;
-  if (p.few) {
-    DecFewArgs f = {};
-    f.q = a.q;
-    f.k = a.k;
-    f.v = a.v;
-    f.kc = a.kc;
-    f.vc = a.vc;
-    f.length = a.length;
-    f.tree = a.tree;
-    f.part_o = a.part_o;
-    f.part_ml = a.part_ml;
-    f.logits = a.logits;
-    f.qb = st[0][0], f.qh = st[0][1], f.qn = st[0][2];
-    f.kb = st[1][0], f.kh = st[1][1], f.kn = (u32)st[1][2];
-    f.vb = st[2][0], f.vh = st[2][1], f.vn = (u32)st[2][2];
-    f.kcb = st[3][0], f.kch = st[3][1], f.kcn = (u32)st[3][2];
-    f.vcb = st[4][0], f.vch = st[4][1], f.vcn = (u32)st[4][2];
-    f.tree_stride = tree_batch_stride;
-    f.T = a.T;
-    f.C = a.C;
-    f.D = a.D;
-    f.R = a.R;
-    f.S = p.S;
-    f.max_tiles = a.max_tiles;
-    f.qand = a.qand;
-    f.qxor = a.qxor;
-    f.scale_log2 = a.scale_log2;
-    if (int rc = dec_launch(who, kn.few[0], dim3((unsigned)p.S, (unsigned)Hkv, (unsigned)B), dim3(256), f, stream)) return rc;
-    DecFewJoinArgs o = {};
-    o.part_o = (DecF32In)a.part_o;
-    o.part_ml = (DecF32In)a.part_ml;
-    o.logits = (DecF32In)a.logits;
-    o.length = a.length;
-    dec_set(o.out, out);
-    dec_set(o.lse, lse);
-    dec_set(o.imp, importance);
-    dec_set(o.norm, value_norm);
-    dec_set(o.imp_out, importance_out);
-    dec_set(o.new_imp, new_importance);
-    o.v = a.v;
-    o.imp_stride = importance_stride;
-    o.norm_stride = value_norm_stride;
-    o.impo_stride = importance_out_stride;
-    o.vb = f.vb;
-    o.vh = f.vh;
-    o.vn = f.vn;
-    o.T = a.T;
-    o.C = a.C;
-    o.D = a.D;
-    o.R = a.R;
-    o.S = p.S;
-    o.max_tiles = a.max_tiles;
-    o.decay_log2 = a.decay_log2;
-    const int64_t per = logits ? std::min<int64_t>((a.max_tiles + 7) / 8, std::max<int64_t>(1, kDecJoinBlocks / a.BH)) : 0;
-    return dec_launch(who, kn.few[1], dim3((unsigned)(a.R + per), (unsigned)Hkv, (unsigned)B), dim3(256), o, stream);
-  }
-  if (p.wide) {
-    DecWideArgs f = {};
-    f.q = a.q;
-    f.k = a.k;
-    f.v = a.v;
-    f.kc = a.kc;
-    f.vc = a.vc;
-    f.length = a.length;
-    f.tree = a.tree;
-    f.part_o = a.part_o;
-    f.part_ml = a.part_ml;
-    f.seg = a.seg;
-    f.qb = st[0][0], f.qh = st[0][1], f.qn = st[0][2];
-    f.kb = st[1][0], f.kh = st[1][1], f.kn = (u32)st[1][2];
-    f.vb = st[2][0], f.vh = st[2][1], f.vn = (u32)st[2][2];
-    f.kcb = st[3][0], f.kch = st[3][1], f.kcn = (u32)st[3][2];
-    f.vcb = st[4][0], f.vch = st[4][1], f.vcn = (u32)st[4][2];
-    f.tree_stride = tree_batch_stride;
-    f.T = a.T;
-    f.C = a.C;
-    f.D = a.D;
-    f.G = a.G;
-    f.Hkv = a.Hkv;
-    f.BH = a.BH;
-    f.R = a.R;
-    f.RB = a.RB;
-    f.RW = a.RW;
-    f.nb = a.nb;
-    f.qand = a.qand;
-    f.qxor = a.qxor;
-    f.scale_log2 = a.scale_log2;
-    if (int rc = dec_launch(who, kn.wide[p.waves == 8], dim3((unsigned)p.nb), dim3(64 * p.waves), f, stream)) return rc;
-  } else {
-    if (int rc = dec_launch(who, kn.rows[vec], dim3((unsigned)p.nb), dim3(256), a, stream)) return rc;
-  }
+  a.qb = st[0][0], a.qh = st[0][1], a.qn = st[0][2], a.qc = st[0][3];
+  a.kb = st[1][0], a.kh = st[1][1], a.kn = (u32)st[1][2], a.kn64 = st[1][2], a.kd = st[1][3];
+  a.vb = st[2][0], a.vh = st[2][1], a.vn = (u32)st[2][2], a.vn64 = st[2][2], a.vd = st[2][3];
+  a.kcb = st[3][0], a.kch = st[3][1], a.kcn = (u32)st[3][2], a.kcn64 = st[3][2], a.kcd = st[3][3];
+  a.vcb = st[4][0], a.vch = st[4][1], a.vcn = (u32)st[4][2], a.vcn64 = st[4][2], a.vcd = st[4][3];
+  a.tree_stride = tree_batch_stride;
+  a.T = (int)T;
+  a.C = (int)C;
+  a.D = (int)D;
+  a.R = (int)R;
+  a.RB = p.RB;
+  a.RS = p.RS;
+  a.S = p.S;
+  a.max_tiles = (int)((C + 31) / 32 + (T + 31) / 32);
+  dec_scale(a, scale);
+  if (p.kind == 1) a.scale_log2 = (float)((double)scale * 1.4426950408889634);   // masks after the scale
+  const void* fn = p.kind == 0 ? kn.elements : p.kind == 1 ? kn.few[R > 16] : kn.wide[p.waves == 8];
+  const dim3 grid((unsigned)p.S, (unsigned)Hkv, (unsigned)(B * p.RB));
+  if (int rc = dec_launch(who, fn, grid, dim3(p.kind == 2 ? 64 * p.waves : 256), a, stream)) return rc;
+
   DecJoinArgs o = {};
-  dec_set(o.part_o, ws + p.o);
-  dec_set(o.part_ml, ws + p.ml);
-  dec_set(o.seg, ws + p.seg);
-  o.logits = a.logits;
+  o.part_o = (DecF32In)a.part_o;
+  o.part_ml = (DecF32In)a.part_ml;
+  o.logits = (DecF32In)a.logits;
   o.length = a.length;
   dec_set(o.out, out);
   dec_set(o.lse, lse);
+  dec_set(o.imp, importance);
+  dec_set(o.norm, value_norm);
+  dec_set(o.imp_out, importance_out);
+  dec_set(o.new_imp, new_importance);
   o.v = a.v;
-  std::copy(st[2], st[2] + 3, o.vs);
-  o.vnc = st[2][3];
+  o.imp_stride = importance_stride;
+  o.norm_stride = value_norm_stride;
+  o.impo_stride = importance_out_stride;
+  o.vb = a.vb;
+  o.vh = a.vh;
+  o.vn = a.vn64;
+  o.vd = a.vd;
   o.T = a.T;
   o.C = a.C;
   o.D = a.D;
-  o.G = a.G;
-  o.Hkv = a.Hkv;
-  o.BH = a.BH;
   o.R = a.R;
   o.RB = a.RB;
-  o.RS = p.RS;
+  o.RS = a.RS;
+  o.S = a.S;
   o.max_tiles = a.max_tiles;
-  o.decay_log2 = a.decay_log2;
-  // eight groups on a row where it has many splits, else a group a row
-  const long long rows = (long long)a.BH * a.R;
-  o.split = p.nb >= 8 * a.BH * a.RB ? 8 : 1;
-  o.out_blocks = (int)((rows * o.split + 7) / 8);
-  long long blocks = o.out_blocks;
-  if (importance) {
-    dec_set(a.imp, importance);
-    a.imp_stride = o.imp_stride = importance_stride;
-    dec_set(a.norm, value_norm);
-    a.norm_stride = o.norm_stride = value_norm_stride;
-    dec_set(a.imp_out, importance_out);
-    a.impo_stride = o.impo_stride = importance_out_stride;
-    dec_set(a.new_imp, new_importance);
-    o.imp = a.imp;
-    o.norm = a.norm;
-    o.imp_out = a.imp_out;
-    o.new_imp = a.new_imp;
-  }
-  if (logits) {
-    o.per_head = (int)std::min<long long>((a.max_tiles + 7) / 8, std::max<long long>(1, kDecJoinBlocks / a.BH));
-    blocks += (long long)a.BH * o.per_head;
-  }
-  if (int rc = dec_launch(who, kn.join, dim3((unsigned)blocks), dim3(256), o, stream)) return rc;
+  o.wide = p.kind == 2;
+  o.decay_log2 = (float)((double)recency_decay * 1.4426950408889634);
+  // all of a block's groups of threads on a row where they have slots enough, else one on each
+  const int groups = 256 / (kn.dp / 4);
+  o.rows = 2 * p.S > groups ? 1 : groups;
+  o.out_blocks = (int)((R + o.rows - 1) / o.rows);
+  const int64_t per = logits ? std::min<int64_t>((a.max_tiles + 7) / 8, std::max<int64_t>(1, kDecJoinBlocks / BH)) : 0;
+  if (int rc = dec_launch(who, kn.join, dim3((unsigned)(o.out_blocks + per), (unsigned)Hkv, (unsigned)B), dim3(256), o, stream)) return rc;
   if (!importance || logits) return FE_OK;
-  dec_set(a.lse_in, lse);
-  return dec_replay(who, kn, vec, a, B, st, stream);
+  DecReplayArgs r = {};
+  r.lse = (DecF32In)o.lse;
+  r.imp = o.imp;
+  r.norm = o.norm;
+  r.imp_out = o.imp_out;
+  r.new_imp = o.new_imp;
+  r.imp_stride = importance_stride;
+  r.norm_stride = value_norm_stride;
+  r.impo_stride = importance_out_stride;
+  return dec_replay(who, kn, r, q, k, v, k_cache, length, st, B, Hq, Hkv, T, T, C, D, scale, recency_decay, stream);
 }
 
 extern "C" int fe_replay_path(const void* q, const void* k, const void* v, const void* k_cache, const int32_t* length,
@@ -2272,13 +1767,8 @@ extern "C" int fe_replay_path(const void* q, const void* k, const void* v, const
   const int64_t* in[4] = {q_strides, k_strides, v_strides, k_cache_strides};
   long long st[4][4];
   if (int rc = dec_strides(who, in, st, 4)) return rc;
-  const DecKernels& kn = dec_kernels(D, dtype);
-  const bool vec = vec_ok(q, st[0], B, Hq, T, D) && vec_ok(k, st[1], B, Hkv, T, D) && vec_ok(v, st[2], B, Hkv, T, D) &&
-                   vec_ok(k_cache, st[3], B, Hkv, C, D);
-  DecArgs a = {};
-  dec_common(a, q, k, v, k_cache, length, st, B, Hq, Hkv, T, C, D, scale, recency_decay);
-  a.A = (int)A;
-  dec_set(a.lse_in, lse);
+  DecReplayArgs a = {};
+  dec_set(a.lse, lse);
   dec_set(a.path, path);
   dec_set(a.imp, importance);
   a.imp_stride = importance_stride;
@@ -2287,5 +1777,6 @@ extern "C" int fe_replay_path(const void* q, const void* k, const void* v, const
   dec_set(a.imp_out, importance_out);
   a.impo_stride = importance_out_stride;
   dec_set(a.new_imp, new_importance);
-  return dec_replay(who, kn, vec, a, B, st, (hipStream_t)hip_stream);
+  return dec_replay(who, dec_kernels(D, dtype), a, q, k, v, k_cache, length, st, B, Hq, Hkv, T, A, C, D, scale, recency_decay,
+                    (hipStream_t)hip_stream);
 }
