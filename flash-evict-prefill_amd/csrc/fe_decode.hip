@@ -508,9 +508,8 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void decode_wide_kernel(
   // next one comes in
   constexpr int VB = NW == 8 ? 3 : 2;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[(2 + VB) * TILE];
-  __shared__ u32 s_odd[2][2];            // keys of a tile of new rows with a value that is not finite
+  __shared__ u32 s_odd[kDecMaxTokens / 64][2];   // keys of the tiles of new rows whose value has an infinity or a NaN
   __shared__ u32 s_tree[kDecMaxTokens][2];   // what each query token sees of a tile of new rows
-  __shared__ float s_row[NW][DP];        // a value that is not finite, by each wave
   static_assert((2 + VB) * TILE >= NW * 16 * OST * 4, "16 rows of each wave's output");
   const DecArgs a = dec_hold<0, 4>(args);
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
@@ -562,7 +561,6 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void decode_wide_kernel(
     auto kbuf = [&](int t) -> unsigned char* { return lds + (t & 1) * TILE; };
     auto vbuf = [&](int t) -> unsigned char* { return lds + (2 + t % VB) * TILE; };
     auto store = [&](int t) __attribute__((always_inline)) {
-      const int buf = t & 1;
       unsigned char* kt = kbuf(t);
       unsigned char* vt = vbuf(t);
       const bool nt = t >= nc;
@@ -584,12 +582,12 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void decode_wide_kernel(
         }
       }
       if (nt) {
-        if (tid < 2) s_odd[buf][tid] = 0u;
+        if (tid < 2) s_odd[t - nc][tid] = 0u;
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
           const int key = (i * NT + tid) / CPR;
-          if (key < 64 && dec_nonfinite<E>(vx[i])) atomicOr(&s_odd[buf][key >> 5], 1u << (key & 31));
+          if (key < 64 && dec_nonfinite<E>(vx[i])) atomicOr(&s_odd[t - nc][key >> 5], 1u << (key & 31));
         }
       }
     };
@@ -602,23 +600,13 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void decode_wide_kernel(
     }
     store(t0);
     __syncthreads();
-    u32x4 pf[4];                           // a tile's probabilities, as the product takes them
-    auto product = [&](int t) __attribute__((always_inline)) {
-      unsigned char* vt = vbuf(t);
-#pragma unroll
-      for (int c4 = 0; c4 < 4; ++c4)
-#pragma unroll
-        for (int dt = 0; dt < NDT; ++dt) o[dt] = E::mfma(dec_vfrag<DP>(vt, 16 * c4, dt), pf[c4], o[dt]);
-    };
 #pragma unroll 1
     for (int t = t0; t < t1; ++t) {
       if (t + 1 < t1) load(t + 1);
       {
-        const int buf = t & 1;
         const bool tail = t >= nc;
         const int kb = (tail ? t - nc : t) * 64, rows = tail ? a.T : n;
         unsigned char* kt = kbuf(t);
-        unsigned long long odd = 0;
         if (tail) {
           if (a.tree) {
             // the tile's columns of the mask, a query token a ballot
@@ -629,14 +617,16 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void decode_wide_kernel(
               if (lane < 2) s_tree[u][lane] = (u32)(sees >> (32 * lane));
             }
           }
-          odd = ((unsigned long long)s_odd[buf][1] << 32) | s_odd[buf][0];
+          // 0 * inf would reach the rows that do not see such a key: its value is taken out of the product, and added
+          // to the rows that do after the last tile
+          const unsigned long long odd = ((unsigned long long)s_odd[t - nc][1] << 32) | s_odd[t - nc][0];
           if (odd)
             for (int e = tid; e < 64 * CPR; e += NT)
               if ((odd >> (e / CPR)) & 1u) *(u32x4*)(vbuf(t) + dec_v_at<DP>(e / CPR, e % CPR)) = (u32x4){0u, 0u, 0u, 0u};
           __syncthreads();
         }
+        u32x4 pf[4] = {};                  // the tile's probabilities, as the product takes them
         if (live) {
-          if (late && t > t0) product(t - 1);
           u32 vis[2] = {~0u, ~0u};         // bit 8 (i / 4) + i % 4 of word s: register i of x[s] is of a visible key
           const bool masked = tail || kb + 64 > rows;
           if (masked) {
@@ -697,37 +687,12 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void decode_wide_kernel(
             nm = take ? -mx : nm;
             l *= alpha;
             lr *= alpha;
+            // in place: left to the compiler, every tile copies the accumulators for the rare one that scales them
 #pragma unroll
-            for (int dt = 0; dt < NDT; ++dt) o[dt] *= alpha;
+            for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) asm volatile("v_mul_f32 %0, %1, %0" : "+v"(o[dt][i]) : "v"(alpha));
             exponentials();
-          }
-          if (odd) {
-#pragma unroll 1
-            for (unsigned long long left = odd; left; left &= left - 1) {
-              const int key = __ffsll(left) - 1;
-              // the register that holds the key, in the lanes whose half it is and whose query sees it
-              const int s = key >> 5, reg = 16 * s + 4 * ((key >> 3) & 3) + (key & 3), bit = 8 * ((key >> 3) & 3) + (key & 3);
-              const bool in = ((key >> 2) & 1) == hh && (((s ? vis[1] : vis[0]) >> bit) & 1u);
-              float mine = 0.f;
-#pragma unroll
-              for (int i = 0; i < 32; ++i) mine = i == reg ? x[i >> 4][i & 15] : mine;
-              if (!in) mine = -1.f;
-              const float pk = half_swap_max(mine);      // probabilities are not negative
-              const float nan = half_swap_max(mine != mine ? 1.f : 0.f);
-              const float pr = nan > 0.f ? __builtin_nanf("") : pk;
-              const bool sees = pk >= 0.f || nan > 0.f;
-              const DecIn row = vn + (unsigned long long)(kb + key) * a.vn;
-              for (int ch = lane; ch < DP; ch += 64) s_row[wv][ch] = ch < a.D ? E::to_f32(row[ch]) : 0.f;
-              dec_wave_order();
-#pragma unroll
-              for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                  const float y = s_row[wv][32 * dt + 8 * (i >> 2) + 4 * hh + (i & 3)];
-                  if (sees) o[dt][i] += pr * y;
-                }
-              dec_wave_order();
-            }
           }
           l += ls;
 #pragma unroll
@@ -737,14 +702,59 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void decode_wide_kernel(
               pf[c4][i] = E::pack2(x[c4 >> 1][8 * (c4 & 1) + 2 * i], x[c4 >> 1][8 * (c4 & 1) + 2 * i + 1]);
               lr = E::sum2(pf[c4][i], ones2, lr);
             }
-          if (!late) product(t);
+        }
+        // every wave meets the same barriers, the late ones' before the product
+        if (late) {
+          if (t + 1 < t1) store(t + 1);
+          __syncthreads();
+        }
+        if (live) {
+          unsigned char* vt = vbuf(t);
+#pragma unroll
+          for (int c4 = 0; c4 < 4; ++c4)
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt) o[dt] = E::mfma(dec_vfrag<DP>(vt, 16 * c4, dt), pf[c4], o[dt]);
+        }
+        if (!late) {
+          if (t + 1 < t1) store(t + 1);
+          __syncthreads();
         }
       }
-      if (t + 1 < t1) store(t + 1);
-      __syncthreads();
     }
-
-    if (live && late) product(t1 - 1);
+    if (live) {
+#pragma unroll 1
+      for (int t = max(t0, nc); t < t1; ++t) {
+        const u32 lo = __builtin_amdgcn_readfirstlane(s_odd[t - nc][0]), hi = __builtin_amdgcn_readfirstlane(s_odd[t - nc][1]);
+#pragma unroll 1
+        for (unsigned long long odd = ((unsigned long long)hi << 32) | lo; odd; odd &= odd - 1) {
+          const int u = (t - nc) * 64 + __ffsll(odd) - 1;
+          const DecIn kp = kn + (unsigned long long)u * a.kn, vp = vn + (unsigned long long)u * a.vn;
+          int D = a.D;
+          asm volatile("" : "+s"(D));    // or its comparisons are kept over the loop
+          float x = 0.f;
+#pragma unroll
+          for (int c = 0; c < NDC; ++c) {
+            const int ch = 16 * c + 8 * hh;
+            const u32x4 kk = ch < D ? *(const FE_GLOBAL u32x4*)(kp + ch) : (u32x4){0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              x = __builtin_fmaf(E::to_f32((u16)kk[w]), E::to_f32((u16)qf[c][w]), x);
+              x = __builtin_fmaf(E::to_f32((u16)(kk[w] >> 16)), E::to_f32((u16)(qf[c][w] >> 16)), x);
+            }
+          }
+          const float pr = fast_exp2(half_swap_sum(x) * a.scale_log2 + nm);
+          const bool sees = rv && (a.tree ? a.tree[b * a.tree_stride + tq * a.T + u] != 0 : u <= tq);
+#pragma unroll
+          for (int i = 0; i < 4 * NDT; ++i) {
+            const int ch = 8 * i + 4 * hh;
+            const u32x2 y = ch < D ? *(const FE_GLOBAL u32x2*)(vp + ch) : (u32x2){0u, 0u};
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+              o[i >> 2][4 * (i & 3) + w] += sees ? pr * E::to_f32((u16)(y[w >> 1] >> (16 * (w & 1)))) : 0.f;
+          }
+        }
+      }
+    }
     __syncthreads();                       // LDS is the outputs' from here on
     l = half_swap_sum(l);
     lr = half_swap_sum(lr);
