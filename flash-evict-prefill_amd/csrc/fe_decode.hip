@@ -1143,8 +1143,9 @@ __global__ __launch_bounds__(256) void decode_join_kernel(const DecJoinArgs args
 template <typename E, int DP>
 __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_replay_kernel(const DecReplayArgs args) {
   constexpr int NC = DP / 32, RT = 4, CH = 16 * RT;
-  __shared__ __attribute__((aligned(16))) float bias[CH];
-  __shared__ int place[CH], node[CH];      // a row's index on the path, and its token
+  __shared__ __attribute__((aligned(16))) float bias[4 * CH];
+  __shared__ int place[4 * CH], node[4 * CH];   // a row's index on the path, and its token
+  __shared__ float s_sum[2][4][32];        // a tile's sums of the waves' rows
   const DecReplayArgs a = dec_hold<0, 4>(args);
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, lq = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1162,17 +1163,17 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_replay_kernel(co
     }
   }
   n = __builtin_amdgcn_readfirstlane(min(max(n, 0), a.C));
-  const int nc = (n + 31) / 32, tiles = nc + (a.A + 31) / 32, share = dec_split<4>(tiles, a.S);
+  const int nc = (n + 31) / 32, tiles = nc + (a.A + 31) / 32, share = a.G * a.A > CH ? dec_split<1>(tiles, a.S) : dec_split<4>(tiles, a.S);
   const int t0 = (int)blockIdx.x * share, t1 = min(tiles, t0 + share);
   if (t0 >= t1) return;
-  const int rend = a.G * na;
+  const int rend = a.G * na, ws = rend > CH ? 4 : 1, rw = ws == 4 ? wv * CH : 0;   // the wave's rows in bias, place, node
   const DecIn kc = a.kc + b * a.kcb + hkv * a.kch, kn = a.k + b * a.kb + hkv * a.kh;
   const float keep = fast_exp2(-a.decay_log2 * (float)na);
 
 #pragma unroll 1
-  for (int r0 = 0; r0 == 0 || r0 < rend; r0 += CH) {
+  for (int r0 = 0; r0 == 0 || r0 < rend; r0 += CH * ws) {
     __syncthreads();                        // the rows before are done with
-    if (tid < CH) {
+    if (tid < CH * ws) {
       const int r = r0 + tid;
       float bs = -kDecNegInf;
       int at = 0, nd = 0;
@@ -1192,20 +1193,26 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_replay_kernel(co
     __syncthreads();
     u32x4 qf[RT][NC];
     f32x4 bs[RT];
+    const int mine = rend - r0 - rw;        // rows from the wave's first on
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      if (16 * rt < rend - r0) {
-        const int nd = node[16 * rt + l16];   // a real row in any case
+      if (16 * rt < mine) {
+        const int nd = node[rw + 16 * rt + l16];   // a real row in any case
         const DecIn qp = a.q + b * a.qb + (long long)(hkv * a.G + (nd >> 16)) * a.qh + (nd & 0xffff) * a.qn;
 #pragma unroll
         for (int c = 0; c < NC; ++c) qf[rt][c] = *(const FE_GLOBAL u32x4*)(qp + (DP == a.D || 32 * c + 8 * lq < a.D ? 32 * c + 8 * lq : 0));
-        bs[rt] = *(const f32x4*)(bias + 16 * rt + 4 * lq);
+        bs[rt] = *(const f32x4*)(bias + rw + 16 * rt + 4 * lq);
       }
+    }
+    if (a.D != DP) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) qf[rt][c] &= 32 * c + 8 * lq < a.D ? ~0u : 0u;
     }
     u32x4 kx[2][NC];
     float ox = 0.f, wx = 1.f, old = 0.f, w = 1.f;   // importance and norm of key kb + lane (lanes below 32)
-    int t = -1, next = t0 + wv;
-    bool set = false;
+    int t = -1, next = ws == 4 ? t0 : t0 + wv;
 #pragma unroll 1
     while (true) {
       u32x4 kf[2][NC];
@@ -1245,25 +1252,13 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_replay_kernel(co
           if (a.norm) wx = a.norm[bh * a.norm_stride + key];
         }
       }
-      if (!set) {
-        set = true;
-        if (a.qand != ~0u || a.qxor != 0u || a.D != DP) {
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-              const u32 kept = 32 * c + 8 * lq < a.D ? a.qand : 0u, flip = kept ? a.qxor : 0u;
-              qf[rt][c] = (qf[rt][c] & kept) ^ flip;
-            }
-        }
-      }
       if (t >= 0) {
         const bool tail = t >= nc;
         const int kb = (tail ? t - nc : t) * 32;
         float sum[2] = {0.f, 0.f};
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-          if (16 * rt < rend - r0) {
+          if (16 * rt < mine) {
             // lanes hold keys kb + 16 s + l16; register i holds row 16 rt + 4 lq + i
             f32x4 x[2];
 #pragma unroll
@@ -1274,12 +1269,12 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_replay_kernel(co
             for (int s = 0; s < 2; ++s)
 #pragma unroll
               for (int i = 0; i < 4; ++i) x[s][i] = fast_exp2(x[s][i] * a.scale_log2 - bs[rt][i]);
-            if (tail || 16 * (rt + 1) > rend - r0) {
-              int left = rend - r0;
+            if (tail || 16 * (rt + 1) > mine) {
+              int left = mine;
               asm volatile("" : "+s"(left));   // compared here, not kept as masks across the loop
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                const int rr = 16 * rt + 4 * lq + i, at = place[rr];
+                const int rr = 16 * rt + 4 * lq + i, at = place[rw + rr];
 #pragma unroll
                 for (int s = 0; s < 2; ++s)     // no row, whatever the key; row `at` of the path sees new row u <= at
                   if (rr >= left || (tail && at < kb + 16 * s + l16)) x[s][i] = 0.f;
@@ -1290,9 +1285,17 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_replay_kernel(co
           }
         }
         const float s0 = dec_quad_sum(sum[0]), s1 = dec_quad_sum(sum[1]);
-        const float total = lq == 0 ? s0 : s1;
+        float total = lq == 0 ? s0 : s1;
         const int key = kb + lane;
-        if (!tail) {
+        if (ws == 4) {
+          if (lane < 32) s_sum[t & 1][wv][lane] = total;
+          __syncthreads();
+          const float(&part)[4][32] = s_sum[t & 1];
+          total = (part[0][lane & 31] + part[1][lane & 31]) + (part[2][lane & 31] + part[3][lane & 31]);
+        }
+        if (ws == 4 && wv) {
+          // the first wave's to write
+        } else if (!tail) {
           if (lane < 32 && key < n) a.imp_out[bh * a.impo_stride + key] = old * (r0 ? 1.f : keep) + w * total;
         } else if (lane < 32 && key < a.A) {
           float nu = 1.f;
@@ -1312,7 +1315,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_replay_kernel(co
       }
       if (next >= t1) break;
       t = next;
-      next += 4;
+      next += ws == 4 ? 1 : 4;
     }
   }
 }
@@ -1620,7 +1623,8 @@ int dec_replay(const char* who, const DecKernels& kn, DecReplayArgs& a, const vo
   a.decay_log2 = (float)((double)decay * 1.4426950408889634);
   // as many blocks as the card holds at once, of at least a tile a wave
   const int64_t tiles = (C + 31) / 32 + (A + 31) / 32;
-  a.S = (int)std::max<int64_t>(1, std::min<int64_t>((kn.dp > 128 ? 256 : 512) / (B * Hkv), (tiles + 3) / 4));
+  a.S = (int)std::max<int64_t>(1, std::min<int64_t>((kn.dp > 128 ? 256 : 512) / (B * Hkv), vec && a.G * A > 64 ? tiles : (tiles + 3) / 4));
+  if (vec) a.scale_log2 = (float)((double)scale * 1.4426950408889634);   // masks after the scale
   return dec_launch(who, kn.replay[vec], dim3((unsigned)a.S, (unsigned)Hkv, (unsigned)B), dim3(256), a, stream);
 }
 
