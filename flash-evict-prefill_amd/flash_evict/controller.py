@@ -18,6 +18,12 @@ contract on the installed transformers, so those adapters' callers and tests run
     the prompt ("0.1") or "full".
   * mode "decode": each forward (`use_cache=False`) appends its tokens' K/V to `states`
     and attends over the whole stored cache, so the cache grows after compression.
+  * `decode_budget`, a number of rows, bounds that cache: each layer's K/V go on as a
+    `flash_evict.decode.DecodeCache`, in which new tokens are attended to and scored, and the
+    rows of least importance make room for them (the `decode_recent` newest stay). It
+    continues the importance that `prefill` gave the kept tokens, so it needs a fused
+    prefill and compression (FusedController, StreamingController). None: the cache grows.
+    An addition of this build, as `dynamic_cache()` is.
   * `reset()` clears the states and returns to prefill; `method` and `position_end` are
     kept as the reference's callers set them (RoPE positions here come from position_ids).
   * `dynamic_cache()` hands the stored K/V to transformers as a `DynamicCache` (for
@@ -30,6 +36,7 @@ from torch.nn.attention import SDPBackend, sdpa_kernel
 
 from .baselines import flash_attention, snap_scores, snap_select
 from .cache import gather_tokens
+from .decode import MAX_TOKENS, DecodeCache
 
 # Name of the registered attention implementation (transformers treats names containing
 # "flash" as hub flash-attention kernels, so the name avoids that word).
@@ -90,6 +97,9 @@ class Controller:
         self.method = None
         self.position_end = None
         self.inference_transform = None
+        self.scoring = {}
+        self.decode_budget = None
+        self.decode_recent = 0
         self._layers = [m for m in model.modules() if hasattr(m, "layer_idx") and hasattr(m, "q_proj")]
         for m in self._layers:
             m._flash_evict_controller = self
@@ -127,8 +137,33 @@ class Controller:
         self.states[layer] = {"k": k, "v": v, "snap": snap_scores(q, k, SNAP_WINDOW)}
         return flash_attention(q, k, v)
 
+    def _bound(self, state):
+        """A layer's bounded cache, from the tokens and importance its compression kept."""
+        if "importance" not in state:
+            raise ValueError("decode_budget continues prefill's importance: it needs the fused backend and compression")
+        b, hk, n, d = state["k"].shape
+        if n > self.decode_budget:
+            raise ValueError("decode_budget must not be less than the compressed prompt's budget")
+        cache = DecodeCache(b, hk, d, self.decode_budget, dtype=state["k"].dtype, device=state["k"].device,
+                            recent=self.decode_recent, recency_decay=self.scoring.get("recency_decay", 0.),
+                            value_weighted=self.scoring.get("value_weighted", True))
+        cache.load(state["k"], state["v"], state.pop("importance"), position=state.pop("position"), seen=state.pop("seen"))
+        state["cache"] = cache
+        state["rows"] = n
+        return cache
+
+    def _decode_bounded(self, state, q, k, v, scaling):
+        cache = state["cache"] if "cache" in state else self._bound(state)
+        parts = [cache.decode(q[:, :, i:i + MAX_TOKENS], k[:, :, i:i + MAX_TOKENS], v[:, :, i:i + MAX_TOKENS], scale=scaling)
+                 for i in range(0, q.shape[2], MAX_TOKENS)]
+        state["rows"] = rows = min(cache.budget, state["rows"] + q.shape[2])
+        state["k"], state["v"] = cache.k[:, :, :rows], cache.v[:, :, :rows]
+        return (parts[0] if len(parts) == 1 else torch.cat(parts, 2)).transpose(1, 2)
+
     def _decode_layer(self, layer, q, k, v, scaling):
         state = self.states[layer]
+        if self.decode_budget is not None:
+            return self._decode_bounded(state, q, k, v, scaling)
         state["k"] = torch.cat((state["k"], k), 2)
         state["v"] = torch.cat((state["v"], v), 2)
         keys, vals = state["k"], state["v"]

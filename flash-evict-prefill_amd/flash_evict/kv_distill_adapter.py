@@ -11,7 +11,8 @@ flash_evict/kv_distill_adapter.py:16-67 in anishesg/flash-evict-prefill).
   pool_kernel      SnapKV-style pooling of the importance before top-k
 `compress("fused_<budget>", prompt_length)` keeps, per layer and KV head, the `budget`
 tokens select_tokens picks from that layer's importance and gathers their K/V; any other
-method goes to the baseline Controller. Decoding then grows the compacted cache.
+method goes to the baseline Controller. Decoding then grows the compacted cache, or, with
+`decode_budget` set before the compression, goes on within that many rows.
 """
 from .controller import Controller, compact, parse_budget
 from .prefill import prefill, select_tokens
@@ -23,7 +24,6 @@ class FusedController(Controller):
     def __init__(self, model):
         super().__init__(model)
         self.prefill_backend = "baseline"
-        self.scoring = {}
         self.reserved_recent = 0
         self.pool_kernel = 1
 
@@ -33,6 +33,14 @@ class FusedController(Controller):
         out, importance = prefill(q, k, v, scale=scaling, **self.scoring)
         self.states[layer] = {"k": k, "v": v, "importance": importance}
         return out
+
+    def _compact_fused(self, state, budget):
+        """Down to the kept tokens; with a bounded decode cache to come, their importance too."""
+        importance, n = state["importance"], state["k"].shape[2]
+        keep = self._fused_keep(state, budget)
+        compact(state, keep)
+        if self.decode_budget is not None:
+            state.update(importance=importance.gather(2, keep), position=keep.int(), seen=n)
 
     def _fused_keep(self, state, budget):
         """Kept indices [B, Hkv, budget] of one layer; consumes its importance."""
@@ -46,6 +54,6 @@ class FusedController(Controller):
             return super().compress(method, prompt_length)
         budget = parse_budget(method[len(prefix):], prompt_length)
         for state in self.states.values():
-            compact(state, self._fused_keep(state, budget))
+            self._compact_fused(state, budget)
         self.method = method
         self.mode = "decode"

@@ -7,7 +7,8 @@ soon as that layer's attention has run. The attention output every layer passes 
 exact; only the stored K/V shrink, so the full prompt caches of all layers are never held at
 once. Backends: "fused" (the library's importance, the tokens `compress("fused_<budget>")`
 keeps), "snap" (SnapKV over the last 32 queries) and "full" (nothing dropped).
-`finish_prefill()` switches to decoding, which grows the compacted cache.
+`finish_prefill()` switches to decoding, which grows the compacted cache, or with `decode_budget`
+set before the prompt keeps it within that many rows.
 
 `chunk_mlp(model, chunk_size)` bounds the feed-forward activations of long prompts
 (streaming_adapter.py:30-51).
@@ -42,7 +43,7 @@ class StreamingController(FusedController):
         if self.prefill_backend == "fused":
             out = super()._prefill_layer(layer, q, k, v, scaling)
             state = self.states[layer]
-            compact(state, self._fused_keep(state, budget))
+            self._compact_fused(state, budget)
             return out
         out = flash_attention(q, k, v)
         state = self.states[layer] = {"k": k, "v": v}
