@@ -292,12 +292,14 @@ __global__ __launch_bounds__(1024) void insert_few_kernel(const InsArgs args) {
         const int I = __builtin_amdgcn_readlane((int)wave_inclusive_max(k16 == K ? (u32)(i16 + 1) : 0u), 63) - 1;
 #pragma unroll
         for (int q = 0; q < kInsDraw; ++q) vict[q] = q == r ? I : vict[q];
-        if (r + 1 < e && (I & 1023) == tid) {
-          skey[I] = kKeyDrawn;
-          bk = kKeyDrawn;
-          bi = -1;
-          for (int i = tid; i < M; i += 1024)
-            if (skey[i] <= bk && skey[i] != kKeyDrawn) bk = skey[i], bi = i;
+        if (r + 1 < e && ((I & 1023) >> 6) == wv) {
+          // the wave finds its thread's next, a key to a lane
+          const int i = (I & 1023) + 1024 * lane;
+          u32 k = lane < kInsKeys / 1024 && i < M ? skey[i] : kKeyDrawn;
+          if (i == I) k = skey[i] = kKeyDrawn;
+          const u32 wk2 = (u32)__builtin_amdgcn_readlane((int)wave_inclusive_min(k), 63);
+          const int wi2 = __builtin_amdgcn_readlane((int)wave_inclusive_max(k == wk2 && k != kKeyDrawn ? (u32)(i + 1) : 0u), 63) - 1;
+          if ((I & 1023) == tid) bk = wk2, bi = wi2;
         }
       }
       // a victim below F leaves a hole, in order; a candidate at or past F that is no victim moves, in order; new rows
