@@ -599,10 +599,16 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void decode_wide_kernel(
       qf[c] = (qf[c] & keep) ^ flip;
     }
     store(t0);
+    if (t0 + 1 < t1) load(t0 + 1);
     __syncthreads();
+    // the next tile into LDS, the one behind it on its way
+    auto advance = [&](int t) __attribute__((always_inline)) {
+      if (t + 1 < t1) store(t + 1);
+      if (t + 2 < t1) load(t + 2);
+      __syncthreads();
+    };
 #pragma unroll 1
     for (int t = t0; t < t1; ++t) {
-      if (t + 1 < t1) load(t + 1);
       {
         const bool tail = t >= nc;
         const int kb = (tail ? t - nc : t) * 64, rows = tail ? a.T : n;
@@ -704,10 +710,7 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void decode_wide_kernel(
             }
         }
         // every wave meets the same barriers, the late ones' before the product
-        if (late) {
-          if (t + 1 < t1) store(t + 1);
-          __syncthreads();
-        }
+        if (late) advance(t);
         if (live) {
           unsigned char* vt = vbuf(t);
 #pragma unroll
@@ -715,10 +718,7 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void decode_wide_kernel(
 #pragma unroll
             for (int dt = 0; dt < NDT; ++dt) o[dt] = E::mfma(dec_vfrag<DP>(vt, 16 * c4, dt), pf[c4], o[dt]);
         }
-        if (!late) {
-          if (t + 1 < t1) store(t + 1);
-          __syncthreads();
-        }
+        if (!late) advance(t);
       }
     }
     if (live) {
