@@ -20,7 +20,8 @@
 //   decode_join_kernel     joins the splits of the keys: out and lse; and, where the first kernel left its logits
 //                          (few rows), the importance, whose probabilities need the joined lse
 //   decode_replay_kernel   the importance otherwise: S = Q K^T for the rows that stay, lanes holding keys, so that a
-//                          key's sum over the rows is in-lane: p = exp2(x log2e - bias), the bias holding lse and w
+//                          key's sum over the rows is in-lane: w p = exp2((x - lse) log2e + log2 w); the difference is
+//                          taken in lse's own units, where it rounds once
 //                          (decode_replay_elements_kernel for rows that do not allow 16-byte loads)
 //
 // Lengths are known on the device only: a launch's grid comes from the cache's size, and a head's blocks divide the
@@ -85,9 +86,8 @@ struct DecReplayArgs {
   long long imp_stride, norm_stride, impo_stride;
   u32 kn, vn, kcn;         // row strides
   int T, C, D, G, A, S;
-  u32 qand, qxor;
-  float scale_log2, decay_log2;
-  int pad[6];
+  float scale, decay_log2;
+  int pad[8];
   // element loads: 64-bit row strides, channel strides
   long long kn64, vn64, kcn64, qc, kd, vd, kcd;
 };
@@ -1143,7 +1143,7 @@ __global__ __launch_bounds__(256) void decode_join_kernel(const DecJoinArgs args
 template <typename E, int DP>
 __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_replay_kernel(const DecReplayArgs args) {
   constexpr int NC = DP / 32, RT = 4, CH = 16 * RT;
-  __shared__ __attribute__((aligned(16))) float bias[4 * CH];
+  __shared__ __attribute__((aligned(16))) float lse[4 * CH], weight[4 * CH];   // a row's, and log2 of w
   __shared__ int place[4 * CH], node[4 * CH];   // a row's index on the path, and its token
   __shared__ float s_sum[2][4][32];        // a tile's sums of the waves' rows
   const DecReplayArgs a = dec_hold<0, 4>(args);
@@ -1166,7 +1166,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_replay_kernel(co
   const int nc = (n + 31) / 32, tiles = nc + (a.A + 31) / 32, share = a.G * a.A > CH ? dec_split<1>(tiles, a.S) : dec_split<4>(tiles, a.S);
   const int t0 = (int)blockIdx.x * share, t1 = min(tiles, t0 + share);
   if (t0 >= t1) return;
-  const int rend = a.G * na, ws = rend > CH ? 4 : 1, rw = ws == 4 ? wv * CH : 0;   // the wave's rows in bias, place, node
+  const int rend = a.G * na, ws = rend > CH ? 4 : 1, rw = ws == 4 ? wv * CH : 0;   // the wave's rows in lse, weight, place, node
   const DecIn kc = a.kc + b * a.kcb + hkv * a.kch, kn = a.k + b * a.kb + hkv * a.kh;
   const float keep = fast_exp2(-a.decay_log2 * (float)na);
 
@@ -1175,24 +1175,24 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_replay_kernel(co
     __syncthreads();                        // the rows before are done with
     if (tid < CH * ws) {
       const int r = r0 + tid;
-      float bs = -kDecNegInf;
+      float z = -kDecNegInf;                // no row: no weight
       int at = 0, nd = 0;
       if (r < rend) {
         const int g = r / na;
         at = r - g * na;
         nd = path ? path[at] : at;
-        const float z = a.lse[((long long)bh * a.G + g) * a.T + nd];
-        // nothing visible (lse = -inf): the row gives no weight
-        if (z != kDecNegInf) bs = z * (1.f / kLn2) + a.decay_log2 * (float)(na - 1 - at);
+        z = a.lse[((long long)bh * a.G + g) * a.T + nd];
+        z = z == kDecNegInf ? -kDecNegInf : z;   // nothing visible: no weight
         nd |= g << 16;
       }
-      bias[tid] = bs;
+      lse[tid] = z;
+      weight[tid] = a.decay_log2 * (float)(at + 1 - na);
       place[tid] = at;
       node[tid] = nd;
     }
     __syncthreads();
     u32x4 qf[RT][NC];
-    f32x4 bs[RT];
+    f32x4 zs[RT], lw[RT];
     const int mine = rend - r0 - rw;        // rows from the wave's first on
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -1201,7 +1201,8 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_replay_kernel(co
         const DecIn qp = a.q + b * a.qb + (long long)(hkv * a.G + (nd >> 16)) * a.qh + (nd & 0xffff) * a.qn;
 #pragma unroll
         for (int c = 0; c < NC; ++c) qf[rt][c] = *(const FE_GLOBAL u32x4*)(qp + (DP == a.D || 32 * c + 8 * lq < a.D ? 32 * c + 8 * lq : 0));
-        bs[rt] = *(const f32x4*)(bias + rw + 16 * rt + 4 * lq);
+        zs[rt] = *(const f32x4*)(lse + rw + 16 * rt + 4 * lq);
+        lw[rt] = *(const f32x4*)(weight + rw + 16 * rt + 4 * lq);
       }
     }
     if (a.D != DP) {
@@ -1268,7 +1269,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_replay_kernel(co
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) x[s][i] = fast_exp2(x[s][i] * a.scale_log2 - bs[rt][i]);
+              for (int i = 0; i < 4; ++i) x[s][i] = fast_exp2(__builtin_fmaf(__builtin_fmaf(x[s][i], a.scale, -zs[rt][i]), 1.f / kLn2, lw[rt][i]));
             if (tail || 16 * (rt + 1) > mine) {
               int left = mine;
               asm volatile("" : "+s"(left));   // compared here, not kept as masks across the loop
@@ -1346,7 +1347,7 @@ __global__ __launch_bounds__(256, 2) void decode_replay_elements_kernel(const De
   constexpr int NDC = DP / 16, CPR = DP / 8, TILE = 64 * DP, CH = DP > 128 ? 32 : 64;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[4][TILE];
   __shared__ __attribute__((aligned(1024))) unsigned char lds_q[CH * DP * 2];
-  __shared__ __attribute__((aligned(16))) float bias[CH];
+  __shared__ __attribute__((aligned(16))) float lse[CH], weight[CH];
   __shared__ int place[CH];                 // row's index on the path
   const int lane = threadIdx.x & 63, l32 = lane & 31, hh = lane >> 5;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1366,16 +1367,16 @@ __global__ __launch_bounds__(256, 2) void decode_replay_elements_kernel(const De
       __syncthreads();                      // the rows before are done with
       for (int i = threadIdx.x; i < CH; i += 256) {
         const int r = r0 + i;
-        float bs = -kDecNegInf;
+        float z = -kDecNegInf;              // no row: no weight
         int at = 0;
         if (r < rows) {
           const int g = r / na, node = path ? path[r - g * na] : r - g * na;
           at = r - g * na;
-          const float z = a.lse[((long long)bh * a.G + g) * a.T + node];
-          // nothing visible (lse = -inf): the row gives no weight
-          if (z != kDecNegInf) bs = z * (1.f / kLn2) + a.decay_log2 * (float)(na - 1 - at);
+          z = a.lse[((long long)bh * a.G + g) * a.T + node];
+          z = z == kDecNegInf ? -kDecNegInf : z;   // nothing visible: no weight
         }
-        bias[i] = bs;
+        lse[i] = z;
+        weight[i] = a.decay_log2 * (float)(at + 1 - na);
         place[i] = at;
       }
 #pragma unroll 1
@@ -1385,7 +1386,7 @@ __global__ __launch_bounds__(256, 2) void decode_replay_elements_kernel(const De
         if (r < rows) {
           const int g = r / na, node = path ? path[r - g * na] : r - g * na;
           const DecIn qp = a.q + b * a.qb + (long long)(hkv * a.G + g) * a.qh + node * a.qn;
-          x = (dec_load8(qp, a.qc, ch, a.D) & a.qand) ^ a.qxor;
+          x = dec_load8(qp, a.qc, ch, a.D);
         }
         *(u32x4*)(lds_q + dec_k_at<DP>(e / CPR, ch)) = x;
       }
@@ -1420,9 +1421,9 @@ __global__ __launch_bounds__(256, 2) void decode_replay_elements_kernel(const De
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int rr = rt + 8 * (i >> 2) + 4 * hh + (i & 3);
-            float p = fast_exp2(x[i] * a.scale_log2 - bias[rr]);
+            float p = fast_exp2(__builtin_fmaf(__builtin_fmaf(x[i], a.scale, -lse[rr]), 1.f / kLn2, weight[rr]));
             if (tail && place[rr] < kb + l32) p = 0.f;   // row i of the path sees new row u <= i
-            if (bias[rr] == -kDecNegInf) p = 0.f;        // no row, whatever the key
+            if (lse[rr] == -kDecNegInf) p = 0.f;         // no row, whatever the key
             sum += p;
           }
         }
@@ -1592,8 +1593,7 @@ void dec_set(P& to, Q* from) { to = (P)(uintptr_t)from; }
 
 // A negative scale runs as |scale| on -Q, a zero one as 1 on zeros (a masked logit, -inf, times a zero scale would be
 // NaN).
-template <typename A>
-void dec_scale(A& a, float scale) {
+void dec_scale(DecArgs& a, float scale) {
   a.qand = scale == 0.f ? 0u : ~0u;
   a.qxor = scale < 0.f ? 0x80008000u : 0u;
   a.scale_log2 = scale == 0.f ? 1.f : (float)(fabs((double)scale) * 1.4426950408889634);
@@ -1619,12 +1619,11 @@ int dec_replay(const char* who, const DecKernels& kn, DecReplayArgs& a, const vo
   a.D = (int)D;
   a.G = (int)(Hq / Hkv);
   a.A = (int)A;
-  dec_scale(a, scale);
+  a.scale = scale;
   a.decay_log2 = (float)((double)decay * 1.4426950408889634);
   // as many blocks as the card holds at once, of at least a tile a wave
   const int64_t tiles = (C + 31) / 32 + (A + 31) / 32;
   a.S = (int)std::max<int64_t>(1, std::min<int64_t>((kn.dp > 128 ? 256 : 512) / (B * Hkv), vec && a.G * A > 64 ? tiles : (tiles + 3) / 4));
-  if (vec) a.scale_log2 = (float)((double)scale * 1.4426950408889634);   // masks after the scale
   return dec_launch(who, kn.replay[vec], dim3((unsigned)a.S, (unsigned)Hkv, (unsigned)B), dim3(256), a, stream);
 }
 
