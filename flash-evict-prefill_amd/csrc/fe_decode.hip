@@ -36,6 +36,7 @@
 
 #include "fe_attn.h"
 #include "fe_internal.h"
+#include "fe_radix.h"
 #include "../../include/flash_evict.h"
 
 namespace fe {
@@ -58,7 +59,8 @@ typedef FE_GLOBAL float* DecF32;
 typedef const FE_GLOBAL float* DecF32In;
 typedef const FE_GLOBAL int* DecI32In;
 
-// Attention. Slots are ((b * Hkv + j) * RB + row block) * S + split.
+// Attention. Slots: ((b * Hkv + j) * RB + row block) * S + split; of the wide kernel, block * RB + row block, a head's
+// first block and their number in `heads`.
 struct DecArgs {
   DecIn q, k, v, kc, vc;   // queries, new rows, the cache
   DecI32In length;         // [B * Hkv]
@@ -71,7 +73,9 @@ struct DecArgs {
   int T, C, D, R, RB, RS, S, max_tiles;   // R rows of a group in RB blocks of RS; splits; tiles of a full cache
   u32 qand, qxor;          // Q's sign for a negative scale, Q's zeros for a zero one
   float scale_log2;
-  int pad[3];
+  int Hkv, BH, NB;         // the wide kernel's: all heads; blocks they share, or 0: a block each
+  FE_GLOBAL int* heads;    // [B * Hkv][2]
+  int pad[2];
   // element loads: 64-bit row strides, channel strides
   long long kn64, vn64, kcn64, vcn64, qc, kd, vd, kcd, vcd;
 };
@@ -95,7 +99,7 @@ static_assert(offsetof(DecReplayArgs, pad) <= 4 * 64 && sizeof(DecReplayArgs) >=
 
 struct DecJoinArgs {
   DecF32In part_o, part_ml, logits;
-  DecI32In length;
+  DecI32In length, heads;  // heads: of the wide kernel's slots, or null
   FE_GLOBAL u16* out;      // [B, Hq, T, D]
   DecF32 lse;              // [B, Hq, T]
   DecF32In imp, norm;
@@ -103,11 +107,10 @@ struct DecJoinArgs {
   DecIn v;
   long long imp_stride, norm_stride, impo_stride, vb, vh, vn, vd;
   int T, C, D, R, RB, RS, S, max_tiles;
-  int wide;                // tiles of 64 keys
   int rows;                // output rows of a block: 1, all its threads on it, or a group of threads on each
   int out_blocks;          // of a head
   float decay_log2;
-  int pad[16];
+  int pad[15];
 };
 static_assert(offsetof(DecJoinArgs, pad) <= 4 * 64 && sizeof(DecJoinArgs) >= 4 * 64, "argument window");
 
@@ -517,12 +520,46 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void decode_wide_kernel(
   const bool late = VB == 3 && wv >= 4;
   u32 ones2;
   asm volatile("s_mov_b32 %0, %1" : "=s"(ones2) : "i"(E::kOnes2));
-  const int hkv = (int)blockIdx.y, z = (int)blockIdx.z, b = a.RB == 1 ? z : z / a.RB, rb = z - b * a.RB;
-  const int bh = b * (int)gridDim.y + hkv;
-  const int n = __builtin_amdgcn_readfirstlane(min(max(a.length[bh], 0), a.C));
-  const int nc = (n + 63) / 64, tiles = dec_tiles<64>(n, a.T), share = dec_split<1>(tiles, a.S);
-  const int t0 = (int)blockIdx.x * share, t1 = min(tiles, t0 + share);
-  if (t0 >= t1) return;
+  const int rb = (int)blockIdx.y;
+  int bh = (int)blockIdx.x, n, t0 = 0, t1;
+  if (a.NB) {
+    // A lane has heads `lane` and `lane + 64`. Every block takes `share` tiles of one head, the least that the blocks
+    // suffice for: heads of many tiles get many blocks.
+    int at[2], own[2], end[2];
+    u32 tl[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) at[i] = a.length[min(lane + 64 * i, a.BH - 1)];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      at[i] = min(max(at[i], 0), a.C);
+      tl[i] = lane + 64 * i < a.BH ? (u32)dec_tiles<64>(at[i], a.T) : 0u;
+    }
+    u32 share = ((u32)__builtin_amdgcn_readlane(wave_inclusive_scan((int)(tl[0] + tl[1])), 63) + a.NB - 1) / a.NB;
+    while (true) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) own[i] = (int)((tl[i] + share - 1) / share);
+      end[1] = wave_inclusive_scan(own[0] + own[1]);
+      if (__builtin_amdgcn_readlane(end[1], 63) <= a.NB) break;
+      share += 1 + (share >> 4);            // (ends: at most total / share + BH blocks, and NB >= 2 BH)
+    }
+    end[0] = wave_inclusive_scan(own[0]);
+    end[1] = __builtin_amdgcn_readlane(end[0], 63) + wave_inclusive_scan(own[1]);
+    const unsigned long long in0 = __ballot(end[0] > (int)blockIdx.x), in1 = __ballot(end[1] > (int)blockIdx.x);
+    if (!in1) return;
+    const int which = in0 ? 0 : 1, from = __ffsll(in0 ? in0 : in1) - 1;
+    bh = from + 64 * which;
+    n = __builtin_amdgcn_readlane(which ? at[1] : at[0], from);
+    const int count = __builtin_amdgcn_readlane(which ? own[1] : own[0], from);
+    const int first = __builtin_amdgcn_readlane(which ? end[1] : end[0], from) - count;
+    t0 = ((int)blockIdx.x - first) * (int)share;
+    t1 = min(dec_tiles<64>(n, a.T), t0 + (int)share);
+    if (t0 == 0 && rb == 0 && tid < 2) a.heads[2 * bh + tid] = tid ? count : first;
+  } else {
+    n = __builtin_amdgcn_readfirstlane(min(max(a.length[bh], 0), a.C));
+    t1 = dec_tiles<64>(n, a.T);
+    if (rb == 0 && tid < 2) a.heads[2 * bh + tid] = tid ? 1 : bh;
+  }
+  const int b = bh / a.Hkv, hkv = bh - b * a.Hkv, nc = (n + 63) / 64;
   {
     const int r = rb * a.RS + wv * 32 + l32;
     const bool live = wv * 32 < a.RS && rb * a.RS + wv * 32 < a.R;   // the wave has rows
@@ -758,7 +795,7 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void decode_wide_kernel(
     __syncthreads();                       // LDS is the outputs' from here on
     l = half_swap_sum(l);
     lr = half_swap_sum(lr);
-    const long long slot = ((long long)bh * a.RB + rb) * a.S + blockIdx.x;
+    const long long slot = (long long)blockIdx.x * a.RB + rb;
     if (live) {
       const float inv = lr == 0.f ? 0.f : 1.f / lr;
       if (rv && hh == 0) {
@@ -986,12 +1023,19 @@ __global__ __launch_bounds__(256) void decode_join_kernel(const DecJoinArgs args
   const int RS = a.RS;
   if ((int)blockIdx.x < a.out_blocks) {
     const int grp = tid / LPR, c4 = tid - grp * LPR;
-    const int all = a.wide ? dec_tiles<64>(n, a.T) : dec_tiles<32>(n, a.T);
-    const int share = a.wide ? dec_split<1>(all, a.S) : dec_split<4>(all, a.S), count = (all + share - 1) / share;
     const int row = (int)blockIdx.x * a.rows + (a.rows > 1 ? grp : 0), step = a.rows > 1 ? 1 : NG;
     const bool rv = grp < NG && row < a.R;
     const int rb = a.RB == 1 ? 0 : row / RS;
-    const long long first = ((long long)bh * a.RB + rb) * a.S;
+    long long first = ((long long)bh * a.RB + rb) * a.S, pitch = RS;   // the row's slots: the first, values between them
+    int count;
+    if (a.heads) {
+      first = (long long)a.heads[2 * bh] * a.RB + rb;
+      count = a.heads[2 * bh + 1];
+      pitch = (long long)RS * a.RB;
+    } else {
+      const int all = dec_tiles<32>(n, a.T), share = dec_split<4>(all, a.S);
+      count = (all + share - 1) / share;
+    }
     const DecF32In ml = a.part_ml + first * 2 * RS + (row - rb * RS);
     const DecF32In po = a.part_o + (first * RS + (row - rb * RS)) * DP + 4 * c4;
     float m = kDecNegInf, l = 0.f;
@@ -1003,9 +1047,9 @@ __global__ __launch_bounds__(256) void decode_join_kernel(const DecJoinArgs args
 #pragma unroll
       for (int i = 0; i < PF; ++i) {
         const int s = min(s0 + i * step, count - 1);
-        ms[i] = ml[(long long)s * 2 * RS];
-        ls[i] = ml[(long long)s * 2 * RS + RS];
-        x[i] = *(const FE_GLOBAL f32x4*)(po + (long long)s * RS * DP);
+        ms[i] = ml[s * 2 * pitch];
+        ls[i] = ml[s * 2 * pitch + RS];
+        x[i] = *(const FE_GLOBAL f32x4*)(po + s * pitch * DP);
       }
 #pragma unroll
       for (int i = 0; i < PF; ++i)
@@ -1523,7 +1567,7 @@ int dec_check(const char* who, int64_t B, int64_t Hq, int64_t Hkv, int64_t T, in
     return FE_ERR_INVALID;
   }
   // grid axes: KV heads, and batch rows times blocks of at least 32 rows
-  if (C > (1LL << 30) || Hkv > 65535 || B > 65535 || Hq / Hkv > 32767 || B * ((Hq / Hkv * T + 31) / 32) > 65535) {
+  if (C > (1LL << 30) || Hkv > 65535 || B > 65535 || B * Hkv > (1LL << 30) || Hq / Hkv > 32767 || B * ((Hq / Hkv * T + 31) / 32) > 65535) {
     set_error(w + ": sizes exceed the supported range");
     return FE_ERR_UNSUPPORTED;
   }
@@ -1551,7 +1595,8 @@ int dec_strides(const char* who, const int64_t* const* in, long long (*out)[4], 
 struct DecPlan {
   int kind;                    // 0: elements, 1: few, 2: wide
   int waves, RB, RS, S;        // waves of a wide block; row blocks of a head, rows of one, splits
-  size_t o, ml, logits, bytes; // offsets
+  int NB;                      // blocks (of each row block) that the heads of a wide launch share, or 0
+  size_t o, ml, heads, logits, bytes; // offsets
 };
 DecPlan dec_plan(int64_t BH, int64_t R, int64_t C, int64_t T, int64_t DP, bool vec, bool weights) {
   DecPlan p = {};
@@ -1563,15 +1608,17 @@ DecPlan dec_plan(int64_t BH, int64_t R, int64_t C, int64_t T, int64_t DP, bool v
   // as many blocks as the card holds at once, of at least a tile a wave
   const int64_t KT = p.kind == 2 ? 64 : 32, tiles = (C + KT - 1) / KT + (T + KT - 1) / KT;
   const int64_t resident = DP > 128 || (p.kind == 2 && p.waves == 8) ? 256 : 512;
-  p.S = (int)std::max<int64_t>(1, std::min(resident / (BH * p.RB), p.kind == 2 ? tiles : (tiles + 3) / 4));
+  p.S = (int)std::max<int64_t>(1, std::min(resident / (BH * p.RB), (tiles + 3) / 4));
+  if (p.kind == 2 && BH <= 128 && 2 * BH * p.RB <= resident) p.NB = (int)std::min(resident / p.RB, BH * tiles);
   auto area = [&](size_t elems) {
     const size_t at = p.bytes;
     p.bytes += (elems * 4 + 255) / 256 * 256;
     return at;
   };
-  const size_t slots = (size_t)BH * p.RB * p.S;
+  const size_t slots = p.kind == 2 ? (size_t)(p.NB ? p.NB : BH) * p.RB : (size_t)BH * p.RB * p.S;
   p.o = area(slots * p.RS * DP);
   p.ml = area(slots * p.RS * 2);
+  p.heads = area(p.kind == 2 ? 2 * BH : 0);
   p.logits = p.bytes;
   if (weights && R <= kDecLogitRows) area((size_t)BH * ((C + 31) / 32 + (T + 31) / 32) * R * 32);
   return p;
@@ -1634,7 +1681,7 @@ using namespace fe;
 
 extern "C" size_t fe_decode_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t C, int64_t D, int weights) {
   if (B < 1 || Hkv < 1 || Hq < Hkv || T < 1 || C < 1 || D < 1 || D > 256 || T > kDecMaxTokens || B > 65535 || Hkv > 65535 ||
-      Hq / Hkv > 32767 || C > (1LL << 30) || B * ((Hq / Hkv * T + 31) / 32) > 65535)
+      B * Hkv > (1LL << 30) || Hq / Hkv > 32767 || C > (1LL << 30) || B * ((Hq / Hkv * T + 31) / 32) > 65535)
     return 0;
   const int64_t dp = dec_kernels(D, 0).dp;
   return std::max(dec_plan(B * Hkv, Hq / Hkv * T, C, T, dp, false, weights != 0).bytes,
@@ -1700,11 +1747,15 @@ extern "C" int fe_decode_attention(const void* q, const void* k, const void* v, 
   a.RB = p.RB;
   a.RS = p.RS;
   a.S = p.S;
+  a.Hkv = (int)Hkv;
+  a.BH = (int)BH;
+  a.NB = p.NB;
+  if (p.kind == 2) dec_set(a.heads, ws + p.heads);
   a.max_tiles = (int)((C + 31) / 32 + (T + 31) / 32);
   dec_scale(a, scale);
   if (p.kind == 1) a.scale_log2 = (float)((double)scale * 1.4426950408889634);   // masks after the scale
   const void* fn = p.kind == 0 ? kn.elements : p.kind == 1 ? kn.few[R > 16] : kn.wide[p.waves == 8];
-  const dim3 grid((unsigned)p.S, (unsigned)Hkv, (unsigned)(B * p.RB));
+  const dim3 grid = p.kind == 2 ? dim3((unsigned)(p.NB ? p.NB : BH), (unsigned)p.RB) : dim3((unsigned)p.S, (unsigned)Hkv, (unsigned)(B * p.RB));
   if (int rc = dec_launch(who, fn, grid, dim3(p.kind == 2 ? 64 * p.waves : 256), a, stream)) return rc;
 
   DecJoinArgs o = {};
@@ -1712,6 +1763,7 @@ extern "C" int fe_decode_attention(const void* q, const void* k, const void* v, 
   o.part_ml = (DecF32In)a.part_ml;
   o.logits = (DecF32In)a.logits;
   o.length = a.length;
+  o.heads = (DecI32In)a.heads;
   dec_set(o.out, out);
   dec_set(o.lse, lse);
   dec_set(o.imp, importance);
@@ -1734,11 +1786,10 @@ extern "C" int fe_decode_attention(const void* q, const void* k, const void* v, 
   o.RS = a.RS;
   o.S = a.S;
   o.max_tiles = a.max_tiles;
-  o.wide = p.kind == 2;
   o.decay_log2 = (float)((double)recency_decay * 1.4426950408889634);
   // all of a block's groups of threads on a row where they have slots enough, else one on each
   const int groups = 256 / (kn.dp / 4);
-  o.rows = 2 * p.S > groups ? 1 : groups;
+  o.rows = 2 * (p.kind == 2 ? p.NB / BH : p.S) > groups ? 1 : groups;
   o.out_blocks = (int)((R + o.rows - 1) / o.rows);
   const int64_t per = logits ? std::min<int64_t>((a.max_tiles + 7) / 8, std::max<int64_t>(1, kDecJoinBlocks / BH)) : 0;
   if (int rc = dec_launch(who, kn.join, dim3((unsigned)(o.out_blocks + per), (unsigned)Hkv, (unsigned)B), dim3(256), o, stream)) return rc;

@@ -90,6 +90,28 @@ def test_chunk(case):
     _attend_and_check(q, k, v, kc, vc, length, importance=before)
 
 
+@pytest.mark.parametrize("rows", [(16, 1), (17, 1), (1, 24), (4, 8)], ids=str)
+@pytest.mark.parametrize("d", [64, 72, 96, 128, 192, 250, 256])
+def test_rows_about_a_tile_of_queries(rows, d):
+    """16, 17, 24 and 32 query rows to a KV head in every tile dim, with a length that ends inside a tile."""
+    g, t = rows
+    q, k, v, kc, vc = make(1, 2 * g, 2, t, 300, d, BF if d % 128 else FP, 12, "contiguous")
+    length = torch.tensor([[300, 141]], dtype=torch.int32).cuda()
+    imp, norm = _scores(1, 2, 300, vc, 5)
+    _attend_and_check(q, k, v, kc, vc, length, importance=imp, value_norm=norm, recency_decay=0.05)
+    _attend_and_check(q, k, v, kc, vc, length, scale=-0.3)
+
+
+@pytest.mark.parametrize("b,hk,g,t,c,d", [(9, 8, 8, 5, 150, 64), (17, 8, 9, 4, 70, 64), (1, 2, 5, 120, 900, 64), (2, 1, 3, 256, 257, 192),
+                                          (3, 2, 4, 33, 2500, 80)])
+def test_heads_of_different_lengths_share_the_blocks(b, hk, g, t, c, d):
+    """More than 32 rows a KV head: up to and over 128 heads, several row blocks, few and many tiles a head."""
+    q, k, v, kc, vc = make(b, g * hk, hk, t, c, d, BF, 13)
+    length = _lengths(b, hk, c, 14)
+    imp, norm = _scores(b, hk, c, vc, 15)
+    _attend_and_check(q, k, v, kc, vc, length, importance=imp, value_norm=norm, recency_decay=0.01)
+
+
 TREES = [(1, 8, 2, 2, 40, 64, BF), (2, 8, 2, 13, 100, 128, FP), (1, 28, 4, 64, 333, 128, BF), (2, 4, 2, 61, 64, 80, FP),
          (1, 4, 1, 128, 200, 128, BF), (1, 2, 2, 250, 31, 256, FP), (1, 4, 2, 33, 50, 100, BF)]
 
