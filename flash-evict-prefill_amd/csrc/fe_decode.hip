@@ -12,7 +12,7 @@
 // Counting recency back from the newest token, a prompt's importance continued chunk by chunk is the
 // importance of the whole (fe_prefill's).
 //
-//   decode_few_kernel      up to 32 query rows r = g * T + t of a group, the steps of one or a few tokens: each wave takes
+//   decode_few_kernel      up to 16 query rows r = g * T + t of a group, the steps of one or a few tokens: each wave takes
 //                          32 keys at a time for all of them, S^T = K Q^T and O^T = V^T P^T on MFMA, with the rows' running
 //                          maximum and sum
 //   decode_wide_kernel     more rows: each wave holds 32 of them, the block's waves share tiles of 64 keys in LDS
@@ -47,6 +47,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) dec_s16x4 dec_lds_s16x4;
 
 constexpr int kDecMaxTokens = 256;   // new tokens of a call
+constexpr int kDecFewRows = 16;      // rows of a group, up to which decode_few_kernel takes them
 // Rows of a group up to which the attention leaves its logits for the importance: 8 bytes a row and key, written and
 // read, against the 2 D of reading K again.
 constexpr int kDecLogitRows = 16;
@@ -248,40 +249,35 @@ __device__ __forceinline__ float dec_quad_sum(float x) {
   return half_swap_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
-// Block (split, KV head, batch row), QT tiles of 16 rows. S^T = K Q^T and O^T = V^T P^T with 16 queries in the lanes' low
-// four bits: 32 keys are two accumulators of S^T, whose registers (keys 4 (lane / 16) + i of each) are P^T's operand as
+// Block (split, KV head, batch row). S^T = K Q^T and O^T = V^T P^T with the 16 rows in the lanes' low four bits: 32 keys
+// are two accumulators of S^T, whose registers (keys 4 (lane / 16) + i of each) are P^T's operand as
 // they are; V^T's comes from transposing reads in that key order.
 // What bounds it: HBM where the cache is long (the next 32 keys' K and V are on their way to registers while a wave
 // works on these); where it is short, the reading of its own code and the one round trip to memory, so the loads of
 // a tile appear in the code once, rows past the end are read as the last, and nothing is divided that need not be.
-template <typename E, int DP, int QT>
+template <typename E, int DP>
 __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_few_kernel(const DecArgs args) {
-  constexpr int NC = DP / 32, NT16 = DP / 16, CPR = DP / 8, NL = DP / 16, TILE = 64 * DP, OST = DP + 4, RS = 16 * QT;
-  constexpr int WLDS = QT == 1 ? 2 * TILE : 32 * OST * 4;   // a wave's LDS: a K and a V tile, then its output
+  constexpr int NC = DP / 32, NT16 = DP / 16, CPR = DP / 8, NL = DP / 16, TILE = 64 * DP, OST = DP + 4, RS = 16;
+  constexpr int WLDS = 2 * TILE;         // a wave's LDS: a K and a V tile, then its output
   __shared__ __attribute__((aligned(1024))) unsigned char lds[4][WLDS];
   __shared__ float sm[3][4][RS];
-  static_assert(WLDS >= 2 * TILE && WLDS >= RS * OST * 4 && WLDS >= (32 * RS + DP) * 4, "output, or probabilities and a value, in a wave's tiles");
+  static_assert(WLDS >= RS * OST * 4 && WLDS >= (32 * RS + DP) * 4, "output, or probabilities and a value, in a wave's tiles");
   const DecArgs a = dec_hold<0, 4>(args);
   const int lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hkv = (int)blockIdx.y, b = (int)blockIdx.z, bh = b * (int)gridDim.y + hkv;
   int n = a.length[bh];
-  // this lane's query rows (row 0 where there is none: its results go nowhere)
-  int tq[QT];
-  u32x4 qf[QT][NC];
+  // this lane's query row (row 0 where there is none: its results go nowhere)
+  const int r = l16 < a.R ? l16 : 0, g = a.T == 1 ? r : r / a.T, tq = r - g * a.T;
+  u32x4 qf[NC];
+  {
+    const DecIn qp = a.q + b * a.qb + (long long)(hkv * (a.R / a.T) + g) * a.qh + tq * a.qn;
 #pragma unroll
-  for (int q = 0; q < QT; ++q) {
-    const int r = 16 * q + l16 < a.R ? 16 * q + l16 : 0, g = a.T == 1 ? r : r / a.T;
-    tq[q] = r - g * a.T;
-    const DecIn qp = a.q + b * a.qb + (long long)(hkv * (a.R / a.T) + g) * a.qh + tq[q] * a.qn;
-#pragma unroll
-    for (int c = 0; c < NC; ++c) qf[q][c] = *(const FE_GLOBAL u32x4*)(qp + (DP == a.D || 32 * c + 8 * lq < a.D ? 32 * c + 8 * lq : 0));
+    for (int c = 0; c < NC; ++c) qf[c] = *(const FE_GLOBAL u32x4*)(qp + (DP == a.D || 32 * c + 8 * lq < a.D ? 32 * c + 8 * lq : 0));
   }
   if (a.D != DP) {
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int q = 0; q < QT; ++q) qf[q][c] &= 32 * c + 8 * lq < a.D ? ~0u : 0u;
+    for (int c = 0; c < NC; ++c) qf[c] &= 32 * c + 8 * lq < a.D ? ~0u : 0u;
   }
   const DecIn kc = a.kc + b * a.kcb + hkv * a.kch, vc = a.vc + b * a.vcb + hkv * a.vch;
   const DecIn kn = a.k + b * a.kb + hkv * a.kh, vn = a.v + b * a.vb + hkv * a.vh;
@@ -292,15 +288,10 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_few_kernel(const
 
   unsigned char* kt = lds[wv];
   unsigned char* vt = lds[wv] + TILE;
-  f32x4 o[QT][NT16];
-  float m[QT], l[QT], lr[QT];              // l, lr: of the lane's keys
+  f32x4 o[NT16];
+  float m = kDecNegInf, l = 0.f, lr = 0.f;   // l, lr: of the lane's keys
 #pragma unroll
-  for (int q = 0; q < QT; ++q) {
-    m[q] = kDecNegInf;
-    l[q] = lr[q] = 0.f;
-#pragma unroll
-    for (int i = 0; i < NT16; ++i) o[q][i] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  }
+  for (int i = 0; i < NT16; ++i) o[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
   u32x4 kx[NL] = {}, vx[NL] = {};
   int t = -1, next = t0 + wv;
 #pragma unroll 1
@@ -355,97 +346,83 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_few_kernel(const
           if ((odd >> (e / CPR)) & 1u) *(u32x4*)(vt + dec_v_at<DP>(e / CPR, e % CPR)) = (u32x4){0u, 0u, 0u, 0u};
       }
       dec_wave_order();
-      f32x4 x[QT][2];
+      f32x4 x[2];
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-          if (QT > 1 && c % 4 == 0) __builtin_amdgcn_sched_barrier(0);   // four fragments in flight
           const u32x4 kf = *(const u32x4*)(kt + dec_k_at<DP>(16 * s + l16, 4 * c + lq));
-#pragma unroll
-          for (int q = 0; q < QT; ++q) x[q][s] = dec_mfma16<E>(kf, qf[q][c], c == 0 ? (f32x4){0.f, 0.f, 0.f, 0.f} : x[q][s]);
+          x[s] = dec_mfma16<E>(kf, qf[c], c == 0 ? (f32x4){0.f, 0.f, 0.f, 0.f} : x[s]);
         }
-      u32x4 pf[QT];
-      u32 vis[QT];                          // bit 4 s + i: register i of x[s], key kb + 16 s + 4 lq + i, is visible
+      u32x4 pf;
+      u32 vis = 0xffu;                      // bit 4 s + i: register i of x[s], key kb + 16 s + 4 lq + i, is visible
 #pragma unroll
-      for (int q = 0; q < QT; ++q) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[q][i >> 2][i & 3] *= a.scale_log2;
-        vis[q] = 0xffu;
-        if (tail || kb + 32 > rows) {
-          const FE_GLOBAL unsigned char* row = a.tree + b * a.tree_stride + tq[q] * a.T;
-          vis[q] = 0;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int key = kb + 16 * (i >> 2) + 4 * lq + (i & 3);
-            bool see = key < rows;
-            if (tail) see = see && (a.tree ? row[see ? key : 0] != 0 : key <= tq[q]);
-            vis[q] |= (see ? 1u : 0u) << i;
-            x[q][i >> 2][i & 3] = see ? x[q][i >> 2][i & 3] : kDecNegInf;
-          }
-        }
-        float mn = kDecNegInf;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) mn = fmaxf(mn, x[q][i >> 2][i & 3]);
-        if (QT == 1 && a.logits && l16 < a.R) {
-          const DecF32 lp = a.logits + (((long long)bh * a.max_tiles + t) * a.R + l16) * 32 + 4 * lq;
-          *(FE_GLOBAL f32x4*)lp = x[q][0];
-          *(FE_GLOBAL f32x4*)(lp + 16) = x[q][1];
-        }
-        mn = fmaxf(m[q], dec_quad_max(mn));
-        const float ref = mn == kDecNegInf ? 0.f : mn;
-        const float alpha = fast_exp2(m[q] - ref);
-        m[q] = mn;
-        float ls = 0.f, lrs = 0.f;
+      for (int i = 0; i < 8; ++i) x[i >> 2][i & 3] *= a.scale_log2;
+      if (tail || kb + 32 > rows) {
+        const FE_GLOBAL unsigned char* row = a.tree + b * a.tree_stride + tq * a.T;
+        vis = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          x[q][i >> 2][i & 3] = fast_exp2(x[q][i >> 2][i & 3] - ref);
-          ls += x[q][i >> 2][i & 3];
+          const int key = kb + 16 * (i >> 2) + 4 * lq + (i & 3);
+          bool see = key < rows;
+          if (tail) see = see && (a.tree ? row[see ? key : 0] != 0 : key <= tq);
+          vis |= (see ? 1u : 0u) << i;
+          x[i >> 2][i & 3] = see ? x[i >> 2][i & 3] : kDecNegInf;
         }
+      }
+      float mn = kDecNegInf;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          pf[q][i] = E::pack2(x[q][i >> 1][2 * (i & 1)], x[q][i >> 1][2 * (i & 1) + 1]);
-          lrs += E::to_f32((u16)pf[q][i]) + E::to_f32((u16)(pf[q][i] >> 16));
-        }
-        l[q] = l[q] * alpha + ls;
-        lr[q] = lr[q] * alpha + lrs;
-        if (__ballot(alpha != 1.f)) {
+      for (int i = 0; i < 8; ++i) mn = fmaxf(mn, x[i >> 2][i & 3]);
+      if (a.logits && l16 < a.R) {
+        const DecF32 lp = a.logits + (((long long)bh * a.max_tiles + t) * a.R + l16) * 32 + 4 * lq;
+        *(FE_GLOBAL f32x4*)lp = x[0];
+        *(FE_GLOBAL f32x4*)(lp + 16) = x[1];
+      }
+      mn = fmaxf(m, dec_quad_max(mn));
+      const float ref = mn == kDecNegInf ? 0.f : mn;
+      const float alpha = fast_exp2(m - ref);
+      m = mn;
+      float ls = 0.f, lrs = 0.f;
 #pragma unroll
-          for (int i = 0; i < NT16; ++i) o[q][i] *= alpha;
-        }
+      for (int i = 0; i < 8; ++i) {
+        x[i >> 2][i & 3] = fast_exp2(x[i >> 2][i & 3] - ref);
+        ls += x[i >> 2][i & 3];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        pf[i] = E::pack2(x[i >> 1][2 * (i & 1)], x[i >> 1][2 * (i & 1) + 1]);
+        lrs += E::to_f32((u16)pf[i]) + E::to_f32((u16)(pf[i] >> 16));
+      }
+      l = l * alpha + ls;
+      lr = lr * alpha + lrs;
+      if (__ballot(alpha != 1.f)) {
+#pragma unroll
+        for (int i = 0; i < NT16; ++i) o[i] *= alpha;
       }
 #pragma unroll
       for (int i = 0; i < NT16; ++i) {
-        if (QT > 1 && i % 4 == 0) __builtin_amdgcn_sched_barrier(0);
         // channels 16 i + l16: keys 4 lq .. + 3, then 16 + 4 lq .. + 3
         const int row = 4 * lq + (l16 >> 2);
         unsigned char* p = vt + row * (DP * 2) + ((i >> 1) ^ dec_vswz<DP>(row)) * 64 + 32 * (i & 1) + 8 * (l16 & 3);
         const u32x2 ux = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((dec_lds_s16x4*)(dec_lds_ptr)p));
         const u32x2 uy = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((dec_lds_s16x4*)(dec_lds_ptr)(p + 16 * DP * 2)));
-#pragma unroll
-        for (int q = 0; q < QT; ++q) o[q][i] = dec_mfma16<E>((u32x4){ux[0], ux[1], uy[0], uy[1]}, pf[q], o[q][i]);
+        o[i] = dec_mfma16<E>((u32x4){ux[0], ux[1], uy[0], uy[1]}, pf, o[i]);
       }
       if (odd) {
         dec_wave_order();
         float* sp = (float*)kt;             // [32 keys][RS rows] probabilities (-1: hidden)
         float* val = sp + 32 * RS;          // a value's channels
 #pragma unroll
-        for (int q = 0; q < QT; ++q)
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            sp[(16 * (i >> 2) + 4 * lq + (i & 3)) * RS + 16 * q + l16] = (vis[q] >> i) & 1u ? x[q][i >> 2][i & 3] : -1.f;
+        for (int i = 0; i < 8; ++i) sp[(16 * (i >> 2) + 4 * lq + (i & 3)) * RS + l16] = (vis >> i) & 1u ? x[i >> 2][i & 3] : -1.f;
         for (u32 left = odd; left; left &= left - 1) {
           const int key = __ffs((int)left) - 1;
           for (int ch = lane; ch < DP; ch += 64) val[ch] = ch < a.D ? E::to_f32(vn[(unsigned long long)(kb + key) * a.vn + ch]) : 0.f;
           dec_wave_order();
+          const float p = sp[key * RS + l16];
 #pragma unroll
-          for (int q = 0; q < QT; ++q) {
-            const float p = sp[key * RS + 16 * q + l16];
-#pragma unroll
-            for (int i = 0; i < NT16; ++i) {
-              const f32x4 y = *(const f32x4*)(val + 16 * i + 4 * lq);
-              if (p >= 0.f || p != p) o[q][i] += p * y;
-            }
+          for (int i = 0; i < NT16; ++i) {
+            const f32x4 y = *(const f32x4*)(val + 16 * i + 4 * lq);
+            if (p >= 0.f || p != p) o[i] += p * y;
           }
           dec_wave_order();
         }
@@ -459,17 +436,15 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_few_kernel(const
 
   // join the four waves (waves without a tile have a maximum of -inf and zeros)
   float* mine = (float*)lds[wv];
-#pragma unroll
-  for (int q = 0; q < QT; ++q) {
-    const float ls = dec_quad_sum(l[q]), lrs = dec_quad_sum(lr[q]);
-    if (lq == 0) {
-      sm[0][wv][16 * q + l16] = m[q];
-      sm[1][wv][16 * q + l16] = ls;
-      sm[2][wv][16 * q + l16] = lrs;
-    }
-#pragma unroll
-    for (int i = 0; i < NT16; ++i) *(f32x4*)(mine + (16 * q + l16) * OST + 16 * i + 4 * lq) = o[q][i];
+  l = dec_quad_sum(l);
+  lr = dec_quad_sum(lr);
+  if (lq == 0) {
+    sm[0][wv][l16] = m;
+    sm[1][wv][l16] = l;
+    sm[2][wv][l16] = lr;
   }
+#pragma unroll
+  for (int i = 0; i < NT16; ++i) *(f32x4*)(mine + l16 * OST + 16 * i + 4 * lq) = o[i];
   __syncthreads();
   const long long slot = (long long)bh * a.S + blockIdx.x;
 #pragma unroll 1
@@ -1501,15 +1476,15 @@ __global__ __launch_bounds__(256, 2) void decode_replay_elements_kernel(const De
 
 #define FE_DEC_DIMS(X) X(64) X(96) X(128) X(192) X(256)
 #define FE_DEC_ROW(DP, E, T)                                                                                            \
-  {DP, T, {(const void*)decode_few_kernel<E, DP, 1>, (const void*)decode_few_kernel<E, DP, 2>},                         \
+  {DP, T, (const void*)decode_few_kernel<E, DP>,                                                                        \
    {(const void*)decode_wide_kernel<E, DP, 4>, (const void*)decode_wide_kernel<E, DP, (DP > 128 ? 4 : 8)>},             \
    (const void*)decode_elements_kernel<E, DP>, (const void*)decode_join_kernel<E, DP>,                                  \
    {(const void*)decode_replay_elements_kernel<E, DP>, (const void*)decode_replay_kernel<E, DP>}},
 #define FE_DEC_ROWS(DP) FE_DEC_ROW(DP, F16, FE_DTYPE_F16) FE_DEC_ROW(DP, BF16, FE_DTYPE_BF16)
-// Kernels by tile dim: few of up to 16 and 32 rows, wide of four waves, and of eight where their registers allow it.
+// Kernels by tile dim: wide of four waves, and of eight where their registers allow it.
 struct DecKernels {
   int dp, dtype;
-  const void* few[2];
+  const void* few;
   const void* wide[2];
   const void* elements;
   const void* join;
@@ -1525,10 +1500,10 @@ const DecKernels& dec_kernels(int64_t D, int dtype) {
 
 void append_decode_resources(std::string& out) {
   for (const auto& e : kDecKernels) {
-    const void* fns[8] = {e.few[0], e.few[1], e.wide[0], e.wide[1], e.join, e.replay[1], e.elements, e.replay[0]};
-    const char* names[8] = {"decode_few16", "decode_few32", "decode_wide4", "decode_wide8", "decode_join", "decode_replay", "decode_elements", "decode_replay_elements"};
-    for (int i = 0; i < 8; ++i) {
-      if (i == 3 && e.dp > 128) continue;
+    const void* fns[7] = {e.few, e.wide[0], e.wide[1], e.join, e.replay[1], e.elements, e.replay[0]};
+    const char* names[7] = {"decode_few", "decode_wide4", "decode_wide8", "decode_join", "decode_replay", "decode_elements", "decode_replay_elements"};
+    for (int i = 0; i < 7; ++i) {
+      if (i == 2 && e.dp > 128) continue;
       hipFuncAttributes attr;
       if (hipFuncGetAttributes(&attr, fns[i]) != hipSuccess) continue;
       char buf[512];
@@ -1601,10 +1576,10 @@ struct DecPlan {
 DecPlan dec_plan(int64_t BH, int64_t R, int64_t C, int64_t T, int64_t DP, bool vec, bool weights) {
   DecPlan p = {};
   const int64_t RT = (R + 31) / 32;
-  p.kind = !vec ? 0 : RT == 1 ? 1 : 2;
+  p.kind = !vec ? 0 : R <= kDecFewRows ? 1 : 2;
   p.waves = DP > 128 || RT <= 4 ? 4 : 8;
   p.RB = (int)(p.kind == 2 ? (RT + p.waves - 1) / p.waves : RT);
-  p.RS = (int)(p.kind == 2 ? 32 * ((RT + p.RB - 1) / p.RB) : p.kind == 1 && R <= 16 ? 16 : 32);
+  p.RS = (int)(p.kind == 2 ? 32 * ((RT + p.RB - 1) / p.RB) : p.kind == 1 ? 16 : 32);
   // as many blocks as the card holds at once, of at least a tile a wave
   const int64_t KT = p.kind == 2 ? 64 : 32, tiles = (C + KT - 1) / KT + (T + KT - 1) / KT;
   const int64_t resident = DP > 128 || (p.kind == 2 && p.waves == 8) ? 256 : 512;
@@ -1754,7 +1729,7 @@ extern "C" int fe_decode_attention(const void* q, const void* k, const void* v, 
   a.max_tiles = (int)((C + 31) / 32 + (T + 31) / 32);
   dec_scale(a, scale);
   if (p.kind == 1) a.scale_log2 = (float)((double)scale * 1.4426950408889634);   // masks after the scale
-  const void* fn = p.kind == 0 ? kn.elements : p.kind == 1 ? kn.few[R > 16] : kn.wide[p.waves == 8];
+  const void* fn = p.kind == 0 ? kn.elements : p.kind == 1 ? kn.few : kn.wide[p.waves == 8];
   const dim3 grid = p.kind == 2 ? dim3((unsigned)(p.NB ? p.NB : BH), (unsigned)p.RB) : dim3((unsigned)p.S, (unsigned)Hkv, (unsigned)(B * p.RB));
   if (int rc = dec_launch(who, fn, grid, dim3(p.kind == 2 ? 64 * p.waves : 256), a, stream)) return rc;
 

@@ -33,7 +33,7 @@ typedef FE_GLOBAL u16* InsOut;
 
 constexpr int kInsFew = 256;         // new rows, and evicted ones, of insert_few_kernel
 constexpr int kInsKeys = 32768;      // its candidates (128 KiB of LDS)
-constexpr int kInsDraw = 8;          // victims drawn one by one
+constexpr int kInsDraw = 32;         // victims drawn one by one
 
 struct InsArgs {
   InsIn k, v;
@@ -277,9 +277,7 @@ __global__ __launch_bounds__(1024) void insert_few_kernel(const InsArgs args) {
       }
     }
     if (e <= kInsDraw) {
-      int vict[kInsDraw];
-#pragma unroll
-      for (int r = 0; r < kInsDraw; ++r) vict[r] = 0x7fffffff;
+      int vict = 0x7fffffff;                // lane r: the r-th drawn
 #pragma unroll 1
       for (int r = 0; r < e; ++r) {
         const u32 wk = (u32)__builtin_amdgcn_readlane((int)wave_inclusive_min(bk), 63);
@@ -290,8 +288,7 @@ __global__ __launch_bounds__(1024) void insert_few_kernel(const InsArgs args) {
         const int i16 = red_i[r & 1][lane & 15];
         const u32 K = (u32)__builtin_amdgcn_readlane((int)wave_inclusive_min(k16), 63);
         const int I = __builtin_amdgcn_readlane((int)wave_inclusive_max(k16 == K ? (u32)(i16 + 1) : 0u), 63) - 1;
-#pragma unroll
-        for (int q = 0; q < kInsDraw; ++q) vict[q] = q == r ? I : vict[q];
+        if (lane == r) vict = I;
         if (r + 1 < e && ((I & 1023) >> 6) == wv) {
           // the wave finds its thread's next, a key to a lane
           const int i = (I & 1023) + 1024 * lane;
@@ -304,32 +301,28 @@ __global__ __launch_bounds__(1024) void insert_few_kernel(const InsArgs args) {
       }
       // a victim below F leaves a hole, in order; a candidate at or past F that is no victim moves, in order; new rows
       // below F that are no victims stay
-      if (tid < e) {
-        int mine = 0, hole = 0, before = 0, same = 0;
-#pragma unroll
-        for (int q = 0; q < kInsDraw; ++q) mine = q == tid ? vict[q] : mine;
-#pragma unroll
-        for (int q = 0; q < kInsDraw; ++q) {
-          hole += vict[q] < mine ? 1 : 0;                       // holes before this one (victims below it are below F)
-          before += vict[q] >= F && vict[q] < F + tid ? 1 : 0;  // victims at or past F before candidate F + tid
-          same += vict[q] == F + tid ? 1 : 0;
+      auto drawn = [&](int q) { return __builtin_amdgcn_readlane(vict, q); };
+      if (wv == 0) {
+        int hole = 0, before = 0, same = 0;
+#pragma unroll 1
+        for (int q = 0; q < e; ++q) {
+          const int x = drawn(q);
+          hole += x < vict ? 1 : 0;                       // holes before this one (victims below it are below F)
+          before += x >= F && x < F + lane ? 1 : 0;       // victims at or past F before candidate F + lane
+          same += x == F + lane ? 1 : 0;
         }
-        if (mine < F) s_dst[hole] = mine;
-        if (!same) s_src[tid - before] = F + tid;
+        if (lane < e && vict < F) s_dst[hole] = vict;
+        if (lane < e && !same) s_src[lane - before] = F + lane;
       }
-      int past = 0, fresh = 0;
-#pragma unroll
-      for (int q = 0; q < kInsDraw; ++q) {
-        past += vict[q] >= F && vict[q] < M ? 1 : 0;
-        fresh += vict[q] >= n && vict[q] < F ? 1 : 0;
-      }
+      const int past = __popcll(__ballot(vict >= F && vict < M)), fresh = __popcll(__ballot(vict >= n && vict < F));
       moves = e - past;
       for (int i = tid; i < F - n; i += 1024) {
         int before = 0, same = 0;
-#pragma unroll
-        for (int q = 0; q < kInsDraw; ++q) {
-          before += vict[q] >= n && vict[q] < n + i ? 1 : 0;
-          same += vict[q] == n + i ? 1 : 0;
+#pragma unroll 1
+        for (int q = 0; q < e; ++q) {
+          const int x = drawn(q);
+          before += x >= n && x < n + i ? 1 : 0;
+          same += x == n + i ? 1 : 0;
         }
         if (!same) s_src[kInsFew + i - before] = s_dst[kInsFew + i - before] = n + i;
       }

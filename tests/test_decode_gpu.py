@@ -301,6 +301,17 @@ def test_insert(case, ties):
         _insert_and_check(s, k, v, budget, recent=recent, new_importance=new.cuda() if step else None)
 
 
+@pytest.mark.parametrize("t", [9, 31, 32, 33, 47])
+@pytest.mark.parametrize("room", [0, 3])
+def test_insert_as_many_as_are_drawn_one_by_one(t, room):
+    """Up to 32 evictions, and more; from a full cache and from one with room for some of the rows; ties."""
+    s = _state(2, 2, 1500, 48, BF, 99, torch.tensor([[1500 - room, 1500], [1490, 700]], dtype=torch.int32).cuda(), ties=True)
+    for step in range(2):
+        k, v = seeded_randn((2, 2, t, 48), BF, 92 + step), seeded_randn((2, 2, t, 48), BF, 95 + step)
+        new = torch.randint(0, 4, (2, 2, t), generator=torch.Generator().manual_seed(step)).float()
+        _insert_and_check(s, k, v, 1500, recent=5, new_importance=new.cuda())
+
+
 @pytest.mark.parametrize("ties", [False, True], ids=["", "ties"])
 def test_insert_a_path(ties):
     b, hk, c, d, t = 3, 2, 200, 64, 30
