@@ -92,7 +92,8 @@ struct DecReplayArgs {
   u32 kn, vn, kcn;         // row strides
   int T, C, D, G, A, S;
   float scale, decay_log2;
-  int pad[8];
+  int Hkv, BH, NB;         // all heads; blocks they share, or 0: S for each
+  int pad[5];
   // element loads: 64-bit row strides, channel strides
   long long kn64, vn64, kcn64, qc, kd, vd, kcd;
 };
@@ -220,6 +221,46 @@ __device__ __forceinline__ int dec_tiles(int n, int fresh) { return (n + KT - 1)
 template <int PER>
 __device__ __forceinline__ int dec_split(int tiles, int S) { return ((tiles + PER * S - 1) / (PER * S)) * PER; }
 
+// A block's part of NB blocks that BH <= 128 heads share (NB >= 2 BH): tiles t0 .. t1 - 1 of a head of n rows, which has
+// the blocks first .. first + count - 1. Every block takes `share` tiles (a multiple of per) of one head, the least
+// that the blocks suffice for: long heads get many blocks.
+struct DecPart {
+  int bh, n, t0, t1, first, count;
+};
+template <int KT>
+__device__ __forceinline__ bool dec_assign(DecI32In length, int BH, int C, int fresh, int NB, int per, DecPart& part) {
+  const int lane = threadIdx.x & 63;       // a lane has heads `lane` and `lane + 64`
+  int at[2], own[2], end[2];
+  u32 tl[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) at[i] = length[min(lane + 64 * i, BH - 1)];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    at[i] = min(max(at[i], 0), C);
+    tl[i] = lane + 64 * i < BH ? (u32)dec_tiles<KT>(at[i], fresh) : 0u;
+  }
+  u32 share = ((u32)__builtin_amdgcn_readlane(wave_inclusive_scan((int)(tl[0] + tl[1])), 63) + NB - 1) / NB;
+  share = (share + per - 1) / per * per;
+  while (true) {                            // (ends: total / share + BH blocks are enough)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) own[i] = (int)((tl[i] + share - 1) / share);
+    end[0] = wave_inclusive_scan(own[0]);
+    end[1] = __builtin_amdgcn_readlane(end[0], 63) + wave_inclusive_scan(own[1]);
+    if (__builtin_amdgcn_readlane(end[1], 63) <= NB) break;
+    share += per * (1 + share / (16 * per));
+  }
+  const unsigned long long in0 = __ballot(end[0] > (int)blockIdx.x), in1 = __ballot(end[1] > (int)blockIdx.x);
+  if (!in1) return false;
+  const int from = __ffsll(in0 ? in0 : in1) - 1;
+  part.bh = from + (in0 ? 0 : 64);
+  part.n = __builtin_amdgcn_readlane(in0 ? at[0] : at[1], from);
+  part.count = __builtin_amdgcn_readlane(in0 ? own[0] : own[1], from);
+  part.first = __builtin_amdgcn_readlane(in0 ? end[0] : end[1], from) - part.count;
+  part.t0 = ((int)blockIdx.x - part.first) * (int)share;
+  part.t1 = min(dec_tiles<KT>(part.n, fresh), part.t0 + (int)share);
+  return true;
+}
+
 // Zeros in place of the rows past the last (V: 0 * inf is not 0).
 template <int DP, int NT, int NL>
 __device__ __forceinline__ void dec_cut_rows(int kb, int rows, int tid, u32x4 (&x)[NL]) {
@@ -265,8 +306,17 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_few_kernel(const
   const DecArgs a = dec_hold<0, 4>(args);
   const int lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int hkv = (int)blockIdx.y, b = (int)blockIdx.z, bh = b * (int)gridDim.y + hkv;
-  int n = a.length[bh];
+  int hkv = (int)blockIdx.y, b = (int)blockIdx.z, bh = b * (int)gridDim.y + hkv, n, t0 = 0, t1 = 0;
+  long long slot = (long long)bh * a.S + blockIdx.x;
+  if (a.NB) {
+    DecPart p;
+    if (!dec_assign<32>(a.length, a.BH, a.C, a.T, a.NB, 4, p)) return;
+    bh = p.bh, n = p.n, t0 = p.t0, t1 = p.t1, slot = blockIdx.x;
+    b = bh / a.Hkv, hkv = bh - b * a.Hkv;
+    if (t0 == 0 && threadIdx.x < 2) a.heads[2 * bh + threadIdx.x] = threadIdx.x ? p.count : p.first;
+  } else {
+    n = a.length[bh];
+  }
   // this lane's query row (row 0 where there is none: its results go nowhere)
   const int r = l16 < a.R ? l16 : 0, g = a.T == 1 ? r : r / a.T, tq = r - g * a.T;
   u32x4 qf[NC];
@@ -282,9 +332,12 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_few_kernel(const
   const DecIn kc = a.kc + b * a.kcb + hkv * a.kch, vc = a.vc + b * a.vcb + hkv * a.vch;
   const DecIn kn = a.k + b * a.kb + hkv * a.kh, vn = a.v + b * a.vb + hkv * a.vh;
   n = __builtin_amdgcn_readfirstlane(min(max(n, 0), a.C));
-  const int nc = (n + 31) / 32, tiles = nc + (a.T + 31) / 32, share = dec_split<4>(tiles, a.S);
-  const int t0 = (int)blockIdx.x * share, t1 = min(tiles, t0 + share);
-  if (t0 >= t1) return;
+  const int nc = (n + 31) / 32;
+  if (!a.NB) {
+    const int tiles = nc + (a.T + 31) / 32, share = dec_split<4>(tiles, a.S);
+    t0 = (int)blockIdx.x * share, t1 = min(tiles, t0 + share);
+    if (t0 >= t1) return;
+  }
 
   unsigned char* kt = lds[wv];
   unsigned char* vt = lds[wv] + TILE;
@@ -446,7 +499,6 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_few_kernel(const
 #pragma unroll
   for (int i = 0; i < NT16; ++i) *(f32x4*)(mine + l16 * OST + 16 * i + 4 * lq) = o[i];
   __syncthreads();
-  const long long slot = (long long)bh * a.S + blockIdx.x;
 #pragma unroll 1
   for (int e = threadIdx.x; e < a.R * (DP / 4); e += 256) {
     const int row = e / (DP / 4), ch = 4 * (e % (DP / 4));
@@ -498,37 +550,10 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void decode_wide_kernel(
   const int rb = (int)blockIdx.y;
   int bh = (int)blockIdx.x, n, t0 = 0, t1;
   if (a.NB) {
-    // A lane has heads `lane` and `lane + 64`. Every block takes `share` tiles of one head, the least that the blocks
-    // suffice for: heads of many tiles get many blocks.
-    int at[2], own[2], end[2];
-    u32 tl[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) at[i] = a.length[min(lane + 64 * i, a.BH - 1)];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      at[i] = min(max(at[i], 0), a.C);
-      tl[i] = lane + 64 * i < a.BH ? (u32)dec_tiles<64>(at[i], a.T) : 0u;
-    }
-    u32 share = ((u32)__builtin_amdgcn_readlane(wave_inclusive_scan((int)(tl[0] + tl[1])), 63) + a.NB - 1) / a.NB;
-    while (true) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) own[i] = (int)((tl[i] + share - 1) / share);
-      end[1] = wave_inclusive_scan(own[0] + own[1]);
-      if (__builtin_amdgcn_readlane(end[1], 63) <= a.NB) break;
-      share += 1 + (share >> 4);            // (ends: at most total / share + BH blocks, and NB >= 2 BH)
-    }
-    end[0] = wave_inclusive_scan(own[0]);
-    end[1] = __builtin_amdgcn_readlane(end[0], 63) + wave_inclusive_scan(own[1]);
-    const unsigned long long in0 = __ballot(end[0] > (int)blockIdx.x), in1 = __ballot(end[1] > (int)blockIdx.x);
-    if (!in1) return;
-    const int which = in0 ? 0 : 1, from = __ffsll(in0 ? in0 : in1) - 1;
-    bh = from + 64 * which;
-    n = __builtin_amdgcn_readlane(which ? at[1] : at[0], from);
-    const int count = __builtin_amdgcn_readlane(which ? own[1] : own[0], from);
-    const int first = __builtin_amdgcn_readlane(which ? end[1] : end[0], from) - count;
-    t0 = ((int)blockIdx.x - first) * (int)share;
-    t1 = min(dec_tiles<64>(n, a.T), t0 + (int)share);
-    if (t0 == 0 && rb == 0 && tid < 2) a.heads[2 * bh + tid] = tid ? count : first;
+    DecPart p;
+    if (!dec_assign<64>(a.length, a.BH, a.C, a.T, a.NB, 1, p)) return;
+    bh = p.bh, n = p.n, t0 = p.t0, t1 = p.t1;
+    if (t0 == 0 && rb == 0 && tid < 2) a.heads[2 * bh + tid] = tid ? p.count : p.first;
   } else {
     n = __builtin_amdgcn_readfirstlane(min(max(a.length[bh], 0), a.C));
     t1 = dec_tiles<64>(n, a.T);
@@ -1083,8 +1108,9 @@ __global__ __launch_bounds__(256) void decode_join_kernel(const DecJoinArgs args
   }
 
   // a head's R <= kDecLogitRows rows, one row block; tiles of 32 keys
-  const int nc = (n + 31) / 32, tiles = dec_tiles<32>(n, a.T), share = dec_split<4>(tiles, a.S), count = (tiles + share - 1) / share;
-  const long long first = (long long)bh * a.S;
+  const int nc = (n + 31) / 32, tiles = dec_tiles<32>(n, a.T), share = dec_split<4>(tiles, a.S);
+  const int count = a.heads ? a.heads[2 * bh + 1] : (tiles + share - 1) / share;
+  const long long first = a.heads ? a.heads[2 * bh] : (long long)bh * a.S;
   const int part = (int)blockIdx.x - a.out_blocks, step = 8 * ((int)gridDim.x - a.out_blocks), l32 = tid & 31;
   int t = part * 8 + (tid >> 5);
   if (part * 8 >= tiles) return;
@@ -1168,9 +1194,17 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_replay_kernel(co
   const DecReplayArgs a = dec_hold<0, 4>(args);
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, lq = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int hkv = (int)blockIdx.y, b = (int)blockIdx.z, bh = b * (int)gridDim.y + hkv;
+  int hkv = (int)blockIdx.y, b = (int)blockIdx.z, bh = b * (int)gridDim.y + hkv, n, t0 = 0, t1 = 0;
+  if (a.NB) {
+    DecPart p;
+    if (!dec_assign<32>(a.length, a.BH, a.C, a.A, a.NB, a.G * a.A > CH ? 1 : 4, p)) return;
+    bh = p.bh, n = p.n, t0 = p.t0, t1 = p.t1;
+    b = bh / a.Hkv, hkv = bh - b * a.Hkv;
+  } else {
+    n = a.length[bh];
+  }
   const DecI32In path = a.path ? a.path + (long long)b * a.A : a.path;
-  int n = a.length[bh], na = a.A;
+  int na = a.A;
   if (path) {
     na = 0;
     for (int i0 = 0; i0 < a.A; i0 += 64) {
@@ -1182,9 +1216,12 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_replay_kernel(co
     }
   }
   n = __builtin_amdgcn_readfirstlane(min(max(n, 0), a.C));
-  const int nc = (n + 31) / 32, tiles = nc + (a.A + 31) / 32, share = a.G * a.A > CH ? dec_split<1>(tiles, a.S) : dec_split<4>(tiles, a.S);
-  const int t0 = (int)blockIdx.x * share, t1 = min(tiles, t0 + share);
-  if (t0 >= t1) return;
+  const int nc = (n + 31) / 32;
+  if (!a.NB) {
+    const int tiles = nc + (a.A + 31) / 32, share = a.G * a.A > CH ? dec_split<1>(tiles, a.S) : dec_split<4>(tiles, a.S);
+    t0 = (int)blockIdx.x * share, t1 = min(tiles, t0 + share);
+    if (t0 >= t1) return;
+  }
   const int rend = a.G * na, ws = rend > CH ? 4 : 1, rw = ws == 4 ? wv * CH : 0;   // the wave's rows in lse, weight, place, node
   const DecIn kc = a.kc + b * a.kcb + hkv * a.kch, kn = a.k + b * a.kb + hkv * a.kh;
   const float keep = fast_exp2(-a.decay_log2 * (float)na);
@@ -1566,6 +1603,13 @@ int dec_strides(const char* who, const int64_t* const* in, long long (*out)[4], 
   return FE_OK;
 }
 
+// Whether the heads of a launch share `blocks` blocks by their lengths, which a block has to read first (0.5 us). Heads of
+// one batch row mostly are of one length, and short calls (few rows) are left without. Trees of 61 tokens over two rows
+// of 32768 and 24576: 82 -> 77.6 us; of 64 tokens over eight equal rows 54.8 -> 55.4.
+bool dec_shared(int kind, int64_t B, int64_t BH, int64_t blocks) {
+  return kind != 0 && (kind == 2 || B > 1) && BH <= 128 && 2 * BH <= blocks;
+}
+
 // How an attention launch is laid out; the same for the workspace's size and the call.
 struct DecPlan {
   int kind;                    // 0: elements, 1: few, 2: wide
@@ -1573,7 +1617,7 @@ struct DecPlan {
   int NB;                      // blocks (of each row block) that the heads of a wide launch share, or 0
   size_t o, ml, heads, logits, bytes; // offsets
 };
-DecPlan dec_plan(int64_t BH, int64_t R, int64_t C, int64_t T, int64_t DP, bool vec, bool weights) {
+DecPlan dec_plan(int64_t B, int64_t BH, int64_t R, int64_t C, int64_t T, int64_t DP, bool vec, bool weights) {
   DecPlan p = {};
   const int64_t RT = (R + 31) / 32;
   p.kind = !vec ? 0 : R <= kDecFewRows ? 1 : 2;
@@ -1584,16 +1628,16 @@ DecPlan dec_plan(int64_t BH, int64_t R, int64_t C, int64_t T, int64_t DP, bool v
   const int64_t KT = p.kind == 2 ? 64 : 32, tiles = (C + KT - 1) / KT + (T + KT - 1) / KT;
   const int64_t resident = DP > 128 || (p.kind == 2 && p.waves == 8) ? 256 : 512;
   p.S = (int)std::max<int64_t>(1, std::min(resident / (BH * p.RB), (tiles + 3) / 4));
-  if (p.kind == 2 && BH <= 128 && 2 * BH * p.RB <= resident) p.NB = (int)std::min(resident / p.RB, BH * tiles);
+  if (dec_shared(p.kind, B, BH, resident / p.RB)) p.NB = (int)std::min(resident / p.RB, BH * (p.kind == 2 ? tiles : (tiles + 3) / 4));
   auto area = [&](size_t elems) {
     const size_t at = p.bytes;
     p.bytes += (elems * 4 + 255) / 256 * 256;
     return at;
   };
-  const size_t slots = p.kind == 2 ? (size_t)(p.NB ? p.NB : BH) * p.RB : (size_t)BH * p.RB * p.S;
+  const size_t slots = p.NB ? (size_t)p.NB * p.RB : (size_t)BH * p.RB * (p.kind == 2 ? 1 : p.S);
   p.o = area(slots * p.RS * DP);
   p.ml = area(slots * p.RS * 2);
-  p.heads = area(p.kind == 2 ? 2 * BH : 0);
+  p.heads = area(p.kind == 2 || p.NB ? 2 * BH : 0);
   p.logits = p.bytes;
   if (weights && R <= kDecLogitRows) area((size_t)BH * ((C + 31) / 32 + (T + 31) / 32) * R * 32);
   return p;
@@ -1646,7 +1690,12 @@ int dec_replay(const char* who, const DecKernels& kn, DecReplayArgs& a, const vo
   // as many blocks as the card holds at once, of at least a tile a wave
   const int64_t tiles = (C + 31) / 32 + (A + 31) / 32;
   a.S = (int)std::max<int64_t>(1, std::min<int64_t>((kn.dp > 128 ? 256 : 512) / (B * Hkv), vec && a.G * A > 64 ? tiles : (tiles + 3) / 4));
-  return dec_launch(who, kn.replay[vec], dim3((unsigned)a.S, (unsigned)Hkv, (unsigned)B), dim3(256), a, stream);
+  a.Hkv = (int)Hkv;
+  a.BH = (int)(B * Hkv);
+  const int64_t blocks = kn.dp > 128 ? 256 : 512;
+  if (dec_shared(vec, B, B * Hkv, blocks)) a.NB = (int)std::min<int64_t>(blocks, B * Hkv * (a.G * A > 64 ? tiles : (tiles + 3) / 4));
+  const dim3 grid = a.NB ? dim3((unsigned)a.NB) : dim3((unsigned)a.S, (unsigned)Hkv, (unsigned)B);
+  return dec_launch(who, kn.replay[vec], grid, dim3(256), a, stream);
 }
 
 }  // namespace
@@ -1659,8 +1708,8 @@ extern "C" size_t fe_decode_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, 
       B * Hkv > (1LL << 30) || Hq / Hkv > 32767 || C > (1LL << 30) || B * ((Hq / Hkv * T + 31) / 32) > 65535)
     return 0;
   const int64_t dp = dec_kernels(D, 0).dp;
-  return std::max(dec_plan(B * Hkv, Hq / Hkv * T, C, T, dp, false, weights != 0).bytes,
-                  dec_plan(B * Hkv, Hq / Hkv * T, C, T, dp, true, weights != 0).bytes);
+  return std::max(dec_plan(B, B * Hkv, Hq / Hkv * T, C, T, dp, false, weights != 0).bytes,
+                  dec_plan(B, B * Hkv, Hq / Hkv * T, C, T, dp, true, weights != 0).bytes);
 }
 
 extern "C" int fe_decode_attention(const void* q, const void* k, const void* v, const void* k_cache, const void* v_cache,
@@ -1694,7 +1743,7 @@ extern "C" int fe_decode_attention(const void* q, const void* k, const void* v, 
   const bool vec = vec_ok(q, st[0], B, Hq, T, D) && vec_ok(k, st[1], B, Hkv, T, D) && vec_ok(v, st[2], B, Hkv, T, D) &&
                    vec_ok(k_cache, st[3], B, Hkv, C, D) && vec_ok(v_cache, st[4], B, Hkv, C, D);
   const int64_t BH = B * Hkv, R = Hq / Hkv * T;
-  const DecPlan p = dec_plan(BH, R, C, T, kn.dp, vec, importance != nullptr);
+  const DecPlan p = dec_plan(B, BH, R, C, T, kn.dp, vec, importance != nullptr);
   const bool logits = importance && R <= kDecLogitRows;
   char* ws = (char*)workspace;
   hipStream_t stream = (hipStream_t)hip_stream;
@@ -1725,12 +1774,12 @@ extern "C" int fe_decode_attention(const void* q, const void* k, const void* v, 
   a.Hkv = (int)Hkv;
   a.BH = (int)BH;
   a.NB = p.NB;
-  if (p.kind == 2) dec_set(a.heads, ws + p.heads);
+  if (p.kind == 2 || p.NB) dec_set(a.heads, ws + p.heads);
   a.max_tiles = (int)((C + 31) / 32 + (T + 31) / 32);
   dec_scale(a, scale);
   if (p.kind == 1) a.scale_log2 = (float)((double)scale * 1.4426950408889634);   // masks after the scale
   const void* fn = p.kind == 0 ? kn.elements : p.kind == 1 ? kn.few : kn.wide[p.waves == 8];
-  const dim3 grid = p.kind == 2 ? dim3((unsigned)(p.NB ? p.NB : BH), (unsigned)p.RB) : dim3((unsigned)p.S, (unsigned)Hkv, (unsigned)(B * p.RB));
+  const dim3 grid = p.NB ? dim3((unsigned)p.NB, (unsigned)p.RB) : p.kind == 2 ? dim3((unsigned)BH, (unsigned)p.RB) : dim3((unsigned)p.S, (unsigned)Hkv, (unsigned)(B * p.RB));
   if (int rc = dec_launch(who, fn, grid, dim3(p.kind == 2 ? 64 * p.waves : 256), a, stream)) return rc;
 
   DecJoinArgs o = {};
@@ -1764,7 +1813,7 @@ extern "C" int fe_decode_attention(const void* q, const void* k, const void* v, 
   o.decay_log2 = (float)((double)recency_decay * 1.4426950408889634);
   // all of a block's groups of threads on a row where they have slots enough, else one on each
   const int groups = 256 / (kn.dp / 4);
-  o.rows = 2 * (p.kind == 2 ? p.NB / BH : p.S) > groups ? 1 : groups;
+  o.rows = 2 * (p.NB ? p.NB / BH : p.kind == 2 ? 1 : p.S) > groups ? 1 : groups;
   o.out_blocks = (int)((R + o.rows - 1) / o.rows);
   const int64_t per = logits ? std::min<int64_t>((a.max_tiles + 7) / 8, std::max<int64_t>(1, kDecJoinBlocks / BH)) : 0;
   if (int rc = dec_launch(who, kn.join, dim3((unsigned)(o.out_blocks + per), (unsigned)Hkv, (unsigned)B), dim3(256), o, stream)) return rc;
