@@ -24,11 +24,16 @@
 //                          taken in lse's own units, where it rounds once
 //                          (decode_replay_elements_kernel for rows that do not allow 16-byte loads)
 //
+// Sums, maxima and partial outputs are FP32. Probabilities are rounded to the inputs' type, as the second product takes
+// them: half a step of each, which the output's own rounding has too; outputs are normalised by the sum of the rounded
+// ones. lse and the importance take the exact ones.
+//
 // Lengths are known on the device only: a launch's grid comes from the cache's size, and a head's blocks divide the
-// tiles that its length has. Short calls are bound by the reading of code and arguments and by trips to memory one after
-// the other, so the kernels read their arguments at once (dec_hold), have the loads of a tile in the code once, read
-// rows past the end as the last, and divide little: the first version of this file, which did none of that, took 15.4 +
-// 11.0 us for a step over 1024 rows of 8 heads, against 6.4 + 4.6 us.
+// tiles that its length has, or all heads' blocks all tiles (dec_assign).
+// Short calls are bound by code that runs for the first time and by trips to memory one after the other. So registers
+// do not spill, the loads of a tile are in the code once, rows past the end are read as the last, arguments are read at
+// once (dec_hold), and little is divided: the first version of this file, which did none of that, took 15.4 + 11.0 us
+// for a step over 1024 rows of 8 heads, against 6.1 + 5.3 us.
 #include <math.h>
 #include <stddef.h>
 #include <algorithm>
@@ -47,11 +52,15 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) dec_s16x4 dec_lds_s16x4;
 
 constexpr int kDecMaxTokens = 256;   // new tokens of a call
-constexpr int kDecFewRows = 16;      // rows of a group, up to which decode_few_kernel takes them
+// Rows of a group up to which decode_few_kernel takes them: it has one tile of 16. With a second one it took 11.3 us for
+// 32 rows of 8 heads over 1024 rows of the cache and 38.5 us of 32 heads over 8192, the wide kernel 12.4 and 31.2.
+constexpr int kDecFewRows = 16;
 // Rows of a group up to which the attention leaves its logits for the importance: 8 bytes a row and key, written and
-// read, against the 2 D of reading K again.
+// read, against the 2 D of reading K again. Measured with the logits and without, 8 heads: 4 rows over 131072 keys 123
+// and 164 us, over 1024 11.5 and 13.9; 16 rows over 65536 65 and 74.
 constexpr int kDecLogitRows = 16;
-constexpr int kDecJoinBlocks = 1024;   // blocks that share the importance of all heads
+// Blocks that share the importance of all heads: a step over 131072 rows 128.7 us with 256, 123 with 1024, 128 with 4096.
+constexpr int kDecJoinBlocks = 1024;
 // Pointers to global memory, said to be: a pointer that the compiler loses sight of (dec_hold) would be read with flat
 // instructions, which wait for LDS too.
 #define FE_GLOBAL __attribute__((address_space(1)))
@@ -117,8 +126,7 @@ struct DecJoinArgs {
 static_assert(offsetof(DecJoinArgs, pad) <= 4 * 64 && sizeof(DecJoinArgs) >= 4 * 64, "argument window");
 
 // The kernel's arguments, NV * 64 bytes of them from byte FIRST on read at once and kept in registers. Left to the
-// compiler, each is read where it is first used and again wherever that saves registers; arguments lie in host memory,
-// and a wave waited some 2000 cycles for every such read .
+// compiler, each is read where it is first used and again wherever that saves registers, with a wait each time.
 template <int FIRST, int NV, typename A>
 __device__ __forceinline__ A dec_hold(const A& arg) {
   static_assert(sizeof(A) >= FIRST + NV * 64, "argument window");
@@ -293,9 +301,10 @@ __device__ __forceinline__ float dec_quad_sum(float x) {
 // Block (split, KV head, batch row). S^T = K Q^T and O^T = V^T P^T with the 16 rows in the lanes' low four bits: 32 keys
 // are two accumulators of S^T, whose registers (keys 4 (lane / 16) + i of each) are P^T's operand as
 // they are; V^T's comes from transposing reads in that key order.
+// Waves take keys for themselves, without a barrier, for the tile of 16 rows leaves the matrix pipe idle most of the time.
 // What bounds it: HBM where the cache is long (the next 32 keys' K and V are on their way to registers while a wave
-// works on these); where it is short, the reading of its own code and the one round trip to memory, so the loads of
-// a tile appear in the code once, rows past the end are read as the last, and nothing is divided that need not be.
+// works on these): 131072 rows of 8 heads, 128 channels, 110 us, 4.9 TB/s. Where it is short, the reading of its own code
+// and the round trips to memory: 1024 rows 6.1 us.
 template <typename E, int DP>
 __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_few_kernel(const DecArgs args) {
   constexpr int NC = DP / 32, NT16 = DP / 16, CPR = DP / 8, NL = DP / 16, TILE = 64 * DP, OST = DP + 4, RS = 16;
@@ -528,8 +537,11 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_few_kernel(const
 // probabilities could overflow (E::kMaxTileSum), as in the prefill kernels, so most tiles spend nothing on maxima and
 // rescaling. The two waves of a SIMD run half a tile apart: one multiplies a tile's probabilities by V right away, the
 // other at the next tile, while the first is at its exponentials.
-// What bounds it: the matrix pipe and the vector work beside it (an exponential a logit); at 256 rows a tile takes
-// about as long as its bytes from HBM.
+// What bounds it: the matrix pipe and the vector work beside it, 6.7 vector instructions to a product, an exponential a
+// logit among them, which together fill 85% of a SIMD's time though they could overlap; LDS is busy 26% of it. Trees of
+// 61 tokens of 7 heads over 4 KV heads' 32768 and 24576 rows, 128 channels: 74 us, 680 TFLOP/s (fp16); of 64 tokens of 4
+// heads over 64 heads of 2304 to 4096 rows: 48 us, 570 TFLOP/s, 2.2 TB/s.
+// One barrier a tile and the waves in step: 5% slower; four waves a block and two blocks a CU: 14% (tree of 64).
 template <typename E, int DP, int NW>
 __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void decode_wide_kernel(const DecArgs args) {
   constexpr int NDC = DP / 16, NDT = DP / 32, CPR = DP / 8, TILE = 128 * DP;   // bytes of 64 rows
@@ -825,7 +837,8 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void decode_wide_kernel(
   }
 }
 
-// 32 rows a block, keys to its waves 32 at a time, everything read element by element.
+// 32 rows a block, keys to its waves 32 at a time, everything read element by element. What bounds it: the instructions
+// that put elements together.
 template <typename E, int DP>
 __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_elements_kernel(const DecArgs a) {
   constexpr int NDC = DP / 16, NDT = DP / 32, CPR = DP / 8, TILE = 64 * DP;   // bytes of 32 rows
@@ -1011,7 +1024,8 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_elements_kernel(
 // Joins the splits. Blocks below out_blocks of a head: output rows, DP / 4 threads on a slot's values, merging slots as
 // they are read (maximum, sum, values); where a row has many slots all of a block's groups of threads are on one row.
 // The others, where there are logits: the head's importance, a tile of 32 keys to 32 lanes.
-// What bounds it: two trips to memory and the reading of its code; on long caches the logits' and weights' bytes.
+// What bounds it: two trips to memory and the reading of its code, 4.7 to 9 us; on long caches the logits' and weights'
+// bytes: 8 heads of 131072 rows 13.3 us, 2.2 TB/s.
 template <typename E, int DP>
 __global__ __launch_bounds__(256) void decode_join_kernel(const DecJoinArgs args) {
   constexpr int LPR = DP / 4, NG = 256 / LPR, PF = 4;   // threads on a slot, groups of them; loads in flight
@@ -1180,11 +1194,13 @@ __global__ __launch_bounds__(256) void decode_join_kernel(const DecJoinArgs args
   }
 }
 
-// Block (split, KV head, batch row), as decode_few_kernel. Rows r = g * A_b + i of the path, 64 at a time, with their Q in
-// registers as four tiles of 16; a wave takes 32 keys at a time, straight into the products' operands (a lane's 16
-// bytes of a key lie beside its neighbours' of the same key, 64 bytes in all), the next 32 on the way. More than 64
-// rows take K again, adding to what the rows before left.
-// What bounds it: reading K; on short caches the trips to memory one after the other (path, then its rows).
+// Blocks as decode_few_kernel's. Rows r = g * A_b + i of the path, 64 to a wave, with their Q in registers as four tiles of
+// 16; a wave takes 32 keys at a time, straight into the products' operands (a lane's 16 bytes of a key lie beside its
+// neighbours' of the same key, 64 bytes in all), the next 32 on the way. Up to 64 rows, the block's waves take different
+// keys; more, the same keys for 64 rows each, summed in LDS (132 rows of 2 heads and 3 batch rows over 5000 keys: 16.4 us
+// with one wave for all of a key's rows, 10.4 so). More than 256 rows take K again, adding to what the rows before left.
+// What bounds it: reading K, 24 rows of 4 heads and 8 batch rows of up to 32768 keys 54 us, 4.1 TB/s; on short caches the
+// trips to memory one after the other (path, its rows, lse): 1024 keys 6.4 us.
 template <typename E, int DP>
 __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_replay_kernel(const DecReplayArgs args) {
   constexpr int NC = DP / 32, RT = 4, CH = 16 * RT;
@@ -1621,6 +1637,8 @@ DecPlan dec_plan(int64_t B, int64_t BH, int64_t R, int64_t C, int64_t T, int64_t
   DecPlan p = {};
   const int64_t RT = (R + 31) / 32;
   p.kind = !vec ? 0 : R <= kDecFewRows ? 1 : 2;
+  // eight waves, two on a SIMD, where their registers and rows suffice: 64 rows of 32 heads over 8192 rows 35.4 us with
+  // four and 39.1 with eight, 128 rows 41.8 and 42.7; 256 rows of 64 heads over 4096 76 and 67
   p.waves = DP > 128 || RT <= 4 ? 4 : 8;
   p.RB = (int)(p.kind == 2 ? (RT + p.waves - 1) / p.waves : RT);
   p.RS = (int)(p.kind == 2 ? 32 * ((RT + p.RB - 1) / p.RB) : p.kind == 1 ? 16 : 32);
@@ -1811,7 +1829,8 @@ extern "C" int fe_decode_attention(const void* q, const void* k, const void* v, 
   o.S = a.S;
   o.max_tiles = a.max_tiles;
   o.decay_log2 = (float)((double)recency_decay * 1.4426950408889634);
-  // all of a block's groups of threads on a row where they have slots enough, else one on each
+  // all of a block's groups of threads on a row where they have slots enough, else one on each (256 rows of 64 heads in 4
+  // slots each: 51.0 us in all; all on a row 63.0)
   const int groups = 256 / (kn.dp / 4);
   o.rows = 2 * (p.NB ? p.NB / BH : p.kind == 2 ? 1 : p.S) > groups ? 1 : groups;
   o.out_blocks = (int)((R + o.rows - 1) / o.rows);

@@ -10,8 +10,8 @@
 // vacated slots below F.
 //
 //   insert_few_kernel    up to 256 new rows and 256 evicted ones, on caches of up to 32512 slots: one 1024-thread block a
-//                        head. Order keys are staged in LDS; up to eight victims are drawn one by one as the least key (of
-//                        equal ones the highest slot), more are found by a radix select and an ordered pass
+//                        head. Order keys are staged in LDS; up to 32 victims are drawn one by one as the least key (of equal
+//                        ones the highest slot), more are found by a radix select and an ordered pass
 //   insert_list_kernel   otherwise: the same by a radix select over the head's rows in memory; leaves the list of moves
 //   insert_move_kernel   carries it out, the whole card on it
 #include <math.h>
@@ -31,9 +31,11 @@ namespace fe {
 typedef const FE_GLOBAL u16* InsIn;
 typedef FE_GLOBAL u16* InsOut;
 
-constexpr int kInsFew = 256;         // new rows, and evicted ones, of insert_few_kernel
+// New rows, and evicted ones, of insert_few_kernel: 40 to 250 rows into 8192 take it 32 us, the other two kernels 40.
+constexpr int kInsFew = 256;
 constexpr int kInsKeys = 32768;      // its candidates (128 KiB of LDS)
-constexpr int kInsDraw = 32;         // victims drawn one by one
+// Victims drawn one by one, 0.55 us each: 16 of 8192 rows 13.8 us, by selection 33.
+constexpr int kInsDraw = 32;
 
 struct InsArgs {
   InsIn k, v;
@@ -54,7 +56,7 @@ struct InsArgs {
 };
 static_assert(offsetof(InsArgs, kd) == 4 * 64, "argument window");
 
-// The arguments, read at once and kept in registers: read where they are used, each costs a trip to host memory.
+// The arguments, read at once and kept in registers, not one by one where they are used with a wait each time.
 __device__ __forceinline__ InsArgs ins_hold(const InsArgs& arg) {
   InsArgs a = arg;
   typedef u32 u32x16 __attribute__((ext_vector_type(16), aligned(4)));
@@ -226,6 +228,9 @@ __device__ __forceinline__ void ins_order(Get get, int n, int M, int F, u32 thr,
   }
 }
 
+// Block (KV head, batch row). What bounds it: the trips to memory one after the other (length, keys, rows) and the barrier
+// of each drawn victim: one row into 1024 rows of 8 heads 6.4 us, into 8192 rows of 128 heads 7.7, six into 13107 rows of
+// 32 heads 12.7; by selection the counts' atomics, 250 into 2000 rows of 16 heads 17.7.
 template <bool VEC>
 __global__ __launch_bounds__(1024) void insert_few_kernel(const InsArgs args) {
   __shared__ u32 skey[kInsKeys];
@@ -351,6 +356,7 @@ __global__ __launch_bounds__(1024) void insert_few_kernel(const InsArgs args) {
   }
 }
 
+// Block (KV head, batch row). What bounds it: one CU's reads of the head's keys, once a digit.
 __global__ __launch_bounds__(1024) void insert_list_kernel(const InsArgs args) {
   __shared__ u32 hist[2 * 2048];
   __shared__ __attribute__((aligned(16))) int tmp[2 * kSelWaves];
@@ -391,6 +397,7 @@ __global__ __launch_bounds__(1024) void insert_list_kernel(const InsArgs args) {
   }
 }
 
+// What bounds it: HBM, with rows in no order.
 template <bool VEC>
 __global__ __launch_bounds__(256) void insert_move_kernel(const InsArgs args) {
   const InsArgs a = ins_hold(args);
