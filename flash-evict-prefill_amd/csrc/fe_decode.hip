@@ -364,9 +364,11 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_few_kernel(const
     if (t >= 0) {
       if (kb + 32 > rows) dec_cut_rows<DP, 64>(kb, rows, lane, vx);
       if (a.D != DP) {
+        int D = a.D;
+        asm volatile("" : "+s"(D));
 #pragma unroll
         for (int i = 0; i < NL; ++i)
-          if (8 * ((i * 64 + lane) % CPR) >= a.D) kx[i] = (u32x4){0u, 0u, 0u, 0u};
+          if (8 * ((i * 64 + lane) % CPR) >= D) kx[i] = (u32x4){0u, 0u, 0u, 0u};
       }
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
@@ -388,15 +390,15 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_few_kernel(const
       const int nkb = (nt ? next - nc : next) * 32, last = (nt ? a.T : n) - 1;
       const DecIn kp = nt ? kn : kc, vp = nt ? vn : vc;
       const u32 ks = nt ? a.kn : a.kcn, vs = nt ? a.vn : a.vcn;
+      int D = a.D;
+      asm volatile("" : "+s"(D));          // compared here, not kept as masks over the loop
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
         const int e = i * 64 + lane, ch = 8 * (e % CPR);
         const u32 row = (u32)min(nkb + e / CPR, last);
-        if (64 % CPR == 0 ? true : ch < a.D) {
-          const int cc = DP == a.D || ch < a.D ? ch : 0;
-          kx[i] = *(const FE_GLOBAL u32x4*)(kp + (unsigned long long)row * ks + cc);
-          vx[i] = *(const FE_GLOBAL u32x4*)(vp + (unsigned long long)row * vs + cc);
-        }
+        const int cc = ch < D ? ch : 0;
+        kx[i] = *(const FE_GLOBAL u32x4*)(kp + (unsigned long long)row * ks + cc);
+        vx[i] = *(const FE_GLOBAL u32x4*)(vp + (unsigned long long)row * vs + cc);
       }
     }
     if (t >= 0) {
@@ -614,7 +616,7 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void decode_wide_kernel(
       unsigned char* vt = vbuf(t);
       const bool nt = t >= nc;
       const int kb = (nt ? t - nc : t) * 64, rows = nt ? a.T : n;
-      if (kb + 64 > rows) dec_cut_rows<DP, NT>(kb, rows, tid, vx);
+      dec_cut_rows<DP, NT>(kb, rows, tid, vx);   // (unconditionally, as below)
       if (a.D != DP) {
         int D = a.D;
         asm volatile("" : "+s"(D));
@@ -648,12 +650,15 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void decode_wide_kernel(
       qf[c] = (qf[c] & keep) ^ flip;
     }
     store(t0);
-    if (t0 + 1 < t1) load(t0 + 1);
+    // 256 channels leave no registers for rows on their way: 256 rows of 8 heads over 8192 rows 114 us with them, 59 without
+    constexpr bool AHEAD = DP <= 192;
+    if (AHEAD && t0 + 1 < t1) load(t0 + 1);
     __syncthreads();
     // the next tile into LDS, the one behind it on its way
     auto advance = [&](int t) __attribute__((always_inline)) {
+      if (!AHEAD && t + 1 < t1) load(t + 1);
       if (t + 1 < t1) store(t + 1);
-      if (t + 2 < t1) load(t + 2);
+      if (AHEAD && t + 2 < t1) load(t + 2);
       __syncthreads();
     };
 #pragma unroll 1
