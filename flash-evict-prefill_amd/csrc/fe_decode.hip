@@ -1633,10 +1633,11 @@ int dec_strides(const char* who, const int64_t* const* in, long long (*out)[4], 
 }
 
 // Whether the heads of a launch share `blocks` blocks by their lengths, which a block has to read first (0.5 us). Heads of
-// one batch row mostly are of one length, and short calls (few rows) are left without. Trees of 61 tokens over two rows
-// of 32768 and 24576: 82 -> 77.6 us; of 64 tokens over eight equal rows 54.8 -> 55.4.
-bool dec_shared(int kind, int64_t B, int64_t BH, int64_t blocks) {
-  return kind != 0 && (kind == 2 || B > 1) && BH <= 128 && 2 * BH <= blocks;
+// one batch row mostly are of one length, and without that launches whose tiles all have a block of their own (`need`)
+// gain nothing. Paths of 6 over eight rows of 18432 to 32768: 51.7 us without, 43.9 with; trees of 61 tokens over two rows
+// of 32768 and 24576 82 and 77.6; of 64 tokens over eight equal rows 54.8 and 55.4.
+bool dec_shared(bool wide, int64_t B, int64_t BH, int64_t blocks, int64_t need) {
+  return (wide || (B > 1 && blocks < need)) && BH <= 128 && 2 * BH <= blocks;
 }
 
 // How an attention launch is laid out; the same for the workspace's size and the call.
@@ -1659,7 +1660,8 @@ DecPlan dec_plan(int64_t B, int64_t BH, int64_t R, int64_t C, int64_t T, int64_t
   const int64_t KT = p.kind == 2 ? 64 : 32, tiles = (C + KT - 1) / KT + (T + KT - 1) / KT;
   const int64_t resident = DP > 128 || (p.kind == 2 && p.waves == 8) ? 256 : 512;
   p.S = (int)std::max<int64_t>(1, std::min(resident / (BH * p.RB), (tiles + 3) / 4));
-  if (dec_shared(p.kind, B, BH, resident / p.RB)) p.NB = (int)std::min(resident / p.RB, BH * (p.kind == 2 ? tiles : (tiles + 3) / 4));
+  const int64_t need = BH * (p.kind == 2 ? tiles : (tiles + 3) / 4);
+  if (p.kind != 0 && dec_shared(p.kind == 2, B, BH, resident / p.RB, need)) p.NB = (int)std::min(resident / p.RB, need);
   auto area = [&](size_t elems) {
     const size_t at = p.bytes;
     p.bytes += (elems * 4 + 255) / 256 * 256;
@@ -1724,7 +1726,7 @@ int dec_replay(const char* who, const DecKernels& kn, DecReplayArgs& a, const vo
   a.Hkv = (int)Hkv;
   a.BH = (int)(B * Hkv);
   const int64_t blocks = kn.dp > 128 ? 256 : 512;
-  if (dec_shared(vec, B, B * Hkv, blocks)) a.NB = (int)std::min<int64_t>(blocks, B * Hkv * (a.G * A > 64 ? tiles : (tiles + 3) / 4));
+  if (vec && dec_shared(false, B, B * Hkv, blocks, B * Hkv * (a.G * A > 64 ? tiles : (tiles + 3) / 4))) a.NB = (int)blocks;
   const dim3 grid = a.NB ? dim3((unsigned)a.NB) : dim3((unsigned)a.S, (unsigned)Hkv, (unsigned)B);
   return dec_launch(who, kn.replay[vec], grid, dim3(256), a, stream);
 }

@@ -263,8 +263,9 @@ int fe_replay_path(const void* q, const void* k, const void* v, const void* k_ca
  * the nodes of path[b] as above) as if appended to them, with positions seen[b,j], seen[b,j]+1, ...
  * and importance new_importance [B,Hkv,A] (NULL: 0). F = min(candidates, budget) stay: the rows of
  * the newest `recent` positions (should there be more, those at the lowest slots), then by
- * importance (NaN above every number, -0 equal to 0), equal ones by slot. Of those, rows below slot F stay in place, and the i-th one past it goes to the
- * i-th slot below F that was vacated. Then length = F and seen += the path's nodes; slots from F
+ * importance (NaN above every number, -0 equal to 0), equal ones by slot. Of those, rows below
+ * slot F stay in place, and the i-th one past it goes to the i-th slot below F that was vacated.
+ * Then length = F and seen += the path's nodes; slots from F
  * on are left as they were. value_norm may be NULL; otherwise new rows get the L1 norm of their
  * value. T may be 0 (k and v NULL): an eviction to `budget`. 1 <= budget <= C, recent <= budget.
  * k and v must not overlap the cache. workspace: at least fe_insert_workspace_bytes(...) bytes

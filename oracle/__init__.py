@@ -17,6 +17,8 @@ Modules and the reference code each one restates (anishesg/flash-evict-prefill):
   snap.snap_scores         flash_evict/baselines.py:15-27 (SnapKV observation-window scores)
   gather.gather_tokens     kv_distill.cache.gather_tokens as called at
                            flash_evict/kv_distill_adapter.py:38-39 (KV compaction)
+  decode                   no reference code: decoding over a bounded cache in float64, from
+                           the definitions in include/flash_evict.h
   analytic                 closed forms used by tests/test_prefill.py:87-102,134-146
 
 How each function is pinned (checked against something other than itself):
