@@ -69,8 +69,8 @@ typedef FE_GLOBAL float* DecF32;
 typedef const FE_GLOBAL float* DecF32In;
 typedef const FE_GLOBAL int* DecI32In;
 
-// Attention. Slots: ((b * Hkv + j) * RB + row block) * S + split; of the wide kernel, block * RB + row block, a head's
-// first block and their number in `heads`.
+// Attention. Slots: ((b * Hkv + j) * RB + row block) * S + split; of the wide kernel and where heads share the blocks, block *
+// RB + row block, with a head's first block and their number in `heads`.
 struct DecArgs {
   DecIn q, k, v, kc, vc;   // queries, new rows, the cache
   DecI32In length;         // [B * Hkv]
@@ -83,7 +83,7 @@ struct DecArgs {
   int T, C, D, R, RB, RS, S, max_tiles;   // R rows of a group in RB blocks of RS; splits; tiles of a full cache
   u32 qand, qxor;          // Q's sign for a negative scale, Q's zeros for a zero one
   float scale_log2;
-  int Hkv, BH, NB;         // the wide kernel's: all heads; blocks they share, or 0: a block each
+  int Hkv, BH, NB;         // BH: all heads; NB: blocks they share, or 0
   FE_GLOBAL int* heads;    // [B * Hkv][2]
   int pad[2];
   // element loads: 64-bit row strides, channel strides
@@ -101,7 +101,7 @@ struct DecReplayArgs {
   u32 kn, vn, kcn;         // row strides
   int T, C, D, G, A, S;
   float scale, decay_log2;
-  int Hkv, BH, NB;         // all heads; blocks they share, or 0: S for each
+  int Hkv, BH, NB;         // as above
   int pad[5];
   // element loads: 64-bit row strides, channel strides
   long long kn64, vn64, kcn64, qc, kd, vd, kcd;
@@ -110,7 +110,7 @@ static_assert(offsetof(DecReplayArgs, pad) <= 4 * 64 && sizeof(DecReplayArgs) >=
 
 struct DecJoinArgs {
   DecF32In part_o, part_ml, logits;
-  DecI32In length, heads;  // heads: of the wide kernel's slots, or null
+  DecI32In length, heads;  // heads: as above, or null
   FE_GLOBAL u16* out;      // [B, Hq, T, D]
   DecF32 lse;              // [B, Hq, T]
   DecF32In imp, norm;
@@ -1772,6 +1772,10 @@ extern "C" int fe_decode_attention(const void* q, const void* k, const void* v, 
   if (!workspace || workspace_bytes < need) {
     set_error(std::string(who) + ": workspace too small; need " + std::to_string(need) + " bytes");
     return FE_ERR_WORKSPACE;
+  }
+  if ((uintptr_t)workspace % 16 || (uintptr_t)out % 8) {
+    set_error(std::string(who) + ": workspace must lie on a 16-byte boundary, out on an 8-byte one");
+    return FE_ERR_INVALID;
   }
   const bool vec = vec_ok(q, st[0], B, Hq, T, D) && vec_ok(k, st[1], B, Hkv, T, D) && vec_ok(v, st[2], B, Hkv, T, D) &&
                    vec_ok(k_cache, st[3], B, Hkv, C, D) && vec_ok(v_cache, st[4], B, Hkv, C, D);

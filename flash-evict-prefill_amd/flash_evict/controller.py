@@ -140,7 +140,8 @@ class Controller:
     def _bound(self, state):
         """A layer's bounded cache, from the tokens and importance its compression kept."""
         if "importance" not in state:
-            raise ValueError("decode_budget continues prefill's importance: it needs the fused backend and compression")
+            raise ValueError("decode_budget continues prefill's importance: it needs the fused backend and compression, and to "
+                             "be set before them")
         b, hk, n, d = state["k"].shape
         if n > self.decode_budget:
             raise ValueError("decode_budget must not be less than the compressed prompt's budget")

@@ -230,7 +230,7 @@ int fe_snap_scores(const void* q, const void* k, float* scores, int64_t B, int64
  * Both without their norm when value_norm is NULL. importance_out may be importance; slots from
  * length on are left as they were. A hidden new row never reaches a query, whatever it holds.
  * workspace: at least fe_decode_workspace_bytes(...) bytes (weights != 0: with importance),
- * 16-byte aligned, not shared by calls that overlap.
+ * 16-byte aligned, not shared by calls that overlap. out: 8-byte aligned.
  */
 size_t fe_decode_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t C, int64_t D, int weights);
 int fe_decode_attention(const void* q, const void* k, const void* v, const void* k_cache, const void* v_cache,

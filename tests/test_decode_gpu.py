@@ -112,6 +112,23 @@ def test_heads_of_different_lengths_share_the_blocks(b, hk, g, t, c, d):
     _attend_and_check(q, k, v, kc, vc, length, importance=imp, value_norm=norm, recency_decay=0.01)
 
 
+@pytest.mark.parametrize("d,dtype", [(64, BF), (128, FP), (192, BF)])
+@pytest.mark.parametrize("alike", [False, True])
+def test_batches_of_many_heads(d, dtype, alike):
+    """Few rows of 64 and 128 heads, more tiles than blocks: steps, a chunk and a path, lengths from 0 to all or alike."""
+    b, hk, c, t = 16 if d > 128 else 32, 4, 1100, 3
+    q, k, v, kc, vc = make(b, 2 * hk, hk, t, c, d, dtype, 16)
+    length = torch.full((b, hk), c, dtype=torch.int32).cuda() if alike else _lengths(b, hk, c, 17)
+    imp, norm = _scores(b, hk, c, vc, 18)
+    _attend_and_check(q[:, :, :1], k[:, :, :1], v[:, :, :1], kc, vc, length, importance=imp, value_norm=norm, recency_decay=0.1)
+    tree = torch.tensor([[1, 0, 0], [1, 1, 0], [1, 0, 1]], dtype=torch.bool).cuda()
+    _, lse, _, _, _ = _attend_and_check(q, k, v, kc, vc, length, tree=tree)
+    path = torch.tensor([[0, 2], [0, -1]], dtype=torch.int32).repeat(b // 2, 1).cuda()
+    got, new = replay_path(q, k, v, kc, length, lse, path, imp, value_norm=norm, recency_decay=0.2)
+    ref = odec.replay(q, k, v, kc, length, lse, path, imp, value_norm=norm, recency_decay=0.2)
+    check_importance(got, new, ref, imp, float(lse[lse != -math.inf].abs().max()), ref["dots"], 4, c, d, True)
+
+
 TREES = [(1, 8, 2, 2, 40, 64, BF), (2, 8, 2, 13, 100, 128, FP), (1, 28, 4, 64, 333, 128, BF), (2, 4, 2, 61, 64, 80, FP),
          (1, 4, 1, 128, 200, 128, BF), (1, 2, 2, 250, 31, 256, FP), (1, 4, 2, 33, 50, 100, BF)]
 

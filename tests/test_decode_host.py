@@ -159,6 +159,7 @@ def _attend_c(L, B=1, Hq=4, Hkv=2, T=3, C=8, D=16, dtype=1, scale=1., decay=0., 
     (dict(decay=-1.), INVALID), (dict(decay=math.nan), INVALID), (dict(length=None), INVALID), (dict(out=None), INVALID),
     (dict(st=None), INVALID), (dict(st=(ctypes.c_int64 * 4)(1, 1, -1, 1)), INVALID), (dict(imp=P, imp_st=7), INVALID),
     (dict(tree_st=-1), INVALID), (dict(ws=None), WORKSPACE), (dict(ws=P), WORKSPACE),
+    (dict(ws=ctypes.c_void_p(4104), ws_bytes=1 << 30), INVALID), (dict(out=ctypes.c_void_p(4100), ws=P, ws_bytes=1 << 30), INVALID),
     (dict(C=(1 << 30) + 1, imp_st=1 << 31), UNSUPPORTED), (dict(B=1 << 25), UNSUPPORTED), (dict(Hq=1 << 17, Hkv=1), UNSUPPORTED),
 ])
 def test_c_decode_attention_refuses(change, code):
