@@ -125,27 +125,27 @@ struct DecJoinArgs {
 };
 static_assert(offsetof(DecJoinArgs, pad) <= 4 * 64 && sizeof(DecJoinArgs) >= 4 * 64, "argument window");
 
-// The kernel's arguments, NV * 64 bytes of them from byte FIRST on read at once and kept in registers. Left to the
-// compiler, each is read where it is first used and again wherever that saves registers, with a wait each time.
-template <int FIRST, int NV, typename A>
+// The kernel's arguments, the first 256 bytes of them read at once and kept in registers. Left to the compiler, each is read
+// where it is first used and again wherever that saves registers, with a wait each time.
+template <typename A>
 __device__ __forceinline__ A dec_hold(const A& arg) {
-  static_assert(sizeof(A) >= FIRST + NV * 64, "argument window");
+  static_assert(sizeof(A) >= 4 * 64, "argument window");
   A a = arg;
   typedef u32 u32x16 __attribute__((ext_vector_type(16), aligned(4)));
   typedef const __attribute__((address_space(4))) u32x16* args_ptr;
-  const args_ptr p = (args_ptr)((const __attribute__((address_space(4))) char*)__builtin_amdgcn_kernarg_segment_ptr() + FIRST);
-  u32x16 v[NV];
+  const args_ptr p = (args_ptr)__builtin_amdgcn_kernarg_segment_ptr();
+  u32x16 v[4];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) v[i] = p[i];
-  if constexpr (NV == 4) asm volatile("" : "+s"(v[0]), "+s"(v[1]), "+s"(v[2]), "+s"(v[3]));
+  for (int i = 0; i < 4; ++i) v[i] = p[i];
+  asm volatile("" : "+s"(v[0]), "+s"(v[1]), "+s"(v[2]), "+s"(v[3]));
   // from here on word by word: a spilled register of 16 words would come back whole for each word of it
-  u32 w[NV * 16];
+  u32 w[64];
 #pragma unroll
-  for (int i = 0; i < NV * 16; ++i) {
+  for (int i = 0; i < 64; ++i) {
     w[i] = v[i / 16][i % 16];
     asm volatile("" : "+s"(w[i]));
   }
-  __builtin_memcpy((char*)&a + FIRST, w, NV * 64);
+  __builtin_memcpy((char*)&a, w, 4 * 64);
   return a;
 }
 
@@ -312,7 +312,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_few_kernel(const
   __shared__ __attribute__((aligned(1024))) unsigned char lds[4][WLDS];
   __shared__ float sm[3][4][RS];
   static_assert(WLDS >= RS * OST * 4 && WLDS >= (32 * RS + DP) * 4, "output, or probabilities and a value, in a wave's tiles");
-  const DecArgs a = dec_hold<0, 4>(args);
+  const DecArgs a = dec_hold(args);
   const int lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int hkv = (int)blockIdx.y, b = (int)blockIdx.z, bh = b * (int)gridDim.y + hkv, n, t0 = 0, t1 = 0;
@@ -555,7 +555,7 @@ __global__ __launch_bounds__(NW * 64, DP > 128 ? 1 : 2) void decode_wide_kernel(
   __shared__ u32 s_odd[kDecMaxTokens / 64][2];   // keys of the tiles of new rows whose value has an infinity or a NaN
   __shared__ u32 s_tree[kDecMaxTokens][2];   // what each query token sees of a tile of new rows
   static_assert((2 + VB) * TILE >= NW * 16 * OST * 4, "16 rows of each wave's output");
-  const DecArgs a = dec_hold<0, 4>(args);
+  const DecArgs a = dec_hold(args);
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hh = lane >> 5;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const bool late = VB == 3 && wv >= 4;
@@ -1044,7 +1044,7 @@ __global__ __launch_bounds__(256) void decode_join_kernel(const DecJoinArgs args
   constexpr int LPR = DP / 4, NG = 256 / LPR, PF = 4;   // threads on a slot, groups of them; loads in flight
   __shared__ float sm[16][16], sl[16][16], bias[16];
   __shared__ f32x4 so[NG * LPR];
-  const DecJoinArgs a = dec_hold<0, 4>(args);
+  const DecJoinArgs a = dec_hold(args);
   const int tid = threadIdx.x, hkv = (int)blockIdx.y, b = (int)blockIdx.z, bh = b * (int)gridDim.y + hkv;
   const int n = __builtin_amdgcn_readfirstlane(min(max(a.length[bh], 0), a.C));
   const int RS = a.RS;
@@ -1220,7 +1220,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void decode_replay_kernel(co
   __shared__ __attribute__((aligned(16))) float lse[4 * CH], weight[4 * CH];   // a row's, and log2 of w
   __shared__ int place[4 * CH], node[4 * CH];   // a row's index on the path, and its token
   __shared__ float s_sum[2][4][32];        // a tile's sums of the waves' rows
-  const DecReplayArgs a = dec_hold<0, 4>(args);
+  const DecReplayArgs a = dec_hold(args);
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, lq = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   int hkv = (int)blockIdx.y, b = (int)blockIdx.z, bh = b * (int)gridDim.y + hkv, n, t0 = 0, t1 = 0;
